@@ -218,6 +218,72 @@ typedef struct eux_gemm_desc {
 EUX_API int eux_gemm_launch(const eux_gemm_desc* d, void* stream);
 EUX_API int eux_gemm_num_sms(void);
 
+/* ---- choice of experts from router logits (moe_route.cu) ---- */
+#define EUX_ROUTE_MAX_EXPERTS 1024
+typedef struct eux_route_desc {
+  const void* logits;    /* [n_tokens, n_experts], rows logits_stride elements apart, f32 or bf16 */
+  const float* bias;     /* [n_experts], added to a score for the choice only; may be NULL */
+  int32_t* topk_idx;     /* out [n_tokens, topk]: expert, -1 where none is left */
+  float* topk_w;         /* out [n_tokens, topk] */
+  int64_t logits_stride;
+  int32_t n_tokens, n_experts, topk;
+  int32_t dtype;         /* EUX_DT_F32 or EUX_DT_BF16 */
+  int32_t sigmoid;       /* 0: softmax over the experts */
+  int32_t groups;        /* equal runs of experts; 1: none */
+  int32_t topk_groups;   /* runs that are kept */
+  int32_t renormalize;   /* weights divided by their sum */
+  float scale;
+  int32_t reserved0;
+} eux_route_desc;
+EUX_API int eux_route_launch(const eux_route_desc* d, void* stream);
+EUX_API int eux_route_preload(void);
+
+/* ---- a whole expert layer for a few tokens (moe_experts.cu) ----
+ * out[t] = sum_k topk_w[t,k] * W_down[e] (silu(W_gate[e] x[t]) * (W_up[e] x[t])), e = topk_idx[t,k]; entries with e outside
+ * [0, n_experts) add nothing. Two launches; topk_idx and topk_w are read by both. */
+#define EUX_EXPERTS_MAX_TOKENS 128
+#define EUX_EXPERTS_MAX_EXPERTS 1024
+typedef struct eux_experts_desc {
+  const void* x;               /* [n_tokens, hidden] bf16, rows x_stride elements apart */
+  const int32_t* topk_idx;     /* [n_tokens, topk] */
+  const float* topk_w;         /* [n_tokens, topk] */
+  void* out;                   /* [n_tokens, hidden] bf16, rows out_stride elements apart; may be x */
+  const void* w_gate_up;       /* [n_experts, 2 * inner, hidden]: gate rows, then up rows */
+  const void* w_down;          /* [n_experts, hidden, inner] */
+  const float* gate_up_scale;  /* fp8: [n_experts, ceil(2 * inner / 128), ceil(hidden / 128)] */
+  const float* down_scale;     /* fp8: [n_experts, ceil(hidden / 128), ceil(inner / 128)] */
+  void* workspace;             /* eux_experts_workspace_bytes, of this call alone until it ends */
+  uint32_t* counters;          /* eux_experts_counter_words, zero on entry, zero on exit */
+  uint32_t* status;
+  int64_t x_stride, out_stride;
+  uint64_t wait_timeout_ns;
+  int32_t n_tokens, hidden, inner, n_experts, topk;
+  int32_t fp8;                 /* 0: bf16 weights; 1: e4m3 weights with one fp32 scale per 128 x 128 block */
+} eux_experts_desc;
+EUX_API int eux_experts_launch(const eux_experts_desc* d, void* stream);
+EUX_API size_t eux_experts_workspace_bytes(const eux_experts_desc* d);
+EUX_API size_t eux_experts_counter_words(const eux_experts_desc* d);
+EUX_API int eux_experts_preload(void);
+
+/* ---- low-rank adapters of many requests (lora.cu): out[t] = y[t] + scale[i] * B[i] (A[i] x[t]), i = ids[t] ---- */
+#define EUX_LORA_MAX_RANK 128
+typedef struct eux_lora_desc {
+  const void* x;        /* [n_tokens, k] bf16, rows x_stride elements apart */
+  const int32_t* ids;   /* [n_tokens]: outside [0, n_adapters) a token has no adapter, out = y */
+  const void* y;        /* [n_tokens, n] bf16, rows y_stride elements apart */
+  void* out;            /* [n_tokens, n] bf16, rows out_stride elements apart; may be y */
+  const void* a;        /* [n_adapters, rank, k] bf16 */
+  const void* b;        /* [n_adapters, n, rank] bf16 */
+  const float* scale;   /* [n_adapters] */
+  void* workspace;      /* eux_lora_workspace_bytes, of this call alone until it ends */
+  int64_t x_stride, y_stride, out_stride;
+  int32_t n_tokens, k, n, rank, n_adapters;
+  int32_t reserved0;
+} eux_lora_desc;
+EUX_API int eux_lora_launch(const eux_lora_desc* d, void* stream);
+EUX_API size_t eux_lora_workspace_bytes(const eux_lora_desc* d);
+EUX_API int eux_lora_preload(void);
+
 #ifdef __cplusplus
 }
 #endif

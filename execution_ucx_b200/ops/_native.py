@@ -72,6 +72,32 @@ class GemmDesc(C.Structure):
     ]
 
 
+class RouteDesc(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("bias", C.c_void_p), ("topk_idx", C.c_void_p), ("topk_w", C.c_void_p), ("logits_stride", C.c_int64),
+        ("n_tokens", C.c_int32), ("n_experts", C.c_int32), ("topk", C.c_int32), ("dtype", C.c_int32), ("sigmoid", C.c_int32),
+        ("groups", C.c_int32), ("topk_groups", C.c_int32), ("renormalize", C.c_int32), ("scale", C.c_float), ("reserved0", C.c_int32),
+    ]
+
+
+class ExpertsDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("topk_idx", C.c_void_p), ("topk_w", C.c_void_p), ("out", C.c_void_p), ("w_gate_up", C.c_void_p),
+        ("w_down", C.c_void_p), ("gate_up_scale", C.c_void_p), ("down_scale", C.c_void_p), ("workspace", C.c_void_p),
+        ("counters", C.c_void_p), ("status", C.c_void_p), ("x_stride", C.c_int64), ("out_stride", C.c_int64),
+        ("wait_timeout_ns", C.c_uint64), ("n_tokens", C.c_int32), ("hidden", C.c_int32), ("inner", C.c_int32),
+        ("n_experts", C.c_int32), ("topk", C.c_int32), ("fp8", C.c_int32),
+    ]
+
+
+class LoraDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("ids", C.c_void_p), ("y", C.c_void_p), ("out", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p),
+        ("scale", C.c_void_p), ("workspace", C.c_void_p), ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("out_stride", C.c_int64),
+        ("n_tokens", C.c_int32), ("k", C.c_int32), ("n", C.c_int32), ("rank", C.c_int32), ("n_adapters", C.c_int32), ("reserved0", C.c_int32),
+    ]
+
+
 # The same layouts for one pack call per launch: setting the fields of a ctypes structure one by one costs more host
 # time than the launch itself. The launch functions take the packed bytes where they take a pointer to the structure.
 XFER_HEAD = struct.Struct("<QQQiiifii")
@@ -79,6 +105,10 @@ XFER_DIMS = struct.Struct("<8q8q")
 XFER_TAIL = struct.Struct("<8Q")
 MOE_DESC = struct.Struct("<8i12Q")
 GEMM_DESC = struct.Struct("<7Q4i6Q2i")
+ROUTE_DESC = struct.Struct("<4Qq8ifi")
+EXPERTS_DESC = struct.Struct("<11Q2qQ6i")
+LORA_DESC = struct.Struct("<8Q3q6i")
+assert ROUTE_DESC.size == C.sizeof(RouteDesc) and EXPERTS_DESC.size == C.sizeof(ExpertsDesc) and LORA_DESC.size == C.sizeof(LoraDesc)
 assert XFER_HEAD.size + XFER_DIMS.size + XFER_TAIL.size == C.sizeof(XferDesc)
 assert MOE_DESC.size == C.sizeof(MoeDesc) and GEMM_DESC.size == C.sizeof(GemmDesc)
 
@@ -130,6 +160,11 @@ def load():
     lib.eux_moe_dispatch_launch.argtypes = [P, I, P]
     lib.eux_moe_expert_ready_launch.argtypes = [P, P]
     lib.eux_moe_combine_launch.argtypes = [P, I, P]
+    for op in ("route", "experts", "lora"):
+        getattr(lib, f"eux_{op}_launch").argtypes = [P, P]
+    for size in ("eux_experts_workspace_bytes", "eux_experts_counter_words", "eux_lora_workspace_bytes"):
+        getattr(lib, size).argtypes = [P]
+        getattr(lib, size).restype = C.c_size_t
     if hasattr(lib, "eux_gemm_launch"):
         lib.eux_gemm_launch.argtypes = [P, P]
         lib.eux_gemm_num_sms.argtypes = []
@@ -152,7 +187,7 @@ def _preload(lib) -> None:
             return
     except Exception:
         return
-    for fn in ("eux_xfer_preload", "eux_moe_preload", "eux_gemm_preload"):
+    for fn in ("eux_xfer_preload", "eux_moe_preload", "eux_gemm_preload", "eux_route_preload", "eux_experts_preload", "eux_lora_preload"):
         if hasattr(lib, fn):
             getattr(lib, fn)()
 

@@ -1,0 +1,101 @@
+"""What the operators that are called like a layer share: checks of arguments, the launch on a tensor's own device, and
+zeroed words for kernels that count their CTAs."""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+
+
+def require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def require_rows(t: torch.Tensor, name: str, dtype, cols=None, rows=None) -> None:
+    """A matrix whose rows the kernels can read in 16-byte pieces: unit inner stride, rows and base on 16 bytes, rows that
+    do not overlap."""
+    require(isinstance(t, torch.Tensor) and t.dim() == 2, f"{name} must be a matrix")
+    require(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
+    require(cols is None or t.shape[1] == cols, f"{name} must have {cols} columns, not {t.shape[1]}")
+    require(rows is None or t.shape[0] == rows, f"{name} must have {rows} rows, not {t.shape[0]}")
+    unit = 16 // t.element_size()
+    if t.numel():
+        require(t.shape[1] == 1 or t.stride(1) == 1, f"{name} must have its columns side by side")
+        require(t.shape[0] == 1 or (t.stride(0) % unit == 0 and t.stride(0) >= t.shape[1]), f"{name} must have rows {unit} elements aligned and apart")
+        require(t.data_ptr() % 16 == 0, f"{name} must begin on 16 bytes")
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """The distance of rows; any will do where there is one row."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def require_dense(t: torch.Tensor, name: str, dtype, shape) -> None:
+    require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), f"{name} must have the shape {tuple(shape)}")
+    require(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
+    require(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def require_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None:
+            require(t.device == device, f"{name} is on {t.device}, not on {device}")
+
+
+def require_cuda(device) -> None:
+    require(device.type == "cuda", f"the kernels run on a CUDA device, not on {device}")
+
+
+class on_device:
+    """The given device as the current one, and its current stream: ``with on_device(d) as stream``."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
+class CallCounters:
+    """Zeroed words for calls of a kernel that leaves them zeroed. Calls that may run at the same time get words of their
+    own: those of one stream share some, and every captured call has its own, since graphs may be replayed beside each
+    other and beside plain calls."""
+
+    SLOTS = 16
+
+    def __init__(self, words: int, device):
+        self.words, self.device = words, device
+        self._of_stream = {}
+        self._kept = []
+        with on_device(device):
+            self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0))
+            torch.cuda.current_stream().synchronize()  # captured calls run on any stream
+
+    def get(self, stream: int) -> torch.Tensor:
+        if torch.cuda.is_current_stream_capturing():
+            # zeroed by the graph itself once the words that were zeroed beforehand are given out
+            t = self._spare.pop() if self._spare else torch.zeros(self.words, dtype=torch.int32, device=self.device)
+            self._kept.append(t)
+            return t
+        t = self._of_stream.get(stream)
+        if t is None:
+            t = self._of_stream[stream] = torch.zeros(self.words, dtype=torch.int32, device=self.device)
+        return t
+
+    def reset(self) -> None:
+        """Zeroes all words, after a kernel that gave up: with nothing in flight."""
+        for t in [*self._of_stream.values(), *self._kept]:
+            t.zero_()
+
+
+def check(rc: int, what: str) -> None:
+    if rc:
+        _native.check(rc, what)

@@ -1,0 +1,86 @@
+"""Low-rank adapters of many requests at once, beside a shared projection (see ``csrc/kernels/lora.cu``).
+
+``RemoteGemm`` and its block-scaled forms multiply every token with the one weight that a worker serves. ``LoraAdapters``
+adds what is each request's own: ``out[t] = y[t] + scale[i] * B[i] (A[i] x[t])``, ``i = ids[t]``, for tokens of any
+requests in any order, ``y`` being what the shared projection gave.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _native
+from . import _workspace as ws
+
+_launches = 0
+
+
+def launch_count() -> int:
+    return _launches
+
+
+class LoraAdapters:
+    """The adapters of one projection: ``a`` ``[adapters, rank, K]`` and ``b`` ``[adapters, N, rank]``, bfloat16, and ``scale``
+    ``[adapters]``, float32 (1 if not given). They are used where they lie: the object keeps the tensors and copies nothing, so
+    an adapter that is written into its place holds for the next call. ``rank`` is a multiple of 8 up to 128, K and N are
+    multiples of 8."""
+
+    MAX_RANK = 128
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: Optional[torch.Tensor] = None):
+        ws.require(isinstance(a, torch.Tensor) and a.dim() == 3, "a must be [adapters, rank, K]")
+        ws.require(isinstance(b, torch.Tensor) and b.dim() == 3, "b must be [adapters, N, rank]")
+        self.n_adapters, self.rank, self.K = a.shape
+        self.N = b.shape[1]
+        ws.require(self.n_adapters >= 1, "there must be an adapter")
+        ws.require(8 <= self.rank <= self.MAX_RANK and self.rank % 8 == 0, f"the rank must be a multiple of 8 up to {self.MAX_RANK}, not {self.rank}")
+        ws.require(self.K > 0 and self.N > 0 and self.K % 8 == 0 and self.N % 8 == 0, f"K and N must be multiples of 8, not {self.K} and {self.N}")
+        ws.require_dense(a, "a", torch.bfloat16, (self.n_adapters, self.rank, self.K))
+        ws.require_dense(b, "b", torch.bfloat16, (self.n_adapters, self.N, self.rank))
+        if scale is not None:
+            ws.require_dense(scale, "scale", torch.float32, (self.n_adapters,))
+        self.device = a.device
+        ws.require_device(self.device, b=b, scale=scale)
+        ws.require_cuda(self.device)
+        ws.require((a.data_ptr() | b.data_ptr()) % 16 == 0, "a and b must begin on 16 bytes")
+        self.a, self.b = a, b
+        self.scale = scale if scale is not None else torch.ones(self.n_adapters, dtype=torch.float32, device=self.device)
+        _native.load()
+
+    def __call__(self, x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``x`` is ``[tokens, K]`` and ``y`` ``[tokens, N]``, bfloat16; ``ids`` ``[tokens]``, int32, names each token's adapter. A
+        token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``; the rows
+        of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
+        global _launches
+        ws.require_rows(x, "x", torch.bfloat16, cols=self.K)
+        t = x.shape[0]
+        ws.require_rows(y, "y", torch.bfloat16, cols=self.N, rows=t)
+        ws.require_dense(ids, "ids", torch.int32, (t,))
+        if out is not None:
+            ws.require_rows(out, "out", torch.bfloat16, cols=self.N, rows=t)
+        ws.require_device(self.device, x=x, ids=ids, y=y, out=out)
+        if out is None:
+            out = torch.empty(t, self.N, dtype=torch.bfloat16, device=self.device)
+        if t == 0:
+            return out
+        lib = _native.load()
+        desc = lambda workspace: _native.descriptor(  # noqa: E731
+            _native.LORA_DESC, _native.LoraDesc, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), self.a.data_ptr(), self.b.data_ptr(),
+            self.scale.data_ptr(), workspace, ws.row_stride(x), ws.row_stride(y), ws.row_stride(out), t, self.K, self.N, self.rank,
+            self.n_adapters, 0)
+        with ws.on_device(self.device) as stream:
+            workspace = torch.empty(lib.eux_lora_workspace_bytes(desc(0)), dtype=torch.uint8, device=self.device)
+            ws.check(lib.eux_lora_launch(desc(workspace.data_ptr()), stream), "eux_lora_launch")
+        _launches += 1
+        return out
+
+
+def reference(x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """Plain PyTorch statement in 64 bits."""
+    out = y.double().clone()
+    for i in range(a.shape[0]):
+        rows = (ids == i).nonzero().squeeze(1)
+        if rows.numel():
+            out[rows] += scale[i].double() * ((x[rows].double() @ a[i].double().t()) @ b[i].double().t())
+    return out

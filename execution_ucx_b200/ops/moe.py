@@ -5,14 +5,19 @@
 peer-mapped. ``dispatch`` routes and pushes rows to the expert ranks,
 ``expert_ready`` is where an expert GEMM would run (identity here) and
 ``combine`` pulls the rows back with the gate-weighted sum fused into the read.
+
+``route`` chooses the experts (``csrc/kernels/moe_route.cu``) and ``MoeExperts`` is
+what they compute (``csrc/kernels/moe_experts.cu``): the whole layer of a few tokens
+whose experts are on this GPU, or the experts of rows that a dispatch has brought.
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 
 from . import _native
+from . import _workspace as ws
 from ..parallel.peer import PeerGroup, SymmetricBuffer
 
 _launches = 0
@@ -140,3 +145,158 @@ def reference_dispatch_combine(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: 
     valid = (topk_idx >= 0).float()
     wsum = (topk_w * valid).sum(-1, keepdim=True)
     return xf * wsum
+
+
+# ---- choice of experts ---------------------------------------------------
+
+ROUTE_MAX_EXPERTS = 1024
+
+
+def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+          topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The ``topk`` experts of each token and their weights, as ``MoeAllToAll.dispatch`` and ``MoeExperts`` take them:
+    int32 and float32, both ``[tokens, topk]``, largest score first, ties to the lowest expert.
+
+    ``logits`` is ``[tokens, experts]``, float32 or bfloat16; its rows may lie apart. Scores are the softmax over all
+    experts or the sigmoid of each. ``bias`` (float32, ``[experts]``) is added for the choice and left out of the weights.
+    With ``groups`` the experts are that many equal runs, and only those of the ``topk_groups`` runs with the largest sum
+    of two scores are chosen from. ``renormalize`` divides a token's weights by their sum (a sum of zero gives weights of
+    zero), ``scale`` multiplies them. An expert whose logit or bias is -inf or NaN is never chosen; where fewer than
+    ``topk`` are left, the last places are expert -1 with weight 0. A logit of +inf weighs as the largest number does."""
+    global _launches
+    ws.require(isinstance(logits, torch.Tensor) and logits.dim() == 2, "logits must be a matrix")
+    ws.require(logits.dtype in (torch.float32, torch.bfloat16), f"logits must be float32 or bfloat16, not {logits.dtype}")
+    t, e = logits.shape
+    ws.require(1 <= e <= ROUTE_MAX_EXPERTS, f"there must be 1 to {ROUTE_MAX_EXPERTS} experts, not {e}")
+    ws.require(e == 1 or logits.stride(1) == 1, "a token's logits must lie side by side")
+    ws.require(1 <= topk <= min(32, e), f"topk must be 1 to {min(32, e)}, not {topk}")
+    ws.require(scoring in ("softmax", "sigmoid"), f"scoring must be softmax or sigmoid, not {scoring!r}")
+    ws.require(1 <= groups <= 32 and e % groups == 0, f"{e} experts are not {groups} groups (of up to 32)")
+    ws.require(1 <= topk_groups <= groups, f"topk_groups must be 1 to {groups}, not {topk_groups}")
+    if bias is not None:
+        ws.require_dense(bias, "bias", torch.float32, (e,))
+    device = logits.device
+    ws.require_device(device, bias=bias)
+    ws.require_cuda(device)
+    idx = torch.empty(t, topk, dtype=torch.int32, device=device)
+    w = torch.empty(t, topk, dtype=torch.float32, device=device)
+    if t:
+        desc = _native.descriptor(_native.ROUTE_DESC, _native.RouteDesc, logits.data_ptr(), bias.data_ptr() if bias is not None else 0,
+                                  idx.data_ptr(), w.data_ptr(), ws.row_stride(logits), t, e, topk, _native.torch_dtype_code(logits.dtype),
+                                  int(scoring == "sigmoid"), groups, topk_groups, int(renormalize), float(scale), 0)
+        with ws.on_device(device) as stream:
+            ws.check(_native.load().eux_route_launch(desc, stream), "eux_route_launch")
+        _launches += 1
+    return idx, w
+
+
+# ---- the experts ------------------------------------------------------------
+
+class MoeExperts:
+    """The experts of one GPU: ``out[t] = sum_k w[t,k] * W_down[e] (silu(W_gate[e] x[t]) * (W_up[e] x[t]))``, ``e = idx[t,k]``.
+
+    ``w_gate_up`` is ``[experts, 2 * inner, hidden]`` (gate rows, then up rows) and ``w_down`` ``[experts, hidden, inner]``,
+    both bfloat16, or both float8_e4m3fn with float32 scales of 128 x 128 blocks: ``gate_up_scale`` ``[experts,
+    ceil(2 * inner / 128), ceil(hidden / 128)]`` and ``down_scale`` ``[experts, ceil(hidden / 128), ceil(inner / 128)]`` (what
+    ``remote_gemm.quantize_blocks_128x128`` gives for each expert). They are used where they lie: the object keeps the tensors
+    and copies nothing, so what is written into them holds for the next call. ``hidden`` and ``inner`` are multiples of 8
+    (16 for e4m3).
+
+    Made for few tokens, where the layer is as fast as the weights of the named experts can be read: rows beyond
+    ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again."""
+
+    MAX_TOKENS = 128
+    MAX_EXPERTS = 1024
+
+    def __init__(self, w_gate_up: torch.Tensor, w_down: torch.Tensor, gate_up_scale: Optional[torch.Tensor] = None,
+                 down_scale: Optional[torch.Tensor] = None):
+        for name, w in (("w_gate_up", w_gate_up), ("w_down", w_down)):
+            ws.require(isinstance(w, torch.Tensor) and w.dim() == 3, f"{name} must be [experts, rows, columns]")
+        self.n_experts, self.hidden, self.inner = e, h, i = w_down.shape
+        dtype = w_down.dtype
+        ws.require(dtype in (torch.bfloat16, torch.float8_e4m3fn), f"weights must be bfloat16 or float8_e4m3fn, not {dtype}")
+        self.fp8 = dtype == torch.float8_e4m3fn
+        unit = 16 if self.fp8 else 8
+        ws.require(1 <= e <= self.MAX_EXPERTS, f"there must be 1 to {self.MAX_EXPERTS} experts, not {e}")
+        ws.require(h > 0 and i > 0 and h % unit == 0 and i % unit == 0, f"hidden and inner must be multiples of {unit}, not {h} and {i}")
+        ws.require_dense(w_gate_up, "w_gate_up", dtype, (e, 2 * i, h))
+        ws.require_dense(w_down, "w_down", dtype, (e, h, i))
+        blocks = lambda n: -(-n // 128)  # noqa: E731
+        ws.require((gate_up_scale is not None) == self.fp8 and (down_scale is not None) == self.fp8, "float8_e4m3fn weights have scales, bfloat16 weights none")
+        if self.fp8:
+            ws.require_dense(gate_up_scale, "gate_up_scale", torch.float32, (e, blocks(2 * i), blocks(h)))
+            ws.require_dense(down_scale, "down_scale", torch.float32, (e, blocks(h), blocks(i)))
+        self.device = w_down.device
+        ws.require_device(self.device, w_gate_up=w_gate_up, gate_up_scale=gate_up_scale, down_scale=down_scale)
+        ws.require_cuda(self.device)
+        ws.require((w_gate_up.data_ptr() | w_down.data_ptr()) % 16 == 0, "weights must begin on 16 bytes")
+        self.w_gate_up, self.w_down, self.gate_up_scale, self.down_scale = w_gate_up, w_down, gate_up_scale, down_scale
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        words = _native.load().eux_experts_counter_words(self._desc(self.MAX_TOKENS, 1))
+        self._counters = ws.CallCounters(int(words), self.device)
+
+    def _desc(self, tokens, topk, x=0, idx=0, w=0, out=0, workspace=0, counters=0, x_stride=0, out_stride=0):
+        """An ``eux_experts_desc`` of one pass."""
+        return _native.descriptor(
+            _native.EXPERTS_DESC, _native.ExpertsDesc, x, idx, w, out, self.w_gate_up.data_ptr(), self.w_down.data_ptr(),
+            self.gate_up_scale.data_ptr() if self.fp8 else 0, self.down_scale.data_ptr() if self.fp8 else 0, workspace, counters,
+            self.status.data_ptr(), x_stride, out_stride, 2_000_000_000, tokens, self.hidden, self.inner, self.n_experts, topk, int(self.fp8))
+
+    def __call__(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``x`` is ``[tokens, hidden]`` bfloat16, ``topk_idx`` (int32) and ``topk_w`` (float32) are ``[tokens, topk]``, up to 32
+        per token. An entry whose expert is not in ``[0, experts)`` adds nothing: with the experts of one of several GPUs, pass
+        the indices less the number of its first expert, and add up the GPUs' results. A token without entries gets zeros.
+        ``out`` may be ``x`` itself; the rows of both may lie apart. Sums are in float32; what lies between the two products is
+        rounded to bfloat16. The same arguments give the same bits."""
+        global _launches
+        ws.require_rows(x, "x", torch.bfloat16, cols=self.hidden)
+        t = x.shape[0]
+        ws.require(isinstance(topk_idx, torch.Tensor) and topk_idx.dim() == 2 and topk_idx.shape[0] == t, f"topk_idx must be [{t}, topk]")
+        topk = topk_idx.shape[1]
+        ws.require(1 <= topk <= 32, f"topk must be 1 to 32, not {topk}")
+        ws.require_dense(topk_idx, "topk_idx", torch.int32, (t, topk))
+        ws.require_dense(topk_w, "topk_w", torch.float32, (t, topk))
+        if out is not None:
+            ws.require_rows(out, "out", torch.bfloat16, cols=self.hidden, rows=t)
+        ws.require_device(self.device, x=x, topk_idx=topk_idx, topk_w=topk_w, out=out)
+        if out is None:
+            out = torch.empty(t, self.hidden, dtype=torch.bfloat16, device=self.device)
+        lib = _native.load()
+        xs, os_ = ws.row_stride(x), ws.row_stride(out)
+        with ws.on_device(self.device) as stream:
+            counters = self._counters.get(stream)
+            for first in range(0, t, self.MAX_TOKENS):
+                n = min(self.MAX_TOKENS, t - first)
+                need = lib.eux_experts_workspace_bytes(self._desc(n, topk))
+                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+                desc = self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk, topk_w.data_ptr() + 4 * first * topk,
+                                  out.data_ptr() + 2 * first * os_, workspace.data_ptr(), counters.data_ptr(), xs, os_)
+                ws.check(lib.eux_experts_launch(desc, stream), "eux_experts_launch")
+                _launches += 2
+        return out
+
+    def check_status(self) -> None:
+        s = int(self.status.item())
+        if s:
+            self._counters.reset()
+            self.status.zero_()
+            raise RuntimeError(f"moe experts status code={s & 0xff} where={s >> 8}")
+
+
+def reference_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor,
+                      gate_up_scale: Optional[torch.Tensor] = None, down_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Plain PyTorch statement of the experts in 64 bits."""
+    def full(w, scale):
+        w = w.double()
+        if scale is None:
+            return w
+        return w * scale.double().repeat_interleave(128, 0)[:w.shape[0]].repeat_interleave(128, 1)[:, :w.shape[1]]
+    e, h, i = w_down.shape
+    out = torch.zeros(x.shape[0], h, dtype=torch.float64, device=x.device)
+    for j in range(e):
+        tok, slot = (topk_idx == j).nonzero(as_tuple=True)
+        if tok.numel():
+            gu = x[tok].double() @ full(w_gate_up[j], None if gate_up_scale is None else gate_up_scale[j]).t()
+            y = (torch.nn.functional.silu(gu[:, :i]) * gu[:, i:]) @ full(w_down[j], None if down_scale is None else down_scale[j]).t()
+            out.index_add_(0, tok, y * topk_w[tok, slot].double().unsqueeze(1))
+    return out

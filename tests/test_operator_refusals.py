@@ -1,0 +1,94 @@
+"""What the choice of experts, the expert layer and the adapters refuse, before anything runs on a GPU."""
+import pytest
+import torch
+
+
+def test_route_refuses():
+    from execution_ucx_b200.ops import moe
+    ok = torch.randn(4, 16)
+    for bad, match in [(dict(logits=ok[0]), "matrix"), (dict(logits=ok.half()), "float32 or bfloat16"), (dict(logits=torch.randn(2, 1025)), "1 to 1024"),
+                       (dict(logits=torch.randn(16, 4).t()), "side by side"), (dict(topk=0), "topk"), (dict(topk=17), "topk"),
+                       (dict(logits=torch.randn(2, 40), topk=33), "topk"), (dict(scoring="relu"), "scoring"), (dict(groups=3), "groups"),
+                       (dict(groups=0), "groups"), (dict(groups=4, topk_groups=5), "topk_groups"), (dict(groups=4, topk_groups=0), "topk_groups"),
+                       (dict(bias=torch.zeros(15)), "bias"), (dict(bias=torch.zeros(16).double()), "bias"), (dict(bias=torch.zeros(32)[::2]), "contiguous"),
+                       (dict(logits=torch.randn(2, 0)), "experts"), (dict(), "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            moe.route(**{"logits": ok, "topk": 4, **bad})
+
+
+def test_experts_refuse():
+    from execution_ucx_b200.ops import moe
+    gu, down = torch.zeros(2, 32, 16, dtype=torch.bfloat16), torch.zeros(2, 16, 16, dtype=torch.bfloat16)
+    f8 = torch.float8_e4m3fn
+    s = torch.ones(2, 1, 1)
+    for args, match in [((gu[0], down), "w_gate_up"), ((gu, down[0]), "w_down"), ((gu.half(), down.half()), "bfloat16 or float8"), ((gu.float(), down), "w_gate_up"),
+                        ((gu[:, :30], down), "shape"), ((gu[:1], down), "shape"), ((gu.transpose(1, 2), down.transpose(1, 2)), "shape"),
+                        ((torch.zeros(2, 24, 16, dtype=torch.bfloat16), torch.zeros(2, 16, 12, dtype=torch.bfloat16)), "multiples of 8"),
+                        ((gu, down, s, s), "scales"), ((gu.to(f8), down.to(f8)), "scales"), ((gu.to(f8), down.to(f8), s, None), "scales"),
+                        ((gu.to(f8), down.to(f8), s, torch.ones(2, 1, 2)), "down_scale"), ((gu.to(f8), down.to(f8), s.double(), s), "gate_up_scale"),
+                        ((torch.zeros(2, 48, 16).to(f8), torch.zeros(2, 16, 24).to(f8), s, s), "multiples of 16"),
+                        ((torch.zeros(2, 32, 32, dtype=torch.bfloat16)[:, :, ::2], down), "contiguous"), ((torch.zeros(0, 32, 16, dtype=torch.bfloat16), down[:0]), "experts"),
+                        ((gu, down), "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            moe.MoeExperts(*args)
+
+
+def test_adapters_refuse():
+    from execution_ucx_b200.ops import lora
+    a, b = torch.zeros(3, 16, 32, dtype=torch.bfloat16), torch.zeros(3, 24, 16, dtype=torch.bfloat16)
+    for args, match in [((a[0], b), "a must be"), ((a, b[0]), "b must be"), ((a.half(), b), "a must be"), ((a, b.float()), "b must be"), ((a, b[:2]), "shape"),
+                        ((a[:, :12], b[:, :, :12]), "rank"), ((torch.zeros(1, 136, 32, dtype=torch.bfloat16), torch.zeros(1, 24, 136, dtype=torch.bfloat16)), "rank"),
+                        ((a[:, :, :20], b), "multiples of 8"), ((a, b[:, :20]), "multiples of 8"), ((a, b, torch.ones(2)), "scale"), ((a, b, torch.ones(3).double()), "scale"),
+                        ((a[:, :, :24], b), "contiguous"), ((a[:0], b[:0]), "adapter"), ((a, b), "CUDA")]:
+        with pytest.raises(ValueError, match=match):
+            lora.LoraAdapters(*args)
+
+
+def test_launches_refuse_without_a_gpu(native_build):
+    """The C entry points check what they are given before the first CUDA call."""
+    import ctypes as C
+    from execution_ucx_b200.ops import _native as n
+    lib = n.load()
+    bad = 100001
+    for launch, size in ((lib.eux_route_launch, None), (lib.eux_experts_launch, lib.eux_experts_workspace_bytes), (lib.eux_lora_launch, lib.eux_lora_workspace_bytes)):
+        assert launch(None, None) == bad
+        assert size is None or size(None) == 0
+    good = dict(n_tokens=2, n_experts=16, topk=2, dtype=n.DT_F32, groups=1, topk_groups=1)
+    for change in (dict(n_experts=0), dict(n_experts=1025), dict(topk=17), dict(topk=33, n_experts=64), dict(groups=3), dict(groups=2, topk_groups=3), dict(dtype=n.DT_F16),
+                   dict(n_tokens=-1), dict()):
+        assert lib.eux_route_launch(C.byref(n.RouteDesc(**{**good, **change})), None) == bad   # the last: no pointers
+    assert lib.eux_route_launch(C.byref(n.RouteDesc(**{**good, "n_tokens": 0})), None) == 0
+    good = dict(n_tokens=2, hidden=64, inner=32, n_experts=4, topk=2)
+    for change in (dict(n_tokens=129), dict(n_tokens=-1), dict(hidden=0), dict(hidden=60), dict(inner=33), dict(inner=24, fp8=1), dict(n_experts=0), dict(topk=0), dict(topk=33),
+                   dict(x_stride=4), dict(out_stride=-4), dict()):
+        assert lib.eux_experts_launch(C.byref(n.ExpertsDesc(**{**good, **change})), None) == bad
+    assert lib.eux_experts_launch(C.byref(n.ExpertsDesc(**{**good, "n_tokens": 0})), None) == 0
+    assert lib.eux_experts_workspace_bytes(C.byref(n.ExpertsDesc(**good))) > 0
+    good = dict(n_tokens=2, k=64, n=32, rank=16, n_adapters=2)
+    for change in (dict(n_tokens=-1), dict(k=60), dict(n=0), dict(rank=4), dict(rank=136), dict(rank=20), dict(n_adapters=0), dict(y_stride=2), dict()):
+        assert lib.eux_lora_launch(C.byref(n.LoraDesc(**{**good, **change})), None) == bad
+    assert lib.eux_lora_launch(C.byref(n.LoraDesc(**{**good, "n_tokens": 0})), None) == 0
+
+
+@pytest.mark.gpu
+def test_calls_refuse(cuda_device):
+    from execution_ucx_b200.ops import lora, moe
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=cuda_device)  # noqa: E731
+    layer = moe.MoeExperts(z(2, 32, 16), z(2, 16, 16))
+    x, idx, w = z(4, 16), z(4, 2, dt=torch.int32), z(4, 2, dt=torch.float32)
+    layer(x, idx, w)
+    for args, kw, match in [((x.half(), idx, w), {}, "x must be"), ((z(4, 24), idx, w), {}, "columns"), ((x, idx.long(), w), {}, "topk_idx"), ((x, idx, w.half()), {}, "topk_w"),
+                            ((x, idx[:3], w), {}, "topk_idx"), ((x, idx, w[:, :1]), {}, "topk_w"), ((x, z(4, 0, dt=torch.int32), w), {}, "topk"),
+                            ((x, z(4, 33, dt=torch.int32), z(4, 33, dt=torch.float32)), {}, "topk"), ((z(16, 4).t(), idx, w), {}, "side by side"), ((z(4, 20)[:, :16], idx, w), {}, "aligned"),
+                            ((z(4, 32)[:, 4:20], idx, w), {}, "16 bytes"), ((x, z(2, 4, dt=torch.int32).t(), w), {}, "contiguous"), ((x, idx, w), dict(out=z(3, 16)), "rows"),
+                            ((x, idx, w), dict(out=z(1, 16).expand(4, 16)), "apart"), ((x.cpu(), idx, w), {}, "is on"), ((x, idx.cpu(), w), {}, "is on")]:
+        with pytest.raises(ValueError, match=match):
+            layer(*args, **kw)
+    ad = lora.LoraAdapters(z(3, 16, 32), z(3, 24, 16))
+    x, ids, y = z(4, 32), z(4, dt=torch.int32), z(4, 24)
+    ad(x, ids, y)
+    for args, kw, match in [((x.float(), ids, y), {}, "x must be"), ((z(4, 40), ids, y), {}, "columns"), ((x, ids.long(), y), {}, "ids"), ((x, ids[:3], y), {}, "ids"),
+                            ((x, ids, z(4, 32)), {}, "columns"), ((x, ids, z(3, 24)), {}, "rows"), ((x, ids, y), dict(out=z(4, 24, dt=torch.float32)), "out"),
+                            ((x, z(8, dt=torch.int32)[::2], y), {}, "contiguous"), ((x, ids, y.cpu()), {}, "is on"), ((z(4, 40)[:, 4:36], ids, y), {}, "16 bytes")]:
+        with pytest.raises(ValueError, match=match):
+            ad(*args, **kw)
