@@ -1,9 +1,31 @@
-// A whole mixture-of-experts layer for a few tokens, in two launches:
+// A whole mixture-of-experts layer for a few tokens, in two launches of one kernel's two forms:
 //
-//   h_j = silu(W_gate[e] x_t) * (W_up[e] x_t)      for every entry j = (t, slot) whose expert e is here
-//   out_t = sum over the entries of t of w_j * (W_down[e] h_j)
+//   up:    h_j = silu(W_gate[e] x_t) * (W_up[e] x_t)   for every entry j = (t, slot) whose expert e is here
+//   down:  out_t = sum over the entries of t of w_j * (W_down[e] h_j)
 //
-// One warp per row of a weight and entry: 16 bytes per lane and step, sums in fp32.
+// What bounds it: the weights of the named experts have to come from HBM once, 2 (or 1) bytes for 2 operations per token of
+// the expert; everything else is small. So the kernel is a stream of weights with the products hung on:
+//
+// * The weights of a form are cut into segments, 128 rows of an expert by all of K (up: 64 gate rows and the 64 up rows that
+//   belong to them, with up to 64 of the expert's tokens), and these into blocks of 128 rows x 128 bytes, 16 KiB. All blocks of
+//   all segments stand in one line, and each SM gets the same number of them, one after the other: no SM has more to read
+//   than another, whatever the number of experts and their sizes. Where an SM's share begins or ends inside a tile of
+//   results, it leaves its part in a workspace, and the last to come adds the parts up, in the order of the SMs. For the down
+//   form a tile is 128 rows of the output with all experts, so the weighted sum over a token's experts is made in shared
+//   memory, and only what an SM's share cuts goes through the workspace.
+// * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp fetches the tokens' values beside them
+//   with cp.async (rows are gathered: any tokens, any order), eight warps multiply: four by rows, two by K. The ring runs on
+//   over the borders of segments; the down form's starts before the up form has ended (programmatic dependent launch), since
+//   weights wait for nobody.
+// * The weights are the first operand of mma.sync m16n8k16 and the tokens the second: 8 columns are the smallest padding for
+//   one token. At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks per block, of which
+//   eight tokens take about 130, so operands through registers cost nothing here, and they let e4m3 weights be multiplied with
+//   bfloat16 tokens: widened on the way, exactly (see widen).
+//
+// Sums are float32 throughout. h is rounded to bfloat16, which its product takes; its error, 2^-9 of each term on average, is
+// that of the result's own rounding.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "eux_bulk.cuh"
@@ -11,76 +33,585 @@
 
 namespace eux {
 
-constexpr int kExpertThreads = 256;
+constexpr int kXpWarps = 8;                         // that multiply
+constexpr int kXpConsumers = kXpWarps * 32;
+constexpr int kXpThreads = kXpConsumers + 64;       // and one that fetches weights, one that fetches tokens
+constexpr int kXpRows = 128;                        // rows of weights in a block
+constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
+constexpr int kXpMaxStages = 12;
+constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
+constexpr int kXpMaxGrid = 160;
+constexpr size_t kXpSmem = 227 * 1024;
+constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer cost more to add up than they save
 
-// The dot product of a weight row of n elements with n bf16 values, by a warp.
-template <bool FP8>
-__device__ __forceinline__ float row_dot(const void* w, const float* scale, const __nv_bfloat16* v, int n, int lane) {
-  float acc = 0.f;
-  for (int k = lane * 8; k < n; k += 256) {
-    const uint4 xv = *reinterpret_cast<const uint4*>(v + k);
-    const __nv_bfloat162* x2 = reinterpret_cast<const __nv_bfloat162*>(&xv);
-    float part = 0.f;
-    if (FP8) {
-      const uint2 wv = *reinterpret_cast<const uint2*>((const uint8_t*)w + k);
-      const __nv_fp8_e4m3* w8 = reinterpret_cast<const __nv_fp8_e4m3*>(&wv);
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = __bfloat1622float2(x2[i]);
-        part += float(w8[2 * i]) * a.x + float(w8[2 * i + 1]) * a.y;
-      }
-      acc += part * scale[k / 128];
+struct XpParams {
+  eux_experts_desc d;
+  __nv_bfloat16* h;      // [entries, inner]
+  float* part;           // [grid][2][part_rows][128]
+  int part_rows;
+  int cap;               // tokens of an expert that a segment takes at most
+  int stages;
+  int x_bytes;           // of a stage
+};
+
+// Shared memory behind the ring of weights, in bytes from its end.
+struct XpLayout {
+  int x, stage_sum, acc, scales, bars, tables, total;
+};
+__host__ __device__ inline XpLayout xp_layout(bool down, int stages, int x_bytes, int cap, int n_tokens, int n_experts, int entries) {
+  XpLayout l;
+  int at = stages * kXpBlock;
+  l.x = at, at += stages * x_bytes;
+  l.stage_sum = at, at += cap * kXpLd * 4;
+  l.acc = at, at += down ? n_tokens * kXpLd * 4 : 0;
+  l.scales = at, at += stages * 16;
+  l.bars = at, at += stages * 16;
+  l.tables = at, at += (n_experts + 1) * 8 + 16 + ((entries * 2 + 15) & ~15);
+  l.total = (at + 15) & ~15;
+  return l;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+               "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {  // what is not read is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {  // when this thread's copies so far have landed
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void lds_64(uint32_t& a, uint32_t& b, uint32_t at) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpConsumers) : "memory"); }
+
+// Two e4m3 values, bytes `lo` and `hi` of w as PRMT selectors have it, as bfloat16: sign, exponent and mantissa are moved to
+// their places, which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and
+// multiplied by 2^120. Both steps are exact. NaN (0x7f) would become 480: weights with NaN are refused when they are given.
+template <int SELECT>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  const uint32_t t = __byte_perm(w, 0, SELECT);  // the bytes on top of each half
+  const uint32_t v = (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+  const __nv_bfloat162 big = __floats2bfloat162_rn(0x1p120f, 0x1p120f);
+  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), big);
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// Which entries go to which expert, and the line of segments. The tables lie in shared memory and are the same in all CTAs:
+//   start[a]   where the entries of the a-th named expert begin in `order` (the experts in order, entries of one in order)
+//   first[a]   number of the first chunk (of up to `cap` entries) of that expert; first[named] is their number
+//   expert[a]
+struct XpTables {
+  int* start;        // [named + 1]
+  uint16_t* first;   // [named + 1]
+  uint16_t* expert;  // [named]
+  uint16_t* order;   // [entries]
+  int named;
+};
+
+struct XpSegment {
+  int expert, tile, pos, n;
+};
+
+__device__ __forceinline__ void xp_locate(const XpTables& r, int a, int chunk, XpSegment* s) {
+  const int count = r.start[a + 1] - r.start[a], chunks = r.first[a + 1] - r.first[a];
+  const int each = (count + chunks - 1) / chunks;
+  s->expert = r.expert[a];
+  s->pos = r.start[a] + chunk * each;
+  s->n = min(each, count - chunk * each);
+}
+
+// Segments one after the other; `a` is where the last one was found, which is near.
+template <bool DOWN>
+struct XpWalk {
+  const XpTables& r;
+  int tiles;  // up: row tiles of an expert
+  int a = 0;
+  __device__ XpWalk(const XpTables& r_, int tiles_) : r(r_), tiles(tiles_) {}
+  __device__ XpSegment at(int segment) {
+    XpSegment s;
+    const int all = r.first[r.named];
+    if (DOWN) {
+      s.tile = segment / all;
+      const int q = segment - s.tile * all;
+      if (q < r.first[a]) a = 0;
+      while (q >= r.first[a + 1]) ++a;
+      xp_locate(r, a, q - r.first[a], &s);
     } else {
-      const uint4 wv = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)w + k);
-      const __nv_bfloat162* w2 = reinterpret_cast<const __nv_bfloat162*>(&wv);
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = __bfloat1622float2(x2[i]), b = __bfloat1622float2(w2[i]);
-        part += a.x * b.x + a.y * b.y;
+      while (segment >= tiles * r.first[a + 1]) ++a;
+      const int in = segment - tiles * r.first[a], chunks = r.first[a + 1] - r.first[a];
+      s.tile = in / chunks;
+      xp_locate(r, a, in - s.tile * chunks, &s);
+    }
+    return s;
+  }
+};
+
+// Counts and orders the entries. `counts` is scratch, [warps][n_experts].
+__device__ __forceinline__ void xp_route(const eux_experts_desc& d, int cap, XpTables& r, int* counts, int* named_out) {
+  const int E = d.n_experts, n = d.n_tokens * d.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int W = kXpThreads / 32;
+  const int each = ((n + W - 1) / W + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
+  for (int i = threadIdx.x; i < W * E; i += kXpThreads) counts[i] = 0;
+  __syncthreads();
+  for (int i = lo + lane; i < hi; i += 32) {
+    const int e = d.topk_idx[i];
+    if ((uint32_t)e < (uint32_t)E) atomicAdd(&counts[warp * E + e], 1);
+  }
+  __syncthreads();
+  // warp 0: the named experts, where their entries begin and how many chunks each has
+  if (warp == 0) {
+    int named = 0, at = 0, chunks = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int c = 0;
+      if (e < E)
+        for (int w = 0; w < W; ++w) c += counts[w * E + e];
+      const uint32_t has = __ballot_sync(0xffffffffu, c > 0);
+      if (!has) continue;
+      const int ch = (c + cap - 1) / cap;
+      int c_sum = c, ch_sum = ch;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, c_sum, o), v = __shfl_up_sync(0xffffffffu, ch_sum, o);
+        if (lane >= o) c_sum += u, ch_sum += v;
       }
-      acc += part;
+      if (c > 0) {
+        const int a = named + __popc(has & ((1u << lane) - 1u));
+        r.expert[a] = (uint16_t)e, r.start[a] = at + c_sum - c, r.first[a] = (uint16_t)(chunks + ch_sum - ch);
+        // from counts to places: where each warp's entries of this expert go
+        int p = at + c_sum - c;
+        for (int w = 0; w < W; ++w) {
+          const int m = counts[w * E + e];
+          counts[w * E + e] = p;
+          p += m;
+        }
+      }
+      named += __popc(has);
+      at += __shfl_sync(0xffffffffu, c_sum, 31), chunks += __shfl_sync(0xffffffffu, ch_sum, 31);
+    }
+    if (lane == 0) r.start[named] = at, r.first[named] = (uint16_t)chunks, *named_out = named;
+  }
+  __syncthreads();
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane;
+    const int e = i < hi ? d.topk_idx[i] : -1;
+    const bool here = (uint32_t)e < (uint32_t)E;
+    const uint32_t same = __match_any_sync(0xffffffffu, here ? e : -1);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    if (here) r.order[counts[warp * E + e] + before] = (uint16_t)i;
+    __syncwarp();
+    if (here && before == 0) counts[warp * E + e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  r.named = *named_out;
+}
+
+// What the warps that multiply share.
+struct XpRing {
+  uint32_t w, x, scales, full, empty;
+  int stages, x_bytes;
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == stages) s = 0, ph ^= 1u;
+  }
+};
+
+// blocks [kb, end) of a segment times its tokens, for this warp's 32 rows and its half of each block's K; the two halves' sums
+// are left in `sum` [token][row], which all consumers may read when this returns.
+template <bool FP8, bool DOWN, int NB>
+__device__ __forceinline__ void xp_segment(XpRing& ring, int blocks, int up_border, float* sum, int warp, int lane, volatile int* abort,
+                                           uint64_t timeout_ns) {
+  const int rows = (warp & 3) * 32, half = warp >> 2, g = lane >> 2, c = lane & 3;
+  float acc[2][NB][4] = {};
+  for (int k = 0; k < blocks; ++k) {
+    // A wait that ran out raises `abort`; the warps then finish on whatever lies there, so that they meet at every barrier, and the
+    // status word says that the result is none.
+    mbar_wait(ring.full + 16 * ring.s, ring.ph, abort, timeout_ns);
+    __syncwarp();
+    const uint32_t w = ring.w + ring.s * kXpBlock, x = ring.x + ring.s * ring.x_bytes;
+    if constexpr (!FP8) {
+      uint32_t b1[4];
+      if (NB == 1) ldsm_x4(b1, x + (lane & 7) * 128 + (((half * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int step = half * 2 + ks;
+        uint32_t a[2][4], b[NB > 1 ? NB / 2 : 1][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int row = rows + m * 16 + (lane & 15);
+          ldsm_x4(a[m], w + row * 128 + (((step * 2 + (lane >> 4)) ^ (row & 7)) << 4));
+        }
+        if (NB == 1) {
+          b[0][0] = b1[2 * ks], b[0][1] = b1[2 * ks + 1];
+        } else {
+#pragma unroll
+          for (int j = 0; j < NB / 2; ++j) {
+            const int row = j * 16 + (lane & 7) + ((lane >> 4) << 3);
+            ldsm_x4(b[j], x + row * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            mma_bf16(acc[m][j], a[m][0], a[m][1], a[m][2], a[m][3], b[j / 2][(j & 1) * 2], b[j / 2][(j & 1) * 2 + 1]);
+      }
+    } else {
+      // A 16-byte piece of a row is 16 values of K. ldmatrix gives lane (g, c) the four at 4c: the product takes them as its k = 2c,
+      // 2c + 1, 2c + 8 and 2c + 9, and the tokens' values likewise (the order of K is the product's own affair).
+      float part[2][NB][4] = {};
+#pragma unroll
+      for (int kp = 0; kp < 2; ++kp) {
+        const int step = half * 4 + kp * 2;
+        uint32_t a[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const int row = rows + m * 16 + (lane & 15);
+          ldsm_x4(a[m], w + row * 128 + (((step + (lane >> 4)) ^ (row & 7)) << 4));
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t wa[2][4];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t r0 = a[m][2 * ks], r1 = a[m][2 * ks + 1];
+            wa[m][0] = widen<0x1404>(r0), wa[m][1] = widen<0x1404>(r1), wa[m][2] = widen<0x3424>(r0), wa[m][3] = widen<0x3424>(r1);
+          }
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            const int row = j * 8 + g;
+            uint32_t b0, b1;
+            lds_64(b0, b1, x + row * 256 + ((((step + ks) * 2 + (c >> 1)) ^ ((row & 3) << 1)) << 4) + (c & 1) * 8);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) mma_bf16(part[m][j], wa[m][0], wa[m][1], wa[m][2], wa[m][3], b0, b1);
+          }
+        }
+      }
+      // a block of K is a block of scales; of the rows, the up half may lie in two
+      float sc[3];
+      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(sc[0]), "=f"(sc[1]) : "r"(ring.scales + 16 * ring.s) : "memory");
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sc[2]) : "r"(ring.scales + 16 * ring.s + 8) : "memory");
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float lo = sc[0], hi = sc[0];
+        if (!DOWN && rows >= 64) {
+          const int row = rows - 64 + m * 16 + g;
+          lo = row < up_border ? sc[1] : sc[2], hi = row + 8 < up_border ? sc[1] : sc[2];
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          acc[m][j][0] = fmaf(part[m][j][0], lo, acc[m][j][0]), acc[m][j][1] = fmaf(part[m][j][1], lo, acc[m][j][1]);
+          acc[m][j][2] = fmaf(part[m][j][2], hi, acc[m][j][2]), acc[m][j][3] = fmaf(part[m][j][3], hi, acc[m][j][3]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ring.empty + 16 * ring.s);
+    ring.next();
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (half == h) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float* at = sum + (j * 8 + 2 * c + (q & 1)) * kXpLd + rows + m * 16 + g + (q >> 1) * 8;
+            *at = h == 0 ? acc[m][j][q] : *at + acc[m][j][q];
+          }
+    }
+    consumers_meet();
+  }
+}
+
+__device__ __forceinline__ float4 ldcg_f4(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <bool FP8, bool DOWN>
+__global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ XpParams p) {
+  extern __shared__ __align__(1024) unsigned char xp_smem[];
+  __shared__ int s_abort, s_named, s_last;
+  const eux_experts_desc& d = p.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int entries = d.n_tokens * d.topk;
+  const XpLayout l = xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries);
+  const uint32_t smem = smem_u32(xp_smem);
+  XpRing ring;
+  ring.w = smem, ring.x = smem + l.x, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;
+  ring.stages = p.stages, ring.x_bytes = p.x_bytes;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(ring.full + 16 * i, 1 + 32);
+      mbar_init(ring.empty + 16 * i, kXpWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+  }
+  // The up form waits here for whatever wrote the tokens and their experts. The down form was let in by the up form, behind its
+  // wait: what both read is there, and only what the up form writes is waited for (below).
+  if (!DOWN) wait_for_launch_before();
+  XpTables r;
+  r.start = reinterpret_cast<int*>(xp_smem + l.tables);
+  r.first = reinterpret_cast<uint16_t*>(r.start + d.n_experts + 1);
+  r.expert = r.first + d.n_experts + 1;
+  r.order = r.expert + d.n_experts + 1;
+  xp_route(d, p.cap, r, reinterpret_cast<int*>(xp_smem), &s_named);
+  // the counts lay where weights are about to land
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+
+  const int K = DOWN ? d.inner : d.hidden, per_block = FP8 ? 128 : 64;
+  const int nk = (K + per_block - 1) / per_block;
+  const int tiles = DOWN ? (d.hidden + kXpRows - 1) / kXpRows : (d.inner + 63) / 64;
+  const int chunks = r.first[r.named];
+  const int64_t blocks = (int64_t)tiles * chunks * nk;
+  const int grid = (int)min((int64_t)gridDim.x, max((int64_t)1, blocks / kXpMinBlocks));
+  const int me = blockIdx.x;
+  const int64_t b0 = me < grid ? blocks * me / grid : blocks, b1 = me < grid ? blocks * (me + 1) / grid : blocks;
+  volatile int* abort = &s_abort;
+  XpWalk<DOWN> walk(r, tiles);
+
+  if (warp == kXpWarps) {
+    // ---- weights ----
+    if (lane == 0) {
+      for (int64_t b = b0; b < b1 && !*abort;) {
+        const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+        const XpSegment s = walk.at(seg);
+        for (int k = kb; k < end; ++k) {
+          if (!mbar_wait(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns)) break;
+          const uint32_t bar = ring.full + 16 * ring.s, dst = ring.w + ring.s * kXpBlock;
+          mbar_expect_tx(bar, kXpBlock);
+          if (DOWN) {
+            tma_load_3d(dst, &map, bar, k * per_block, s.tile * kXpRows, s.expert);
+          } else {
+            tma_load_3d(dst, &map, bar, k * per_block, s.tile * 64, s.expert * 2);
+            tma_load_3d(dst + kXpBlock / 2, &map, bar, k * per_block, s.tile * 64, s.expert * 2 + 1);
+          }
+          ring.next();
+        }
+        b += end - kb;
+      }
+      if (*abort) {  // loads that were issued still write shared memory: give them time to land
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+      allow_next_launch();
+    }
+  } else if (warp == kXpWarps + 1) {
+    // ---- the tokens' values (down: their h) and the scales ----
+    if (DOWN) wait_for_launch_before();
+    const int sr = ((DOWN ? d.hidden : 2 * d.inner) + 127) / 128, sk = (K + 127) / 128;
+    for (int64_t b = b0; b < b1;) {
+      const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+      const XpSegment s = walk.at(seg);
+      const int rows = (s.n + 7) & ~7, pieces = FP8 ? 16 : 8;
+      bool gone = false;
+      for (int k = kb; k < end && !gone; ++k) {
+        gone = __any_sync(0xffffffffu, !mbar_wait(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
+        if (gone) break;
+        const uint32_t dst = ring.x + ring.s * ring.x_bytes;
+        for (int i = lane; i < rows * pieces; i += 32) {
+          const int row = i / pieces, piece = i % pieces, at = k * per_block + piece * 8;
+          const bool some = row < s.n && at < K;
+          const int entry = r.order[s.pos + (row < s.n ? row : 0)];
+          const __nv_bfloat16* src = DOWN ? p.h + (int64_t)entry * d.inner : (const __nv_bfloat16*)d.x + (int64_t)(entry / d.topk) * d.x_stride;
+          const int swizzled = FP8 ? piece ^ ((row & 3) << 1) : piece ^ (row & 7);
+          cp_async_16(dst + row * (pieces * 16) + swizzled * 16, src + (some ? at : 0), some ? 16 : 0);
+        }
+        if (FP8 && lane < (DOWN ? 1 : 3)) {
+          // down: the scale of the rows; up: the gate rows', the first up rows', those of the up rows in the next block
+          const int row = DOWN ? s.tile : lane == 0 ? s.tile * 64 / 128 : min((d.inner + s.tile * 64) / 128 + lane - 1, sr - 1);
+          cp_async_4(ring.scales + 16 * ring.s + 4 * lane, (DOWN ? d.down_scale : d.gate_up_scale) + ((int64_t)s.expert * sr + row) * sk + k);
+        }
+        cp_async_arrive(ring.full + 16 * ring.s);
+        ring.next();
+      }
+      if (gone) break;
+      b += end - kb;
+    }
+    cp_async_wait_all();
+  } else {
+    // ---- products ----
+    if (DOWN) wait_for_launch_before();
+    float* const sum = reinterpret_cast<float*>(xp_smem + l.stage_sum);
+    float* const acc = reinterpret_cast<float*>(xp_smem + l.acc);
+    const int tid = threadIdx.x;
+    const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
+    const int64_t tile_blocks = (int64_t)tile_segs * nk;
+    const int width = DOWN ? d.n_tokens : 0;  // rows of a part (up: the segment's tokens)
+    if (DOWN && blocks == 0) {  // no expert is named: the result is zero
+      for (int64_t i = (int64_t)blockIdx.x * kXpConsumers + tid; i < (int64_t)d.n_tokens * (d.hidden / 8); i += (int64_t)gridDim.x * kXpConsumers)
+        st_u4((__nv_bfloat16*)d.out + (i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
+    }
+    for (int64_t b = b0; b < b1;) {
+      const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+      const XpSegment s = walk.at(seg);
+      const int tile = seg / tile_segs;
+      const int64_t tile0 = tile * tile_blocks;
+      if (DOWN && (b == b0 || b == tile0)) {
+        for (int i = tid; i < d.n_tokens * kXpLd; i += kXpConsumers) acc[i] = 0.f;
+      }
+      const int up_border = 128 - (d.inner + s.tile * 64) % 128;
+      const int nb = (s.n + 7) >> 3;
+      if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      b += end - kb;
+      if (DOWN) {
+        // A thread has a row and the tokens of one parity: entries of the same token, also twice of the same expert, are added by one
+        // thread, in order.
+        const int row = tid & 127, parity = tid >> 7;
+        for (int j = 0; j < s.n; ++j) {
+          const int entry = r.order[s.pos + j], t = entry / d.topk;
+          if ((t & 1) == parity) acc[t * kXpLd + row] = fmaf(__ldg(d.topk_w + entry), sum[j * kXpLd + row], acc[t * kXpLd + row]);
+        }
+        consumers_meet();
+      }
+      if (b != b1 && b != tile0 + tile_blocks) continue;
+      // ---- the end of a tile, or of this SM's part of it ----
+      const int first = (int)(((tile0 + 1) * grid - 1) / blocks), last = (int)(((tile0 + tile_blocks) * grid - 1) / blocks);
+      const int rows = DOWN ? width : s.n;
+      const float* const from = DOWN ? acc : sum;
+      bool mine = true;
+      if (first != last) {
+        float* const part = p.part + ((int64_t)me * 2 + (me == first)) * p.part_rows * kXpRows;
+        for (int i = tid; i < rows * (kXpRows / 4); i += kXpConsumers)
+          __stcg(reinterpret_cast<float4*>(part) + i, *reinterpret_cast<const float4*>(from + (i / (kXpRows / 4)) * kXpLd + (i % (kXpRows / 4)) * 4));
+        __threadfence();
+        consumers_meet();
+        // counts up to the number of parts and starts again: ready for the next launch
+        if (tid == 0) s_last = atomicInc(d.counters + (DOWN ? kXpMaxGrid : 0) + first, (unsigned)(last - first)) == (unsigned)(last - first);
+        consumers_meet();
+        mine = s_last != 0;
+        if (mine) __threadfence();
+      }
+      if (mine) {
+        constexpr int Q = DOWN ? kXpRows / 4 : 16;  // four rows of results per thread and step
+        for (int i = tid; i < rows * Q; i += kXpConsumers) {
+          const int j = i / Q, q = (i % Q) * 4;
+          float4 v, u;
+          if (first == last) {
+            v = *reinterpret_cast<const float4*>(from + j * kXpLd + q);
+            if (!DOWN) u = *reinterpret_cast<const float4*>(from + j * kXpLd + 64 + q);
+          } else {
+            v = u = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = first; k <= last; ++k) {
+              const float* part = p.part + (((int64_t)k * 2 + (k == first)) * p.part_rows + j) * kXpRows + q;
+              const float4 a = ldcg_f4(part);
+              v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+              if (!DOWN) {
+                const float4 o = ldcg_f4(part + 64);
+                u.x += o.x, u.y += o.y, u.z += o.z, u.w += o.w;
+              }
+            }
+          }
+          if (DOWN) {
+            const int at = s.tile * kXpRows + q;
+            if (at < d.hidden)
+              *reinterpret_cast<uint2*>((__nv_bfloat16*)d.out + j * d.out_stride + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+          } else {
+            const int at = s.tile * 64 + q;
+            auto gated = [](float g, float w) { return g / (1.f + expf(-g)) * w; };
+            if (at < d.inner)
+              *reinterpret_cast<uint2*>(p.h + (int64_t)r.order[s.pos + j] * d.inner + at) =
+                  make_uint2(pack_bf16(gated(v.x, u.x), gated(v.y, u.y)), pack_bf16(gated(v.z, u.z), gated(v.w, u.w)));
+          }
+        }
+      }
+      consumers_meet();  // what was read is written over next
     }
   }
-  for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  return acc;
+  __syncthreads();
+  if (threadIdx.x == 0 && s_abort) set_status(d.status, EUX_ST_TIMEOUT, DOWN ? 2 : 1);
 }
 
-template <bool FP8>
-__global__ void __launch_bounds__(kExpertThreads) experts_up_kernel(eux_experts_desc d) {
-  const int lane = threadIdx.x & 31, j = blockIdx.y, i = blockIdx.x * (kExpertThreads / 32) + (threadIdx.x >> 5);
-  const int e = d.topk_idx[j];
-  if (e < 0 || e >= d.n_experts || i >= d.inner) return;
-  const __nv_bfloat16* x = (const __nv_bfloat16*)d.x + (int64_t)(j / d.topk) * d.x_stride;
-  const size_t elem = FP8 ? 1 : 2, sr = (2 * d.inner + 127) / 128, sc = (d.hidden + 127) / 128;
-  float v[2];
-  for (int half = 0; half < 2; ++half) {
-    const size_t r = (size_t)i + (size_t)half * d.inner;
-    v[half] = row_dot<FP8>((const char*)d.w_gate_up + ((size_t)e * 2 * d.inner + r) * d.hidden * elem,
-                           d.gate_up_scale + (e * sr + r / 128) * sc, x, d.hidden, lane);
-  }
-  if (lane == 0) ((__nv_bfloat16*)d.workspace)[(size_t)j * d.inner + i] = __float2bfloat16_rn(v[0] / (1.f + __expf(-v[0])) * v[1]);
-}
+// ---- host ----
 
-template <bool FP8>
-__global__ void __launch_bounds__(kExpertThreads) experts_down_kernel(eux_experts_desc d) {
-  const int lane = threadIdx.x & 31, t = blockIdx.y, r = blockIdx.x * (kExpertThreads / 32) + (threadIdx.x >> 5);
-  if (r >= d.hidden) return;
-  const size_t elem = FP8 ? 1 : 2, sr = (d.hidden + 127) / 128, sc = (d.inner + 127) / 128;
-  float y = 0.f;
-  for (int s = 0; s < d.topk; ++s) {
-    const int j = t * d.topk + s, e = d.topk_idx[j];
-    if (e < 0 || e >= d.n_experts) continue;
-    y += d.topk_w[j] * row_dot<FP8>((const char*)d.w_down + ((size_t)e * d.hidden + r) * d.inner * elem,
-                                    d.down_scale + (e * sr + r / 128) * sc, (const __nv_bfloat16*)d.workspace + (size_t)j * d.inner,
-                                    d.inner, lane);
-  }
-  if (lane == 0) ((__nv_bfloat16*)d.out)[(int64_t)t * d.out_stride + r] = __float2bfloat16_rn(y);
+typedef CUresult (*XpEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static XpEncodeFn xp_encode() {
+  static const XpEncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? (XpEncodeFn)p
+               : nullptr;
+  }();
+  return fn;
+}
+// [slices][rows][cols], boxes of box_rows x 128 bytes, 128-byte swizzle; what lies outside is read as zero
+static int xp_map(CUtensorMap* m, const void* base, bool fp8, uint64_t slices, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  const XpEncodeFn fn = xp_encode();
+  if (!fn) return EUX_ERR_UNSUPPORTED;
+  const uint64_t elem = fp8 ? 1 : 2;
+  const cuuint64_t dims[3] = {cols, rows, slices}, strides[2] = {cols * elem, rows * cols * elem};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / elem), box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult rc = fn(m, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? 0 : EUX_ERR_BAD_ARG;
 }
 
 static int experts_check(const eux_experts_desc* d) {
   if (!d || d->n_tokens < 0 || d->n_tokens > EUX_EXPERTS_MAX_TOKENS || d->topk < 1 || d->topk > 32) return EUX_ERR_BAD_ARG;
   if (d->n_experts < 1 || d->n_experts > EUX_EXPERTS_MAX_EXPERTS || d->hidden < 1 || d->inner < 1) return EUX_ERR_BAD_ARG;
+  if (d->hidden > (1 << 20) || d->inner > (1 << 20)) return EUX_ERR_BAD_ARG;
   const int unit = d->fp8 ? 16 : 8;  // rows of weights begin on 16 bytes
   if (d->hidden % unit || d->inner % unit || d->x_stride % 8 || d->out_stride % 8) return EUX_ERR_BAD_ARG;
   return 0;
+}
+// Tokens of an expert in a segment: what the accumulators hold, and with e4m3 weights what the products keep up with.
+// 8, 16, 32 or 64, as the products have them.
+static int xp_cap(const eux_experts_desc* d) {
+  int cap = 8;
+  while (cap < (d->fp8 ? 32 : 64) && cap < d->n_tokens * d->topk) cap *= 2;
+  return cap;
+}
+static int xp_part_rows(const eux_experts_desc* d) { return std::max(xp_cap(d), d->n_tokens); }
+static size_t xp_h_bytes(const eux_experts_desc* d) { return ((size_t)d->n_tokens * d->topk * d->inner * 2 + 255) & ~(size_t)255; }
+
+static int xp_sms(int* dev) {
+  int sms = 148;
+  cudaGetDevice(dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *dev);
+  return std::min(sms, kXpMaxGrid);
+}
+
+template <bool FP8, bool DOWN>
+static int xp_launch(const CUtensorMap& map, XpParams p, int dev, int sms, cudaStream_t st) {
+  const eux_experts_desc& d = p.d;
+  p.x_bytes = p.cap * (FP8 ? 256 : 128);
+  const int entries = d.n_tokens * d.topk;
+  p.stages = kXpMaxStages;
+  // 1 KiB for the variables that the kernel declares itself
+  while (p.stages > 2 && (size_t)xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries).total > kXpSmem - 1024) --p.stages;
+  // the routing's counts lie in the ring before it is filled
+  const XpLayout l = xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries);
+  if ((size_t)l.total > kXpSmem - 1024 || kXpThreads / 32 * d.n_experts * 4 > p.stages * kXpBlock) return EUX_ERR_TOO_LARGE;
+  if (cudaError_t e = allow_smem<moe_experts_kernel<FP8, DOWN>>(dev, kXpSmem - 1024); e != cudaSuccess) return (int)e;
+  return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, l.total, st, map, p);
 }
 
 }  // namespace eux
@@ -88,33 +619,36 @@ static int experts_check(const eux_experts_desc* d) {
 using namespace eux;
 
 extern "C" size_t eux_experts_workspace_bytes(const eux_experts_desc* d) {
-  return experts_check(d) ? 0 : (size_t)d->n_tokens * d->topk * d->inner * 2;
+  if (experts_check(d)) return 0;
+  return xp_h_bytes(d) + (size_t)kXpMaxGrid * 2 * xp_part_rows(d) * kXpRows * 4;
 }
-extern "C" size_t eux_experts_counter_words(const eux_experts_desc* d) { return experts_check(d) ? 0 : 1; }
+extern "C" size_t eux_experts_counter_words(const eux_experts_desc* d) { return experts_check(d) ? 0 : 2 * kXpMaxGrid; }
 
 extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   if (int rc = experts_check(d)) return rc;
   if (d->n_tokens == 0) return 0;
-  if (!d->x || !d->topk_idx || !d->topk_w || !d->out || !d->w_gate_up || !d->w_down || !d->workspace) return EUX_ERR_BAD_ARG;
+  if (!d->x || !d->topk_idx || !d->topk_w || !d->out || !d->w_gate_up || !d->w_down || !d->workspace || !d->counters) return EUX_ERR_BAD_ARG;
   if (d->fp8 && (!d->gate_up_scale || !d->down_scale)) return EUX_ERR_BAD_ARG;
   if (((uintptr_t)d->x | (uintptr_t)d->out | (uintptr_t)d->w_gate_up | (uintptr_t)d->w_down | (uintptr_t)d->workspace) & 15) return EUX_ERR_BAD_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int w = kExpertThreads / 32;
-  const dim3 up((d->inner + w - 1) / w, d->n_tokens * d->topk), down((d->hidden + w - 1) / w, d->n_tokens);
-  if (d->fp8) {
-    experts_up_kernel<true><<<up, kExpertThreads, 0, st>>>(*d);
-    experts_down_kernel<true><<<down, kExpertThreads, 0, st>>>(*d);
-  } else {
-    experts_up_kernel<false><<<up, kExpertThreads, 0, st>>>(*d);
-    experts_down_kernel<false><<<down, kExpertThreads, 0, st>>>(*d);
-  }
-  return (int)cudaGetLastError();
+  CUtensorMap up, down;
+  if (int rc = xp_map(&up, d->w_gate_up, d->fp8, 2 * (uint64_t)d->n_experts, d->inner, d->hidden, 64)) return rc;
+  if (int rc = xp_map(&down, d->w_down, d->fp8, d->n_experts, d->hidden, d->inner, kXpRows)) return rc;
+  XpParams p = {};
+  p.d = *d;
+  p.h = (__nv_bfloat16*)d->workspace;
+  p.part = (float*)((char*)d->workspace + xp_h_bytes(d));
+  p.part_rows = xp_part_rows(d), p.cap = xp_cap(d);
+  int dev = 0;
+  const int sms = xp_sms(&dev);
+  if (int rc = d->fp8 ? xp_launch<true, false>(up, p, dev, sms, st) : xp_launch<false, false>(up, p, dev, sms, st)) return rc;
+  return d->fp8 ? xp_launch<true, true>(down, p, dev, sms, st) : xp_launch<false, true>(down, p, dev, sms, st);
 }
 
 extern "C" int eux_experts_preload(void) {
   cudaFuncAttributes a;
-  const void* kernels[] = {(const void*)experts_up_kernel<false>, (const void*)experts_up_kernel<true>,
-                           (const void*)experts_down_kernel<false>, (const void*)experts_down_kernel<true>};
+  const void* kernels[] = {(const void*)moe_experts_kernel<false, false>, (const void*)moe_experts_kernel<false, true>,
+                           (const void*)moe_experts_kernel<true, false>, (const void*)moe_experts_kernel<true, true>};
   for (const void* k : kernels)
     if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;
   return 0;

@@ -200,7 +200,7 @@ class MoeExperts:
     ceil(2 * inner / 128), ceil(hidden / 128)]`` and ``down_scale`` ``[experts, ceil(hidden / 128), ceil(inner / 128)]`` (what
     ``remote_gemm.quantize_blocks_128x128`` gives for each expert). They are used where they lie: the object keeps the tensors
     and copies nothing, so what is written into them holds for the next call. ``hidden`` and ``inner`` are multiples of 8
-    (16 for e4m3).
+    (16 for e4m3), e4m3 weights no NaN (checked when they are given).
 
     Made for few tokens, where the layer is as fast as the weights of the named experts can be read: rows beyond
     ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again."""
@@ -230,6 +230,10 @@ class MoeExperts:
         ws.require_device(self.device, w_gate_up=w_gate_up, gate_up_scale=gate_up_scale, down_scale=down_scale)
         ws.require_cuda(self.device)
         ws.require((w_gate_up.data_ptr() | w_down.data_ptr()) % 16 == 0, "weights must begin on 16 bytes")
+        if self.fp8:
+            # the kernels widen e4m3 by moving bits, which has no place for NaN
+            nan = sum(((w[j].view(torch.uint8) & 0x7F) == 0x7F).any() for w in (w_gate_up, w_down) for j in range(e))
+            ws.require(int(nan) == 0, "e4m3 weights must not be NaN")
         self.w_gate_up, self.w_down, self.gate_up_scale, self.down_scale = w_gate_up, w_down, gate_up_scale, down_scale
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         words = _native.load().eux_experts_counter_words(self._desc(self.MAX_TOKENS, 1))

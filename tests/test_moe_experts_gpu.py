@@ -179,6 +179,15 @@ def test_e4m3_weights_of_every_code(cuda_device):
     assert torch.equal(out[0, :254].float(), want.to(torch.bfloat16).float())  # 7 bits of 448 times 4 bits: exact before the rounding
 
 
+def test_e4m3_weights_that_are_nan_are_refused(cuda_device):
+    from execution_ucx_b200.ops import moe
+    for which, code in ((0, 0x7f), (1, 0xff)):
+        gu, down, gus, ds = weights(3, 256, 144, True, cuda_device)
+        (gu, down)[which].view(torch.uint8)[2, 5, 9] = code
+        with pytest.raises(ValueError, match="NaN"):
+            moe.MoeExperts(gu, down, gus, ds)
+
+
 def test_two_streams_at_once(cuda_device):
     from execution_ucx_b200.ops import moe
     layer = moe.MoeExperts(*weights(8, 1024, 256, False, cuda_device))
