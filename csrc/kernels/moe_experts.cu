@@ -14,7 +14,7 @@
 //   form a tile is 128 rows of the output with all experts, so the weighted sum over a token's experts is made in shared
 //   memory, and only what an SM's share cuts goes through the workspace.
 // * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp fetches the tokens' values beside them
-//   with cp.async (rows are gathered: any tokens, any order), eight warps multiply: four by rows, two by K. The ring runs on
+//   with cp.async (rows are gathered: any tokens, any order), twelve warps multiply. The ring runs on
 //   over the borders of segments; the down form's starts before the up form has ended (programmatic dependent launch), since
 //   weights wait for nobody.
 // * The weights are the first operand of mma.sync m16n8k16 and the tokens the second: 8 columns are the smallest padding for
@@ -33,15 +33,16 @@
 
 namespace eux {
 
-constexpr int kXpWarps = 8;                         // that multiply
+constexpr int kXpGroups = 3;                        // of warps that multiply: each takes the blocks of every third stage ...
+constexpr int kXpWarps = kXpGroups * 4;             // ... and each of its four warps 32 rows of it
 constexpr int kXpConsumers = kXpWarps * 32;
 constexpr int kXpThreads = kXpConsumers + 64;       // and one that fetches weights, one that fetches tokens
 constexpr int kXpRows = 128;                        // rows of weights in a block
 constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
-constexpr int kXpMaxStages = 12;
+constexpr int kXpMaxStages = 13;
 constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
 constexpr int kXpMaxGrid = 160;
-constexpr size_t kXpSmem = 227 * 1024;
+constexpr size_t kXpDynamic = 226 * 1024;           // shared memory of a launch; the kernel declares a little more itself
 constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer cost more to add up than they save
 
 struct XpParams {
@@ -49,26 +50,28 @@ struct XpParams {
   __nv_bfloat16* h;      // [entries, inner]
   float* part;           // [grid][2][part_rows][128]
   int part_rows;
-  int cap;               // tokens of an expert that a segment takes at most
-  int stages;
-  int x_bytes;           // of a stage
 };
 
-// Shared memory behind the ring of weights, in bytes from its end.
+// Shared memory: the ring of weights (128-byte swizzle: on 1024 bytes), behind it the tokens' values of each stage, the sums
+// of a segment; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
+// many stages there is room for, is known when the entries have been counted.
 struct XpLayout {
-  int x, stage_sum, acc, scales, bars, tables, total;
+  int acc, scales, bars, tables;  // from the beginning
+  int room;                       // bytes in front of these
 };
-__host__ __device__ inline XpLayout xp_layout(bool down, int stages, int x_bytes, int cap, int n_tokens, int n_experts, int entries) {
+__host__ __device__ inline XpLayout xp_layout(bool down, int n_tokens, int n_experts, int entries) {
   XpLayout l;
-  int at = stages * kXpBlock;
-  l.x = at, at += stages * x_bytes;
-  l.stage_sum = at, at += cap * kXpLd * 4;
-  l.acc = at, at += down ? n_tokens * kXpLd * 4 : 0;
-  l.scales = at, at += stages * 16;
-  l.bars = at, at += stages * 16;
-  l.tables = at, at += (n_experts + 1) * 8 + 16 + ((entries * 2 + 15) & ~15);
-  l.total = (at + 15) & ~15;
+  int at = (int)kXpDynamic;
+  at -= ((n_experts + 1) * 8 + entries * 4 + 15) & ~15, l.tables = at;
+  at -= kXpMaxStages * 16, l.bars = at;
+  at -= kXpMaxStages * 16, l.scales = at;
+  at -= down ? n_tokens * kXpLd * 4 : 0, l.acc = at;
+  l.room = at;
   return l;
+}
+__host__ __device__ inline int xp_stages(int room, int cap, int x_bytes) {
+  const int n = (room - cap * kXpLd * 4) / (kXpBlock + x_bytes);
+  return n < kXpMaxStages ? n : kXpMaxStages;
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
@@ -120,6 +123,7 @@ struct XpTables {
   uint16_t* first;   // [named + 1]
   uint16_t* expert;  // [named]
   uint16_t* order;   // [entries]
+  uint16_t* token;   // [entries]: of order
   int named;
 };
 
@@ -161,8 +165,9 @@ struct XpWalk {
   }
 };
 
-// Counts and orders the entries. `counts` is scratch, [warps][n_experts].
-__device__ __forceinline__ void xp_route(const eux_experts_desc& d, int cap, XpTables& r, int* counts, int* named_out) {
+// Counts and orders the entries. `counts` is scratch, [warps][n_experts]. Returns the tokens that a segment takes at most: 8, 16,
+// 32 or 64, as the expert with the most needs and `most` allows.
+__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* counts, int* out) {
   const int E = d.n_experts, n = d.n_tokens * d.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int W = kXpThreads / 32;
   const int each = ((n + W - 1) / W + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
@@ -175,7 +180,14 @@ __device__ __forceinline__ void xp_route(const eux_experts_desc& d, int cap, XpT
   __syncthreads();
   // warp 0: the named experts, where their entries begin and how many chunks each has
   if (warp == 0) {
-    int named = 0, at = 0, chunks = 0;
+    int named = 0, at = 0, chunks = 0, cap = 8, top = 0;
+    for (int e = lane; e < E; e += 32) {
+      int c = 0;
+      for (int w = 0; w < W; ++w) c += counts[w * E + e];
+      top = max(top, c);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    while (cap < top && cap < most) cap *= 2;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + lane;
       int c = 0;
@@ -203,7 +215,7 @@ __device__ __forceinline__ void xp_route(const eux_experts_desc& d, int cap, XpT
       named += __popc(has);
       at += __shfl_sync(0xffffffffu, c_sum, 31), chunks += __shfl_sync(0xffffffffu, ch_sum, 31);
     }
-    if (lane == 0) r.start[named] = at, r.first[named] = (uint16_t)chunks, *named_out = named;
+    if (lane == 0) r.start[named] = at, r.first[named] = (uint16_t)chunks, out[0] = named, out[1] = cap;
   }
   __syncthreads();
   for (int i0 = lo; i0 < hi; i0 += 32) {
@@ -212,13 +224,17 @@ __device__ __forceinline__ void xp_route(const eux_experts_desc& d, int cap, XpT
     const bool here = (uint32_t)e < (uint32_t)E;
     const uint32_t same = __match_any_sync(0xffffffffu, here ? e : -1);
     const int before = __popc(same & ((1u << lane) - 1u));
-    if (here) r.order[counts[warp * E + e] + before] = (uint16_t)i;
+    if (here) {
+      const int at = counts[warp * E + e] + before;
+      r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)(i / d.topk);
+    }
     __syncwarp();
     if (here && before == 0) counts[warp * E + e] += __popc(same);
     __syncwarp();
   }
   __syncthreads();
-  r.named = *named_out;
+  r.named = out[0];
+  return out[1];
 }
 
 // What the warps that multiply share.
@@ -230,55 +246,66 @@ struct XpRing {
   __device__ __forceinline__ void next() {
     if (++s == stages) s = 0, ph ^= 1u;
   }
+  // Of a group, which has the stages group, group + kXpGroups, ... A stage must not change hands: its barrier tells two phases
+  // apart, and a group that came to it from elsewhere, ahead of a load that is late, would take the phase before the last for it.
+  __device__ __forceinline__ void next_of_group(int group, int64_t& block) {
+    block += kXpGroups;
+    if ((s += kXpGroups) >= stages) block += group + stages - s, s = group, ph ^= 1u;
+  }
 };
 
-// blocks [kb, end) of a segment times its tokens, for this warp's 32 rows and its half of each block's K; the two halves' sums
-// are left in `sum` [token][row], which all consumers may read when this returns.
+// The blocks of a segment up to number `end` of this SM's line times the segment's tokens: those in this group's stages, `mine`
+// the next of them, and this warp's 32 rows. All groups' sums are left in `sum` [token][row], which all of them may read when this
+// returns. Groups by blocks and not by parts of one: a block takes a warp some hundred clocks from its arrival to its release,
+// one thing after the other, and so three are under way at once.
 template <bool FP8, bool DOWN, int NB>
-__device__ __forceinline__ void xp_segment(XpRing& ring, int blocks, int up_border, float* sum, int warp, int lane, volatile int* abort,
-                                           uint64_t timeout_ns) {
-  const int rows = (warp & 3) * 32, half = warp >> 2, g = lane >> 2, c = lane & 3;
+__device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t end, int up_border, float* sum, int warp, int lane,
+                                           volatile int* abort, uint64_t timeout_ns) {
+  const int rows = (warp & 3) * 32, group = warp >> 2, g = lane >> 2, c = lane & 3;
   float acc[2][NB][4] = {};
-  for (int k = 0; k < blocks; ++k) {
+  while (mine < end) {
     // A wait that ran out raises `abort`; the warps then finish on whatever lies there, so that they meet at every barrier, and the
     // status word says that the result is none.
     mbar_wait(ring.full + 16 * ring.s, ring.ph, abort, timeout_ns);
     __syncwarp();
     const uint32_t w = ring.w + ring.s * kXpBlock, x = ring.x + ring.s * ring.x_bytes;
     if constexpr (!FP8) {
-      uint32_t b1[4];
-      if (NB == 1) ldsm_x4(b1, x + (lane & 7) * 128 + (((half * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const int step = half * 2 + ks;
-        uint32_t a[2][4], b[NB > 1 ? NB / 2 : 1][4];
+      for (int kp = 0; kp < 2; ++kp) {  // 32 of K
+        uint32_t b1[4];
+        if (NB == 1) ldsm_x4(b1, x + (lane & 7) * 128 + (((kp * 4 + (lane >> 3)) ^ (lane & 7)) << 4));
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int row = rows + m * 16 + (lane & 15);
-          ldsm_x4(a[m], w + row * 128 + (((step * 2 + (lane >> 4)) ^ (row & 7)) << 4));
-        }
-        if (NB == 1) {
-          b[0][0] = b1[2 * ks], b[0][1] = b1[2 * ks + 1];
-        } else {
+        for (int ks = 0; ks < 2; ++ks) {
+          const int step = kp * 2 + ks;
+          uint32_t a[2][4], b[NB > 1 ? NB / 2 : 1][4];
 #pragma unroll
-          for (int j = 0; j < NB / 2; ++j) {
-            const int row = j * 16 + (lane & 7) + ((lane >> 4) << 3);
-            ldsm_x4(b[j], x + row * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+          for (int m = 0; m < 2; ++m) {
+            const int row = rows + m * 16 + (lane & 15);
+            ldsm_x4(a[m], w + row * 128 + (((step * 2 + (lane >> 4)) ^ (row & 7)) << 4));
           }
+          if (NB == 1) {
+            b[0][0] = b1[2 * ks], b[0][1] = b1[2 * ks + 1];
+          } else {
+#pragma unroll
+            for (int j = 0; j < NB / 2; ++j) {
+              const int row = j * 16 + (lane & 7) + ((lane >> 4) << 3);
+              ldsm_x4(b[j], x + row * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              mma_bf16(acc[m][j], a[m][0], a[m][1], a[m][2], a[m][3], b[j / 2][(j & 1) * 2], b[j / 2][(j & 1) * 2 + 1]);
         }
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-            mma_bf16(acc[m][j], a[m][0], a[m][1], a[m][2], a[m][3], b[j / 2][(j & 1) * 2], b[j / 2][(j & 1) * 2 + 1]);
       }
     } else {
       // A 16-byte piece of a row is 16 values of K. ldmatrix gives lane (g, c) the four at 4c: the product takes them as its k = 2c,
       // 2c + 1, 2c + 8 and 2c + 9, and the tokens' values likewise (the order of K is the product's own affair).
       float part[2][NB][4] = {};
 #pragma unroll
-      for (int kp = 0; kp < 2; ++kp) {
-        const int step = half * 4 + kp * 2;
+      for (int kp = 0; kp < 4; ++kp) {
+        const int step = kp * 2;
         uint32_t a[2][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -323,11 +350,10 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int blocks, int up_bord
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(ring.empty + 16 * ring.s);
-    ring.next();
+    ring.next_of_group(group, mine);
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (half == h) {
+  for (int h = 0; h < kXpGroups; ++h) {
+    if (group == h) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -351,20 +377,19 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 template <bool FP8, bool DOWN>
 __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ XpParams p) {
   extern __shared__ __align__(1024) unsigned char xp_smem[];
-  __shared__ int s_abort, s_named, s_last;
+  __shared__ int s_abort, s_route[2], s_last;
   const eux_experts_desc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entries = d.n_tokens * d.topk;
-  const XpLayout l = xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries);
+  const XpLayout l = xp_layout(DOWN, d.n_tokens, d.n_experts, entries);
   const uint32_t smem = smem_u32(xp_smem);
   XpRing ring;
-  ring.w = smem, ring.x = smem + l.x, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;
-  ring.stages = p.stages, ring.x_bytes = p.x_bytes;
+  ring.w = smem, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;
   if (threadIdx.x == 0) {
     s_abort = 0;
-    for (int i = 0; i < p.stages; ++i) {
+    for (int i = 0; i < kXpMaxStages; ++i) {
       mbar_init(ring.full + 16 * i, 1 + 32);
-      mbar_init(ring.empty + 16 * i, kXpWarps);
+      mbar_init(ring.empty + 16 * i, 4);  // the warps of a group
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
@@ -377,7 +402,11 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   r.first = reinterpret_cast<uint16_t*>(r.start + d.n_experts + 1);
   r.expert = r.first + d.n_experts + 1;
   r.order = r.expert + d.n_experts + 1;
-  xp_route(d, p.cap, r, reinterpret_cast<int*>(xp_smem), &s_named);
+  r.token = r.order + entries;
+  const int cap = xp_route(d, FP8 ? 32 : 64, r, reinterpret_cast<int*>(xp_smem), s_route);
+  ring.x_bytes = cap * (FP8 ? 256 : 128);
+  ring.stages = xp_stages(l.room, cap, ring.x_bytes);
+  ring.x = smem + ring.stages * kXpBlock;
   // the counts lay where weights are about to land
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
@@ -435,8 +464,8 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
         for (int i = lane; i < rows * pieces; i += 32) {
           const int row = i / pieces, piece = i % pieces, at = k * per_block + piece * 8;
           const bool some = row < s.n && at < K;
-          const int entry = r.order[s.pos + (row < s.n ? row : 0)];
-          const __nv_bfloat16* src = DOWN ? p.h + (int64_t)entry * d.inner : (const __nv_bfloat16*)d.x + (int64_t)(entry / d.topk) * d.x_stride;
+          const int pos = s.pos + (row < s.n ? row : 0);
+          const __nv_bfloat16* src = DOWN ? p.h + (int64_t)r.order[pos] * d.inner : (const __nv_bfloat16*)d.x + (int64_t)r.token[pos] * d.x_stride;
           const int swizzled = FP8 ? piece ^ ((row & 3) << 1) : piece ^ (row & 7);
           cp_async_16(dst + row * (pieces * 16) + swizzled * 16, src + (some ? at : 0), some ? 16 : 0);
         }
@@ -455,7 +484,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   } else {
     // ---- products ----
     if (DOWN) wait_for_launch_before();
-    float* const sum = reinterpret_cast<float*>(xp_smem + l.stage_sum);
+    float* const sum = reinterpret_cast<float*>(xp_smem + ring.stages * (kXpBlock + ring.x_bytes));
     float* const acc = reinterpret_cast<float*>(xp_smem + l.acc);
     const int tid = threadIdx.x;
     const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
@@ -465,8 +494,11 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       for (int64_t i = (int64_t)blockIdx.x * kXpConsumers + tid; i < (int64_t)d.n_tokens * (d.hidden / 8); i += (int64_t)gridDim.x * kXpConsumers)
         st_u4((__nv_bfloat16*)d.out + (i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
     }
+    int64_t mine = b0 + (warp >> 2);
+    ring.s = warp >> 2;
     for (int64_t b = b0; b < b1;) {
-      const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+      const int seg = (int)(b / nk);
+      const int64_t end = min((int64_t)(seg + 1) * nk, b1);
       const XpSegment s = walk.at(seg);
       const int tile = seg / tile_segs;
       const int64_t tile0 = tile * tile_blocks;
@@ -475,18 +507,18 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       }
       const int up_border = 128 - (d.inner + s.tile * 64) % 128;
       const int nb = (s.n + 7) >> 3;
-      if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, end - kb, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      b += end - kb;
+      if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      b = end;
       if (DOWN) {
-        // A thread has a row and the tokens of one parity: entries of the same token, also twice of the same expert, are added by one
+        // A thread has a row and every third token: entries of the same token, also twice of the same expert, are added by one
         // thread, in order.
-        const int row = tid & 127, parity = tid >> 7;
+        const int row = tid & 127, third = tid >> 7;
         for (int j = 0; j < s.n; ++j) {
-          const int entry = r.order[s.pos + j], t = entry / d.topk;
-          if ((t & 1) == parity) acc[t * kXpLd + row] = fmaf(__ldg(d.topk_w + entry), sum[j * kXpLd + row], acc[t * kXpLd + row]);
+          const int entry = r.order[s.pos + j], t = r.token[s.pos + j];
+          if (t % kXpGroups == third) acc[t * kXpLd + row] = fmaf(__ldg(d.topk_w + entry), sum[j * kXpLd + row], acc[t * kXpLd + row]);
         }
         consumers_meet();
       }
@@ -495,7 +527,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       const int first = (int)(((tile0 + 1) * grid - 1) / blocks), last = (int)(((tile0 + tile_blocks) * grid - 1) / blocks);
       const int rows = DOWN ? width : s.n;
       const float* const from = DOWN ? acc : sum;
-      bool mine = true;
+      bool all_there = true;
       if (first != last) {
         float* const part = p.part + ((int64_t)me * 2 + (me == first)) * p.part_rows * kXpRows;
         for (int i = tid; i < rows * (kXpRows / 4); i += kXpConsumers)
@@ -505,10 +537,10 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
         // counts up to the number of parts and starts again: ready for the next launch
         if (tid == 0) s_last = atomicInc(d.counters + (DOWN ? kXpMaxGrid : 0) + first, (unsigned)(last - first)) == (unsigned)(last - first);
         consumers_meet();
-        mine = s_last != 0;
-        if (mine) __threadfence();
+        all_there = s_last != 0;
+        if (all_there) __threadfence();
       }
-      if (mine) {
+      if (all_there) {
         constexpr int Q = DOWN ? kXpRows / 4 : 16;  // four rows of results per thread and step
         for (int i = tid; i < rows * Q; i += kXpConsumers) {
           const int j = i / Q, q = (i % Q) * 4;
@@ -582,14 +614,7 @@ static int experts_check(const eux_experts_desc* d) {
   if (d->hidden % unit || d->inner % unit || d->x_stride % 8 || d->out_stride % 8) return EUX_ERR_BAD_ARG;
   return 0;
 }
-// Tokens of an expert in a segment: what the accumulators hold, and with e4m3 weights what the products keep up with.
-// 8, 16, 32 or 64, as the products have them.
-static int xp_cap(const eux_experts_desc* d) {
-  int cap = 8;
-  while (cap < (d->fp8 ? 32 : 64) && cap < d->n_tokens * d->topk) cap *= 2;
-  return cap;
-}
-static int xp_part_rows(const eux_experts_desc* d) { return std::max(xp_cap(d), d->n_tokens); }
+static int xp_part_rows(const eux_experts_desc* d) { return std::max(64, d->n_tokens); }
 static size_t xp_h_bytes(const eux_experts_desc* d) { return ((size_t)d->n_tokens * d->topk * d->inner * 2 + 255) & ~(size_t)255; }
 
 static int xp_sms(int* dev) {
@@ -602,16 +627,11 @@ static int xp_sms(int* dev) {
 template <bool FP8, bool DOWN>
 static int xp_launch(const CUtensorMap& map, XpParams p, int dev, int sms, cudaStream_t st) {
   const eux_experts_desc& d = p.d;
-  p.x_bytes = p.cap * (FP8 ? 256 : 128);
-  const int entries = d.n_tokens * d.topk;
-  p.stages = kXpMaxStages;
-  // 1 KiB for the variables that the kernel declares itself
-  while (p.stages > 2 && (size_t)xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries).total > kXpSmem - 1024) --p.stages;
-  // the routing's counts lie in the ring before it is filled
-  const XpLayout l = xp_layout(DOWN, p.stages, p.x_bytes, p.cap, d.n_tokens, d.n_experts, entries);
-  if ((size_t)l.total > kXpSmem - 1024 || kXpThreads / 32 * d.n_experts * 4 > p.stages * kXpBlock) return EUX_ERR_TOO_LARGE;
-  if (cudaError_t e = allow_smem<moe_experts_kernel<FP8, DOWN>>(dev, kXpSmem - 1024); e != cudaSuccess) return (int)e;
-  return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, l.total, st, map, p);
+  // the ring holds a block of every group; the routing's counts lie where the ring will be
+  const int room = xp_layout(DOWN, d.n_tokens, d.n_experts, d.n_tokens * d.topk).room, most = FP8 ? 32 : 64;
+  if (xp_stages(room, most, most * (FP8 ? 256 : 128)) < kXpGroups || kXpThreads / 32 * d.n_experts * 4 > room) return EUX_ERR_TOO_LARGE;
+  if (cudaError_t e = allow_smem<moe_experts_kernel<FP8, DOWN>>(dev, kXpDynamic); e != cudaSuccess) return (int)e;
+  return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, kXpDynamic, st, map, p);
 }
 
 }  // namespace eux
@@ -638,7 +658,7 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   p.d = *d;
   p.h = (__nv_bfloat16*)d->workspace;
   p.part = (float*)((char*)d->workspace + xp_h_bytes(d));
-  p.part_rows = xp_part_rows(d), p.cap = xp_cap(d);
+  p.part_rows = xp_part_rows(d);
   int dev = 0;
   const int sms = xp_sms(&dev);
   if (int rc = d->fp8 ? xp_launch<true, false>(up, p, dev, sms, st) : xp_launch<false, false>(up, p, dev, sms, st)) return rc;
