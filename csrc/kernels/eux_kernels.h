@@ -255,11 +255,16 @@ typedef struct eux_experts_desc {
   void* workspace;             /* eux_experts_workspace_bytes, of this call alone until it ends */
   uint32_t* counters;          /* eux_experts_counter_words, zero on entry, zero on exit */
   uint32_t* status;
+  const void* maps;            /* host memory: what eux_experts_maps made for these weights */
   int64_t x_stride, out_stride;
   uint64_t wait_timeout_ns;
   int32_t n_tokens, hidden, inner, n_experts, topk;
   int32_t fp8;                 /* 0: bf16 weights; 1: e4m3 weights with one fp32 scale per 128 x 128 block */
 } eux_experts_desc;
+#define EUX_EXPERTS_MAPS_BYTES 256
+/* What the launches need to know of where the weights lie, into EUX_EXPERTS_MAPS_BYTES of host memory on 64 bytes; made once
+ * for weights that stay where they are. */
+EUX_API int eux_experts_maps(const eux_experts_desc* d, void* maps);
 EUX_API int eux_experts_launch(const eux_experts_desc* d, void* stream);
 EUX_API size_t eux_experts_workspace_bytes(const eux_experts_desc* d);
 EUX_API size_t eux_experts_counter_words(const eux_experts_desc* d);

@@ -26,6 +26,8 @@
 // that of the result's own rounding.
 #include <cuda.h>
 
+#include <limits.h>
+
 #include <algorithm>
 
 #include "eux_bulk.cuh"
@@ -96,22 +98,23 @@ __device__ __forceinline__ void lds_64(uint32_t& a, uint32_t& b, uint32_t at) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(at) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpConsumers) : "memory"); }
 
-// Two e4m3 values, bytes `lo` and `hi` of w as PRMT selectors have it, as bfloat16: sign, exponent and mantissa are moved to
-// their places, which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and
-// multiplied by 2^120. Both steps are exact. NaN (0x7f) would become 480: weights with NaN are refused when they are given.
-template <int SELECT>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-  const uint32_t t = __byte_perm(w, 0, SELECT);  // the bytes on top of each half
-  const uint32_t v = (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+// Four e4m3 values as bfloat16, bytes 0 and 2 in `even` and 1 and 3 in `odd`: sign, exponent and mantissa are moved to their places,
+// which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and multiplied by
+// 2^120. Both steps are exact. NaN (0x7f) would become 480: weights with NaN are refused when they are given.
+// The shifts to the left are written as products, which the pipe that multiplies can take: integer logic runs at half of a
+// warp's rate, and with six such instructions for four values instead of eight a block keeps an SM busy for ...
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t w4 = w * 16u, w8 = w * 256u, r4 = w >> 4;
+  const uint32_t e = (w4 & 0x07f007f0u) | (w8 & 0x80008000u), o = (r4 & 0x07f007f0u) | (w & 0x80008000u);
   const __nv_bfloat162 big = __floats2bfloat162_rn(0x1p120f, 0x1p120f);
-  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), big);
-  return *reinterpret_cast<uint32_t*>(&r);
+  const __nv_bfloat162 a = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&e), big), b = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&o), big);
+  even = *reinterpret_cast<const uint32_t*>(&a), odd = *reinterpret_cast<const uint32_t*>(&b);
 }
 
 // Which entries go to which expert, and the line of segments. The tables lie in shared memory and are the same in all CTAs:
@@ -165,11 +168,85 @@ struct XpWalk {
   }
 };
 
-// Counts and orders the entries. `counts` is scratch, [warps][n_experts]. Returns the tokens that a segment takes at most: 8, 16,
-// 32 or 64, as the expert with the most needs and `most` allows.
-__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* counts, int* out) {
+// The tables. Returns the tokens that a segment takes at most: 8, 16, 32 or 64, as the expert with the most needs and `most`
+// allows. `scratch` has room for [warps][n_experts] and for four words per thread; `out` for 2.
+//
+// With fewer entries than threads, the place of an entry is the number of entries that go before it, counted by comparing with all of
+// them; beyond, entries are counted per warp and expert. Either way the order is by expert and then by entry, in every CTA.
+__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* scratch, int* out) {
   const int E = d.n_experts, n = d.n_tokens * d.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int W = kXpThreads / 32;
+  const uint32_t below = (1u << lane) - 1u;
+  if (n < kXpThreads) {
+    int* const expert_of = scratch;              // [threads]
+    int* const sorted = scratch + kXpThreads;    // [threads]
+    int* const heads = scratch + 2 * kXpThreads; // [warps]
+    const int i = threadIdx.x;
+    int e = i < n ? d.topk_idx[i] : -1;
+    if ((uint32_t)e >= (uint32_t)E) e = INT_MAX;  // not here: behind all others
+    expert_of[i] = e;
+    if (i == 0) out[0] = 0;
+    __syncthreads();
+    if (warp * 32 < n) {
+      int at = 0;
+      for (int j = 0; j < n; j += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(expert_of + j);  // behind n: INT_MAX, and not before i
+        at += (o.x < e || (o.x == e && j < i)) + (o.y < e || (o.y == e && j + 1 < i)) + (o.z < e || (o.z == e && j + 2 < i)) + (o.w < e || (o.w == e && j + 3 < i));
+      }
+      if (i < n) {
+        sorted[at] = e;
+        r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)(i / d.topk);
+      }
+    }
+    __syncthreads();
+    const int mine = i < n ? sorted[i] : INT_MAX, last = i > 0 && i < n ? sorted[i - 1] : -1;
+    const uint32_t head = __ballot_sync(0xffffffffu, mine != last && mine != INT_MAX), some = __ballot_sync(0xffffffffu, mine != INT_MAX);
+    if (lane == 0) {
+      heads[warp] = __popc(head);
+      if (some) atomicAdd(out, __popc(some));  // the entries that are here
+    }
+    __syncthreads();
+    int before = 0, named = 0;
+    for (int w = 0; w < W; ++w) {
+      before += w < warp ? heads[w] : 0;
+      named += heads[w];
+    }
+    const int here = out[0];
+    if ((head >> lane) & 1u) {
+      const int a = before + __popc(head & below);
+      r.start[a] = i, r.expert[a] = (uint16_t)mine;
+    }
+    if (i == 0) r.start[named] = here, out[1] = 0;
+    __syncthreads();
+    int top = 0;
+    if (i < named) top = r.start[i + 1] - r.start[i];
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0 && top) atomicMax(out + 1, top);
+    if (i <= named) r.first[i] = (uint16_t)i;  // a chunk each, if that does
+    __syncthreads();
+    int cap = 8;
+    while (cap < out[1] && cap < most) cap *= 2;
+    if (out[1] > most) {
+      if (warp == 0) {
+        int chunks = 0;
+        for (int a0 = 0; a0 < named; a0 += 32) {
+          const int a = a0 + lane, ch = a < named ? (r.start[a + 1] - r.start[a] + cap - 1) / cap : 0;
+          int sum = ch;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+          }
+          if (a < named) r.first[a] = (uint16_t)(chunks + sum - ch);
+          chunks += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) r.first[named] = (uint16_t)chunks;
+      }
+      __syncthreads();
+    }
+    r.named = named;
+    return cap;
+  }
+  int* const counts = scratch;
   const int each = ((n + W - 1) / W + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
   for (int i = threadIdx.x; i < W * E; i += kXpThreads) counts[i] = 0;
   __syncthreads();
@@ -202,7 +279,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
         if (lane >= o) c_sum += u, ch_sum += v;
       }
       if (c > 0) {
-        const int a = named + __popc(has & ((1u << lane) - 1u));
+        const int a = named + __popc(has & below);
         r.expert[a] = (uint16_t)e, r.start[a] = at + c_sum - c, r.first[a] = (uint16_t)(chunks + ch_sum - ch);
         // from counts to places: where each warp's entries of this expert go
         int p = at + c_sum - c;
@@ -223,7 +300,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
     const int e = i < hi ? d.topk_idx[i] : -1;
     const bool here = (uint32_t)e < (uint32_t)E;
     const uint32_t same = __match_any_sync(0xffffffffu, here ? e : -1);
-    const int before = __popc(same & ((1u << lane) - 1u));
+    const int before = __popc(same & below);
     if (here) {
       const int at = counts[warp * E + e] + before;
       r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)(i / d.topk);
@@ -300,8 +377,8 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
         }
       }
     } else {
-      // A 16-byte piece of a row is 16 values of K. ldmatrix gives lane (g, c) the four at 4c: the product takes them as its k = 2c,
-      // 2c + 1, 2c + 8 and 2c + 9, and the tokens' values likewise (the order of K is the product's own affair).
+      // A 16-byte piece of a row is 16 values of K. ldmatrix gives lane (g, c) the four at 4c: the first and the third are the product's k = 2c
+      // and 2c + 1, the others 2c + 8 and 2c + 9, and the tokens' values are paired likewise (the order of K is the product's own affair).
       float part[2][NB][4] = {};
 #pragma unroll
       for (int kp = 0; kp < 4; ++kp) {
@@ -318,13 +395,14 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint32_t r0 = a[m][2 * ks], r1 = a[m][2 * ks + 1];
-            wa[m][0] = widen<0x1404>(r0), wa[m][1] = widen<0x1404>(r1), wa[m][2] = widen<0x3424>(r0), wa[m][3] = widen<0x3424>(r1);
+            widen(r0, wa[m][0], wa[m][2]), widen(r1, wa[m][1], wa[m][3]);
           }
 #pragma unroll
           for (int j = 0; j < NB; ++j) {
             const int row = j * 8 + g;
-            uint32_t b0, b1;
-            lds_64(b0, b1, x + row * 256 + ((((step + ks) * 2 + (c >> 1)) ^ ((row & 3) << 1)) << 4) + (c & 1) * 8);
+            uint32_t x0, x1;
+            lds_64(x0, x1, x + row * 256 + ((((step + ks) * 2 + (c >> 1)) ^ ((row & 3) << 1)) << 4) + (c & 1) * 8);
+            const uint32_t b0 = __byte_perm(x0, x1, 0x5410), b1 = __byte_perm(x0, x1, 0x7632);
 #pragma unroll
             for (int m = 0; m < 2; ++m) mma_bf16(part[m][j], wa[m][0], wa[m][1], wa[m][2], wa[m][3], b0, b1);
           }
@@ -642,18 +720,23 @@ extern "C" size_t eux_experts_workspace_bytes(const eux_experts_desc* d) {
   if (experts_check(d)) return 0;
   return xp_h_bytes(d) + (size_t)kXpMaxGrid * 2 * xp_part_rows(d) * kXpRows * 4;
 }
+extern "C" int eux_experts_maps(const eux_experts_desc* d, void* maps) {
+  if (int rc = experts_check(d)) return rc;
+  if (!d->w_gate_up || !d->w_down || !maps || ((uintptr_t)d->w_gate_up | (uintptr_t)d->w_down) & 15 || (uintptr_t)maps & 63) return EUX_ERR_BAD_ARG;
+  CUtensorMap* const m = (CUtensorMap*)maps;
+  if (int rc = xp_map(m, d->w_gate_up, d->fp8, 2 * (uint64_t)d->n_experts, d->inner, d->hidden, 64)) return rc;
+  return xp_map(m + 1, d->w_down, d->fp8, d->n_experts, d->hidden, d->inner, kXpRows);
+}
 extern "C" size_t eux_experts_counter_words(const eux_experts_desc* d) { return experts_check(d) ? 0 : 2 * kXpMaxGrid; }
 
 extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   if (int rc = experts_check(d)) return rc;
   if (d->n_tokens == 0) return 0;
-  if (!d->x || !d->topk_idx || !d->topk_w || !d->out || !d->w_gate_up || !d->w_down || !d->workspace || !d->counters) return EUX_ERR_BAD_ARG;
+  if (!d->x || !d->topk_idx || !d->topk_w || !d->out || !d->w_gate_up || !d->w_down || !d->workspace || !d->counters || !d->maps) return EUX_ERR_BAD_ARG;
   if (d->fp8 && (!d->gate_up_scale || !d->down_scale)) return EUX_ERR_BAD_ARG;
-  if (((uintptr_t)d->x | (uintptr_t)d->out | (uintptr_t)d->w_gate_up | (uintptr_t)d->w_down | (uintptr_t)d->workspace) & 15) return EUX_ERR_BAD_ARG;
+  if (((uintptr_t)d->x | (uintptr_t)d->out | (uintptr_t)d->w_gate_up | (uintptr_t)d->w_down | (uintptr_t)d->workspace) & 15 || (uintptr_t)d->maps & 63) return EUX_ERR_BAD_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
-  CUtensorMap up, down;
-  if (int rc = xp_map(&up, d->w_gate_up, d->fp8, 2 * (uint64_t)d->n_experts, d->inner, d->hidden, 64)) return rc;
-  if (int rc = xp_map(&down, d->w_down, d->fp8, d->n_experts, d->hidden, d->inner, kXpRows)) return rc;
+  const CUtensorMap *up = (const CUtensorMap*)d->maps, *down = up + 1;
   XpParams p = {};
   p.d = *d;
   p.h = (__nv_bfloat16*)d->workspace;
@@ -661,8 +744,8 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   p.part_rows = xp_part_rows(d);
   int dev = 0;
   const int sms = xp_sms(&dev);
-  if (int rc = d->fp8 ? xp_launch<true, false>(up, p, dev, sms, st) : xp_launch<false, false>(up, p, dev, sms, st)) return rc;
-  return d->fp8 ? xp_launch<true, true>(down, p, dev, sms, st) : xp_launch<false, true>(down, p, dev, sms, st);
+  if (int rc = d->fp8 ? xp_launch<true, false>(*up, p, dev, sms, st) : xp_launch<false, false>(*up, p, dev, sms, st)) return rc;
+  return d->fp8 ? xp_launch<true, true>(*down, p, dev, sms, st) : xp_launch<false, true>(*down, p, dev, sms, st);
 }
 
 extern "C" int eux_experts_preload(void) {

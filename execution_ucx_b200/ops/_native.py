@@ -84,7 +84,7 @@ class ExpertsDesc(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("topk_idx", C.c_void_p), ("topk_w", C.c_void_p), ("out", C.c_void_p), ("w_gate_up", C.c_void_p),
         ("w_down", C.c_void_p), ("gate_up_scale", C.c_void_p), ("down_scale", C.c_void_p), ("workspace", C.c_void_p),
-        ("counters", C.c_void_p), ("status", C.c_void_p), ("x_stride", C.c_int64), ("out_stride", C.c_int64),
+        ("counters", C.c_void_p), ("status", C.c_void_p), ("maps", C.c_void_p), ("x_stride", C.c_int64), ("out_stride", C.c_int64),
         ("wait_timeout_ns", C.c_uint64), ("n_tokens", C.c_int32), ("hidden", C.c_int32), ("inner", C.c_int32),
         ("n_experts", C.c_int32), ("topk", C.c_int32), ("fp8", C.c_int32),
     ]
@@ -106,7 +106,7 @@ XFER_TAIL = struct.Struct("<8Q")
 MOE_DESC = struct.Struct("<8i12Q")
 GEMM_DESC = struct.Struct("<7Q4i6Q2i")
 ROUTE_DESC = struct.Struct("<4Qq8ifi")
-EXPERTS_DESC = struct.Struct("<11Q2qQ6i")
+EXPERTS_DESC = struct.Struct("<12Q2qQ6i")
 LORA_DESC = struct.Struct("<8Q3q6i")
 assert ROUTE_DESC.size == C.sizeof(RouteDesc) and EXPERTS_DESC.size == C.sizeof(ExpertsDesc) and LORA_DESC.size == C.sizeof(LoraDesc)
 assert XFER_HEAD.size + XFER_DIMS.size + XFER_TAIL.size == C.sizeof(XferDesc)
@@ -162,6 +162,7 @@ def load():
     lib.eux_moe_combine_launch.argtypes = [P, I, P]
     for op in ("route", "experts", "lora"):
         getattr(lib, f"eux_{op}_launch").argtypes = [P, P]
+    lib.eux_experts_maps.argtypes = [P, P]
     for size in ("eux_experts_workspace_bytes", "eux_experts_counter_words", "eux_lora_workspace_bytes"):
         getattr(lib, size).argtypes = [P]
         getattr(lib, size).restype = C.c_size_t

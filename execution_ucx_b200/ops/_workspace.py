@@ -48,10 +48,10 @@ def require_cuda(device) -> None:
 
 
 class on_device:
-    """The given device as the current one, and its current stream: ``with on_device(d) as stream``."""
+    """The given device as the current one, and its current stream: ``with on_device(index) as stream``."""
 
-    def __init__(self, device):
-        self.index = device.index
+    def __init__(self, index: int):
+        self.index = index
 
     def __enter__(self) -> int:
         self.before = torch.cuda.current_device()
@@ -64,10 +64,10 @@ class on_device:
             torch.cuda.set_device(self.before)
 
 
-class CallCounters:
-    """Zeroed words for calls of a kernel that leaves them zeroed. Calls that may run at the same time get words of their
-    own: those of one stream share some, and every captured call has its own, since graphs may be replayed beside each
-    other and beside plain calls."""
+class CallScratch:
+    """Memory for calls of a kernel: a workspace, and zeroed words that the kernel leaves zeroed. Calls that may run at the
+    same time get memory of their own: those of one stream share some, and every captured call has its own, since graphs may
+    be replayed beside each other and beside plain calls."""
 
     SLOTS = 16
 
@@ -75,24 +75,29 @@ class CallCounters:
         self.words, self.device = words, device
         self._of_stream = {}
         self._kept = []
-        with on_device(device):
-            self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0))
+        with on_device(device.index):
+            self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0)) if words else []
             torch.cuda.current_stream().synchronize()  # captured calls run on any stream
 
-    def get(self, stream: int) -> torch.Tensor:
+    def get(self, stream: int, need: int):
+        """The addresses of ``need`` bytes and of the words, for a call on ``stream``, the current one."""
         if torch.cuda.is_current_stream_capturing():
-            # zeroed by the graph itself once the words that were zeroed beforehand are given out
-            t = self._spare.pop() if self._spare else torch.zeros(self.words, dtype=torch.int32, device=self.device)
-            self._kept.append(t)
-            return t
-        t = self._of_stream.get(stream)
-        if t is None:
-            t = self._of_stream[stream] = torch.zeros(self.words, dtype=torch.int32, device=self.device)
-        return t
+            # In a capture a tensor's memory is the graph's; the words are zeroed by the graph itself once those that were
+            # zeroed beforehand are given out.
+            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            words = self._spare.pop() if self._spare else torch.zeros(self.words, dtype=torch.int32, device=self.device)
+            self._kept.append(words)
+            return workspace.data_ptr(), words.data_ptr()
+        mine = self._of_stream.get(stream)
+        if mine is None or mine[2] < need:
+            words = mine[1] if mine else torch.zeros(self.words, dtype=torch.int32, device=self.device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            mine = self._of_stream[stream] = (workspace, words, need, (workspace.data_ptr(), words.data_ptr()))
+        return mine[3]
 
     def reset(self) -> None:
         """Zeroes all words, after a kernel that gave up: with nothing in flight."""
-        for t in [*self._of_stream.values(), *self._kept]:
+        for t in [m[1] for m in self._of_stream.values()] + self._kept:
             t.zero_()
 
 

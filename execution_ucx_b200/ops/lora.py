@@ -44,36 +44,60 @@ class LoraAdapters:
         ws.require_device(self.device, b=b, scale=scale)
         ws.require_cuda(self.device)
         ws.require((a.data_ptr() | b.data_ptr()) % 16 == 0, "a and b must begin on 16 bytes")
-        self.a, self.b = a, b
-        self.scale = scale if scale is not None else torch.ones(self.n_adapters, dtype=torch.float32, device=self.device)
+        scale = scale if scale is not None else torch.ones(self.n_adapters, dtype=torch.float32, device=self.device)
+        self._weights = (a, b, scale)
+        self._weight_ptrs = (a.data_ptr(), b.data_ptr(), scale.data_ptr())
+        self._index = self.device.index
+        self._need = {}
+        self._scratch = ws.CallScratch(0, self.device)
         _native.load()
+
+    a = property(lambda self: self._weights[0])
+    b = property(lambda self: self._weights[1])
+    scale = property(lambda self: self._weights[2])
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` is ``[tokens, K]`` and ``y`` ``[tokens, N]``, bfloat16; ``ids`` ``[tokens]``, int32, names each token's adapter. A
         token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``; the rows
         of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
         global _launches
+        if not (isinstance(x, torch.Tensor) and isinstance(ids, torch.Tensor) and isinstance(y, torch.Tensor)
+                and x.dtype is torch.bfloat16 and y.dtype is torch.bfloat16 and ids.dtype is torch.int32
+                and x.dim() == y.dim() == 2 and ids.dim() == 1 and x.shape[0] == y.shape[0] == ids.shape[0]
+                and x.shape[1] == self.K and y.shape[1] == self.N and x.is_contiguous() and y.is_contiguous() and ids.is_contiguous()
+                and (x.data_ptr() | y.data_ptr()) % 16 == 0 and x.get_device() == y.get_device() == ids.get_device() == self._index):
+            self._require(x, ids, y)
+        t = ids.shape[0]
+        if out is None:
+            out = torch.empty(t, self.N, dtype=torch.bfloat16, device=self.device)
+        else:
+            ws.require_rows(out, "out", torch.bfloat16, cols=self.N, rows=t)
+            ws.require_device(self.device, out=out)
+        if t == 0:
+            return out
+        lib = _native.load()
+        need = self._need.get(t)
+        if need is None:
+            need = self._need[t] = int(lib.eux_lora_workspace_bytes(self._desc(t)))
+        with ws.on_device(self._index) as stream:
+            workspace, _ = self._scratch.get(stream, need)
+            rc = lib.eux_lora_launch(self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, ws.row_stride(x),
+                                                ws.row_stride(y), ws.row_stride(out)), stream)
+        if rc:
+            _native.check(rc, "eux_lora_launch")
+        _launches += 1
+        return out
+
+    def _desc(self, tokens, x=0, ids=0, y=0, out=0, workspace=0, x_stride=0, y_stride=0, out_stride=0):
+        return _native.descriptor(_native.LORA_DESC, _native.LoraDesc, x, ids, y, out, *self._weight_ptrs, workspace, x_stride, y_stride, out_stride,
+                                  tokens, self.K, self.N, self.rank, self.n_adapters, 0)
+
+    def _require(self, x, ids, y) -> None:
         ws.require_rows(x, "x", torch.bfloat16, cols=self.K)
         t = x.shape[0]
         ws.require_rows(y, "y", torch.bfloat16, cols=self.N, rows=t)
         ws.require_dense(ids, "ids", torch.int32, (t,))
-        if out is not None:
-            ws.require_rows(out, "out", torch.bfloat16, cols=self.N, rows=t)
-        ws.require_device(self.device, x=x, ids=ids, y=y, out=out)
-        if out is None:
-            out = torch.empty(t, self.N, dtype=torch.bfloat16, device=self.device)
-        if t == 0:
-            return out
-        lib = _native.load()
-        desc = lambda workspace: _native.descriptor(  # noqa: E731
-            _native.LORA_DESC, _native.LoraDesc, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), self.a.data_ptr(), self.b.data_ptr(),
-            self.scale.data_ptr(), workspace, ws.row_stride(x), ws.row_stride(y), ws.row_stride(out), t, self.K, self.N, self.rank,
-            self.n_adapters, 0)
-        with ws.on_device(self.device) as stream:
-            workspace = torch.empty(lib.eux_lora_workspace_bytes(desc(0)), dtype=torch.uint8, device=self.device)
-            ws.check(lib.eux_lora_launch(desc(workspace.data_ptr()), stream), "eux_lora_launch")
-        _launches += 1
-        return out
+        ws.require_device(self.device, x=x, ids=ids, y=y)
 
 
 def reference(x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:

@@ -12,6 +12,7 @@ whose experts are on this GPU, or the experts of rows that a dispatch has brough
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import List, Optional, Tuple
 
 import torch
@@ -165,27 +166,40 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: Op
     ``topk`` are left, the last places are expert -1 with weight 0. A logit of +inf weighs as the largest number does."""
     global _launches
     ws.require(isinstance(logits, torch.Tensor) and logits.dim() == 2, "logits must be a matrix")
-    ws.require(logits.dtype in (torch.float32, torch.bfloat16), f"logits must be float32 or bfloat16, not {logits.dtype}")
+    dtype = logits.dtype
     t, e = logits.shape
-    ws.require(1 <= e <= ROUTE_MAX_EXPERTS, f"there must be 1 to {ROUTE_MAX_EXPERTS} experts, not {e}")
-    ws.require(e == 1 or logits.stride(1) == 1, "a token's logits must lie side by side")
-    ws.require(1 <= topk <= min(32, e), f"topk must be 1 to {min(32, e)}, not {topk}")
-    ws.require(scoring in ("softmax", "sigmoid"), f"scoring must be softmax or sigmoid, not {scoring!r}")
-    ws.require(1 <= groups <= 32 and e % groups == 0, f"{e} experts are not {groups} groups (of up to 32)")
-    ws.require(1 <= topk_groups <= groups, f"topk_groups must be 1 to {groups}, not {topk_groups}")
+    stride, inner_stride = logits.stride()
+    if not (dtype is torch.float32 or dtype is torch.bfloat16):
+        raise ValueError(f"logits must be float32 or bfloat16, not {dtype}")
+    if not 1 <= e <= ROUTE_MAX_EXPERTS:
+        raise ValueError(f"there must be 1 to {ROUTE_MAX_EXPERTS} experts, not {e}")
+    if inner_stride != 1 and e != 1:
+        raise ValueError("a token's logits must lie side by side")
+    if not 1 <= topk <= min(32, e):
+        raise ValueError(f"topk must be 1 to {min(32, e)}, not {topk}")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"scoring must be softmax or sigmoid, not {scoring!r}")
+    if not 1 <= groups <= 32 or e % groups:
+        raise ValueError(f"{e} experts are not {groups} groups (of up to 32)")
+    if not 1 <= topk_groups <= groups:
+        raise ValueError(f"topk_groups must be 1 to {groups}, not {topk_groups}")
+    device = logits.device
     if bias is not None:
         ws.require_dense(bias, "bias", torch.float32, (e,))
-    device = logits.device
-    ws.require_device(device, bias=bias)
+        ws.require_device(device, bias=bias)
     ws.require_cuda(device)
-    idx = torch.empty(t, topk, dtype=torch.int32, device=device)
-    w = torch.empty(t, topk, dtype=torch.float32, device=device)
+    # one allocation for both: the weights behind the indices
+    both = torch.empty(2, t, topk, dtype=torch.int32, device=device)
+    idx, w = both[0], both[1].view(torch.float32)
     if t:
+        at = both.data_ptr()
         desc = _native.descriptor(_native.ROUTE_DESC, _native.RouteDesc, logits.data_ptr(), bias.data_ptr() if bias is not None else 0,
-                                  idx.data_ptr(), w.data_ptr(), ws.row_stride(logits), t, e, topk, _native.torch_dtype_code(logits.dtype),
+                                  at, at + 4 * t * topk, stride, t, e, topk, _native.DT_F32 if dtype is torch.float32 else _native.DT_BF16,
                                   int(scoring == "sigmoid"), groups, topk_groups, int(renormalize), float(scale), 0)
-        with ws.on_device(device) as stream:
-            ws.check(_native.load().eux_route_launch(desc, stream), "eux_route_launch")
+        with ws.on_device(device.index) as stream:
+            rc = _native.load().eux_route_launch(desc, stream)
+        if rc:
+            _native.check(rc, "eux_route_launch")
         _launches += 1
     return idx, w
 
@@ -234,17 +248,28 @@ class MoeExperts:
             # the kernels widen e4m3 by moving bits, which has no place for NaN
             nan = sum(((w[j].view(torch.uint8) & 0x7F) == 0x7F).any() for w in (w_gate_up, w_down) for j in range(e))
             ws.require(int(nan) == 0, "e4m3 weights must not be NaN")
-        self.w_gate_up, self.w_down, self.gate_up_scale, self.down_scale = w_gate_up, w_down, gate_up_scale, down_scale
+        self._weights = (w_gate_up, w_down, gate_up_scale, down_scale)
+        self._weight_ptrs = tuple(w.data_ptr() if w is not None else 0 for w in self._weights)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        words = _native.load().eux_experts_counter_words(self._desc(self.MAX_TOKENS, 1))
-        self._counters = ws.CallCounters(int(words), self.device)
+        self._status_ptr, self._index = self.status.data_ptr(), self.device.index
+        self._need = {}
+        lib = _native.load()
+        self._room = C.create_string_buffer(256 + 64)
+        self._maps = (C.addressof(self._room) + 63) & ~63
+        with ws.on_device(self._index):
+            ws.check(lib.eux_experts_maps(self._desc(1, 1), self._maps), "eux_experts_maps")
+        self._scratch = ws.CallScratch(int(lib.eux_experts_counter_words(self._desc(1, 1))), self.device)
+
+    w_gate_up = property(lambda self: self._weights[0])
+    w_down = property(lambda self: self._weights[1])
+    gate_up_scale = property(lambda self: self._weights[2])
+    down_scale = property(lambda self: self._weights[3])
 
     def _desc(self, tokens, topk, x=0, idx=0, w=0, out=0, workspace=0, counters=0, x_stride=0, out_stride=0):
         """An ``eux_experts_desc`` of one pass."""
         return _native.descriptor(
-            _native.EXPERTS_DESC, _native.ExpertsDesc, x, idx, w, out, self.w_gate_up.data_ptr(), self.w_down.data_ptr(),
-            self.gate_up_scale.data_ptr() if self.fp8 else 0, self.down_scale.data_ptr() if self.fp8 else 0, workspace, counters,
-            self.status.data_ptr(), x_stride, out_stride, 2_000_000_000, tokens, self.hidden, self.inner, self.n_experts, topk, int(self.fp8))
+            _native.EXPERTS_DESC, _native.ExpertsDesc, x, idx, w, out, *self._weight_ptrs, workspace, counters, self._status_ptr, self._maps,
+            x_stride, out_stride, 2_000_000_000, tokens, self.hidden, self.inner, self.n_experts, topk, int(self.fp8))
 
     def __call__(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` is ``[tokens, hidden]`` bfloat16, ``topk_idx`` (int32) and ``topk_w`` (float32) are ``[tokens, topk]``, up to 32
@@ -253,6 +278,38 @@ class MoeExperts:
         ``out`` may be ``x`` itself; the rows of both may lie apart. Sums are in float32; what lies between the two products is
         rounded to bfloat16. The same arguments give the same bits."""
         global _launches
+        index, hidden = self._index, self.hidden
+        # what a call usually brings, with as few questions as tell it from everything else
+        if not (isinstance(x, torch.Tensor) and isinstance(topk_idx, torch.Tensor) and isinstance(topk_w, torch.Tensor)
+                and x.dtype is torch.bfloat16 and topk_idx.dtype is torch.int32 and topk_w.dtype is torch.float32
+                and x.dim() == topk_idx.dim() == 2 and topk_idx.shape == topk_w.shape and x.shape[0] == topk_idx.shape[0]
+                and x.shape[1] == hidden and 1 <= topk_idx.shape[1] <= 32
+                and x.is_contiguous() and topk_idx.is_contiguous() and topk_w.is_contiguous() and x.data_ptr() % 16 == 0
+                and x.get_device() == topk_idx.get_device() == topk_w.get_device() == index):
+            self._require(x, topk_idx, topk_w)
+        t, topk = topk_idx.shape
+        if out is None:
+            out = torch.empty(t, hidden, dtype=torch.bfloat16, device=self.device)
+        else:
+            ws.require_rows(out, "out", torch.bfloat16, cols=hidden, rows=t)
+            ws.require_device(self.device, out=out)
+        lib = _native.load()
+        xs, os_ = ws.row_stride(x), ws.row_stride(out)
+        with ws.on_device(index) as stream:
+            for first in range(0, t, self.MAX_TOKENS):
+                n = min(self.MAX_TOKENS, t - first)
+                need = self._need.get((n, topk))
+                if need is None:
+                    need = self._need[n, topk] = int(lib.eux_experts_workspace_bytes(self._desc(n, topk)))
+                workspace, counters = self._scratch.get(stream, need)
+                rc = lib.eux_experts_launch(self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk,
+                                                       topk_w.data_ptr() + 4 * first * topk, out.data_ptr() + 2 * first * os_, workspace, counters, xs, os_), stream)
+                if rc:
+                    _native.check(rc, "eux_experts_launch")
+                _launches += 2
+        return out
+
+    def _require(self, x, topk_idx, topk_w) -> None:
         ws.require_rows(x, "x", torch.bfloat16, cols=self.hidden)
         t = x.shape[0]
         ws.require(isinstance(topk_idx, torch.Tensor) and topk_idx.dim() == 2 and topk_idx.shape[0] == t, f"topk_idx must be [{t}, topk]")
@@ -260,29 +317,12 @@ class MoeExperts:
         ws.require(1 <= topk <= 32, f"topk must be 1 to 32, not {topk}")
         ws.require_dense(topk_idx, "topk_idx", torch.int32, (t, topk))
         ws.require_dense(topk_w, "topk_w", torch.float32, (t, topk))
-        if out is not None:
-            ws.require_rows(out, "out", torch.bfloat16, cols=self.hidden, rows=t)
-        ws.require_device(self.device, x=x, topk_idx=topk_idx, topk_w=topk_w, out=out)
-        if out is None:
-            out = torch.empty(t, self.hidden, dtype=torch.bfloat16, device=self.device)
-        lib = _native.load()
-        xs, os_ = ws.row_stride(x), ws.row_stride(out)
-        with ws.on_device(self.device) as stream:
-            counters = self._counters.get(stream)
-            for first in range(0, t, self.MAX_TOKENS):
-                n = min(self.MAX_TOKENS, t - first)
-                need = lib.eux_experts_workspace_bytes(self._desc(n, topk))
-                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-                desc = self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk, topk_w.data_ptr() + 4 * first * topk,
-                                  out.data_ptr() + 2 * first * os_, workspace.data_ptr(), counters.data_ptr(), xs, os_)
-                ws.check(lib.eux_experts_launch(desc, stream), "eux_experts_launch")
-                _launches += 2
-        return out
+        ws.require_device(self.device, x=x, topk_idx=topk_idx, topk_w=topk_w)
 
     def check_status(self) -> None:
         s = int(self.status.item())
         if s:
-            self._counters.reset()
+            self._scratch.reset()
             self.status.zero_()
             raise RuntimeError(f"moe experts status code={s & 0xff} where={s >> 8}")
 
