@@ -13,8 +13,8 @@
 //   results, it leaves its part in a workspace, and the last to come adds the parts up, in the order of the SMs. For the down
 //   form a tile is 128 rows of the output with all experts, so the weighted sum over a token's experts is made in shared
 //   memory, and only what an SM's share cuts goes through the workspace.
-// * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp fetches the tokens' values beside them
-//   with cp.async (rows are gathered: any tokens, any order), twelve warps multiply. The ring runs on
+// * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp the tokens' values beside them
+//   the same way (rows are gathered, four by a copy: any tokens, any order), twelve warps multiply. The ring runs on
 //   over the borders of segments; the down form's starts before the up form has ended (programmatic dependent launch), since
 //   weights wait for nobody.
 // * The weights are the first operand of mma.sync m16n8k16 and the tokens the second: 8 columns are the smallest padding for
@@ -25,8 +25,6 @@
 // Sums are float32 throughout. h is rounded to bfloat16, which its product takes; its error, 2^-9 of each term on average, is
 // that of the result's own rounding.
 #include <cuda.h>
-
-#include <limits.h>
 
 #include <algorithm>
 
@@ -81,16 +79,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
                "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {  // what is not read is zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Four rows of a matrix, 128 bytes of each from column x on, to four rows of 128 bytes
+__device__ __forceinline__ void tma_gather_4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, const int (&y)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {  // when this thread's copies so far have landed
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -169,135 +164,71 @@ struct XpWalk {
 };
 
 // The tables. Returns the tokens that a segment takes at most: 8, 16, 32 or 64, as the expert with the most needs and `most`
-// allows. `scratch` has room for [warps][n_experts] and for four words per thread; `out` for 2.
-//
-// With fewer entries than threads, the place of an entry is the number of entries that go before it, counted by comparing with all of
-// them; beyond, entries are counted per warp and expert. Either way the order is by expert and then by entry, in every CTA.
-__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* scratch, int* out) {
+// allows. `counts` is scratch, [warps][n_experts]; `out` has room for 4 and two words per warp. Entries are counted per warp and
+// expert, and their places follow: by expert and then by entry, the same in every CTA.
+__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* counts, int* out) {
   const int E = d.n_experts, n = d.n_tokens * d.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int W = kXpThreads / 32;
   const uint32_t below = (1u << lane) - 1u;
-  if (n < kXpThreads) {
-    int* const expert_of = scratch;              // [threads]
-    int* const sorted = scratch + kXpThreads;    // [threads]
-    int* const heads = scratch + 2 * kXpThreads; // [warps]
-    const int i = threadIdx.x;
-    int e = i < n ? d.topk_idx[i] : -1;
-    if ((uint32_t)e >= (uint32_t)E) e = INT_MAX;  // not here: behind all others
-    expert_of[i] = e;
-    if (i == 0) out[0] = 0;
-    __syncthreads();
-    if (warp * 32 < n) {
-      int at = 0;
-      for (int j = 0; j < n; j += 4) {
-        const int4 o = *reinterpret_cast<const int4*>(expert_of + j);  // behind n: INT_MAX, and not before i
-        at += (o.x < e || (o.x == e && j < i)) + (o.y < e || (o.y == e && j + 1 < i)) + (o.z < e || (o.z == e && j + 2 < i)) + (o.w < e || (o.w == e && j + 3 < i));
-      }
-      if (i < n) {
-        sorted[at] = e;
-        r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)(i / d.topk);
-      }
-    }
-    __syncthreads();
-    const int mine = i < n ? sorted[i] : INT_MAX, last = i > 0 && i < n ? sorted[i - 1] : -1;
-    const uint32_t head = __ballot_sync(0xffffffffu, mine != last && mine != INT_MAX), some = __ballot_sync(0xffffffffu, mine != INT_MAX);
-    if (lane == 0) {
-      heads[warp] = __popc(head);
-      if (some) atomicAdd(out, __popc(some));  // the entries that are here
-    }
-    __syncthreads();
-    int before = 0, named = 0;
-    for (int w = 0; w < W; ++w) {
-      before += w < warp ? heads[w] : 0;
-      named += heads[w];
-    }
-    const int here = out[0];
-    if ((head >> lane) & 1u) {
-      const int a = before + __popc(head & below);
-      r.start[a] = i, r.expert[a] = (uint16_t)mine;
-    }
-    if (i == 0) r.start[named] = here, out[1] = 0;
-    __syncthreads();
-    int top = 0;
-    if (i < named) top = r.start[i + 1] - r.start[i];
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top) atomicMax(out + 1, top);
-    if (i <= named) r.first[i] = (uint16_t)i;  // a chunk each, if that does
-    __syncthreads();
-    int cap = 8;
-    while (cap < out[1] && cap < most) cap *= 2;
-    if (out[1] > most) {
-      if (warp == 0) {
-        int chunks = 0;
-        for (int a0 = 0; a0 < named; a0 += 32) {
-          const int a = a0 + lane, ch = a < named ? (r.start[a + 1] - r.start[a] + cap - 1) / cap : 0;
-          int sum = ch;
-          for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-          }
-          if (a < named) r.first[a] = (uint16_t)(chunks + sum - ch);
-          chunks += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (lane == 0) r.first[named] = (uint16_t)chunks;
-      }
-      __syncthreads();
-    }
-    r.named = named;
-    return cap;
-  }
-  int* const counts = scratch;
-  const int each = ((n + W - 1) / W + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
-  for (int i = threadIdx.x; i < W * E; i += kXpThreads) counts[i] = 0;
+  int *const sums = out + 4, *const heads = sums + W;
+  const int used = min(W, (n + 31) / 32);  // warps that have entries
+  const int each = ((n + used - 1) / used + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
+  const int e_first = lo + lane < hi ? d.topk_idx[lo + lane] : -1;
+  for (int i = threadIdx.x; i < used * E; i += kXpThreads) counts[i] = 0;
+  if (threadIdx.x == 0) out[0] = 0;
   __syncthreads();
   for (int i = lo + lane; i < hi; i += 32) {
-    const int e = d.topk_idx[i];
+    const int e = i == lo + lane ? e_first : d.topk_idx[i];
     if ((uint32_t)e < (uint32_t)E) atomicAdd(&counts[warp * E + e], 1);
   }
   __syncthreads();
-  // warp 0: the named experts, where their entries begin and how many chunks each has
-  if (warp == 0) {
-    int named = 0, at = 0, chunks = 0, cap = 8, top = 0;
-    for (int e = lane; e < E; e += 32) {
-      int c = 0;
-      for (int w = 0; w < W; ++w) c += counts[w * E + e];
-      top = max(top, c);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    while (cap < top && cap < most) cap *= 2;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane;
-      int c = 0;
-      if (e < E)
-        for (int w = 0; w < W; ++w) c += counts[w * E + e];
-      const uint32_t has = __ballot_sync(0xffffffffu, c > 0);
-      if (!has) continue;
-      const int ch = (c + cap - 1) / cap;
-      int c_sum = c, ch_sum = ch;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, c_sum, o), v = __shfl_up_sync(0xffffffffu, ch_sum, o);
-        if (lane >= o) c_sum += u, ch_sum += v;
-      }
-      if (c > 0) {
-        const int a = named + __popc(has & below);
-        r.expert[a] = (uint16_t)e, r.start[a] = at + c_sum - c, r.first[a] = (uint16_t)(chunks + ch_sum - ch);
-        // from counts to places: where each warp's entries of this expert go
-        int p = at + c_sum - c;
-        for (int w = 0; w < W; ++w) {
-          const int m = counts[w * E + e];
-          counts[w * E + e] = p;
-          p += m;
-        }
-      }
-      named += __popc(has);
-      at += __shfl_sync(0xffffffffu, c_sum, 31), chunks += __shfl_sync(0xffffffffu, ch_sum, 31);
-    }
-    if (lane == 0) r.start[named] = at, r.first[named] = (uint16_t)chunks, out[0] = named, out[1] = cap;
+  int top = 0;
+  for (int e = threadIdx.x; e < E; e += kXpThreads) {
+    int c = 0;
+    for (int w = 0; w < used; ++w) c += counts[w * E + e];
+    top = max(top, c);
   }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0 && top) atomicMax(out, top);
   __syncthreads();
+  int cap = 8;
+  while (cap < out[0] && cap < most) cap *= 2;
+  int named = 0, all = 0;  // of the experts so far; `all`: entries, and chunks from bit 16
+  for (int e0 = 0; e0 < E; e0 += kXpThreads) {
+    const int e = e0 + threadIdx.x;
+    int c = 0;
+    if (e < E)
+      for (int w = 0; w < used; ++w) c += counts[w * E + e];
+    const uint32_t has = __ballot_sync(0xffffffffu, c > 0);
+    const int v = c | ((c + cap - 1) / cap) << 16;
+    int sum = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    if (lane == 31) sums[warp] = sum, heads[warp] = __popc(has);
+    __syncthreads();
+    int before = all, a = named + __popc(has & below);
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) before += sums[w], a += heads[w];
+      all += sums[w], named += heads[w];
+    }
+    if (c > 0) {
+      before += sum - v;
+      int p = before & 0xffff;
+      r.expert[a] = (uint16_t)e, r.start[a] = p, r.first[a] = (uint16_t)(before >> 16);
+      for (int w = 0; w < used; ++w) {  // from counts to places
+        const int m = counts[w * E + e];
+        counts[w * E + e] = p;
+        p += m;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) r.start[named] = all & 0xffff, r.first[named] = (uint16_t)(all >> 16);
   for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
-    const int e = i < hi ? d.topk_idx[i] : -1;
+    const int e = i0 == lo ? e_first : i < hi ? d.topk_idx[i] : -1;
     const bool here = (uint32_t)e < (uint32_t)E;
     const uint32_t same = __match_any_sync(0xffffffffu, here ? e : -1);
     const int before = __popc(same & below);
@@ -310,8 +241,8 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
     __syncwarp();
   }
   __syncthreads();
-  r.named = out[0];
-  return out[1];
+  r.named = named;
+  return cap;
 }
 
 // What the warps that multiply share.
@@ -339,6 +270,9 @@ template <bool FP8, bool DOWN, int NB>
 __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t end, int up_border, float* sum, int warp, int lane,
                                            volatile int* abort, uint64_t timeout_ns) {
   const int rows = (warp & 3) * 32, group = warp >> 2, g = lane >> 2, c = lane & 3;
+  // Which of eight tokens a column of the product is. With e4m3 weights a half of a warp reads 32 bytes of four tokens at a time: of
+  // every second one, whose places differ under the swizzle.
+  auto column = [](int j) { return FP8 ? (j & 3) * 2 + (j >> 2) : j; };
   float acc[2][NB][4] = {};
   while (mine < end) {
     // A wait that ran out raises `abort`; the warps then finish on whatever lies there, so that they meet at every barrier, and the
@@ -399,9 +333,9 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
           }
 #pragma unroll
           for (int j = 0; j < NB; ++j) {
-            const int row = j * 8 + g;
             uint32_t x0, x1;
-            lds_64(x0, x1, x + row * 256 + ((((step + ks) * 2 + (c >> 1)) ^ ((row & 3) << 1)) << 4) + (c & 1) * 8);
+            const int st = step + ks;
+            lds_64(x0, x1, x + (st >> 2) * (ring.x_bytes / 2) + (j * 8 + column(g)) * 128 + ((((st & 3) * 2 + (c >> 1)) ^ column(g)) << 4) + (c & 1) * 8);
             const uint32_t b0 = __byte_perm(x0, x1, 0x5410), b1 = __byte_perm(x0, x1, 0x7632);
 #pragma unroll
             for (int m = 0; m < 2; ++m) mma_bf16(part[m][j], wa[m][0], wa[m][1], wa[m][2], wa[m][3], b0, b1);
@@ -438,7 +372,7 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float* at = sum + (j * 8 + 2 * c + (q & 1)) * kXpLd + rows + m * 16 + g + (q >> 1) * 8;
+            float* at = sum + (j * 8 + column(2 * c + (q & 1))) * kXpLd + rows + m * 16 + g + (q >> 1) * 8;
             *at = h == 0 ? acc[m][j][q] : *at + acc[m][j][q];
           }
     }
@@ -453,9 +387,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 template <bool FP8, bool DOWN>
-__global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ XpParams p) {
+__global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ XpParams p) {
   extern __shared__ __align__(1024) unsigned char xp_smem[];
-  __shared__ int s_abort, s_route[2], s_last;
+  __shared__ int s_abort, s_last, s_route[4 + 2 * kXpThreads / 32];
   const eux_experts_desc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entries = d.n_tokens * d.topk;
@@ -466,11 +400,12 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int i = 0; i < kXpMaxStages; ++i) {
-      mbar_init(ring.full + 16 * i, 1 + 32);
+      mbar_init(ring.full + 16 * i, 2);   // weights and tokens
       mbar_init(ring.empty + 16 * i, 4);  // the warps of a group
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
   }
   // The up form waits here for whatever wrote the tokens and their experts. The down form was let in by the up form, behind its
   // wait: what both read is there, and only what the up form writes is waited for (below).
@@ -529,36 +464,54 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   } else if (warp == kXpWarps + 1) {
     // ---- the tokens' values (down: their h) and the scales ----
     if (DOWN) wait_for_launch_before();
+    asm volatile("fence.proxy.async;" ::: "memory");  // written by ordinary stores, read by copies
     const int sr = ((DOWN ? d.hidden : 2 * d.inner) + 127) / 128, sk = (K + 127) / 128;
-    for (int64_t b = b0; b < b1;) {
+    bool gone = false;
+    for (int64_t b = b0; b < b1 && !gone;) {
       const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
       const XpSegment s = walk.at(seg);
-      const int rows = (s.n + 7) & ~7, pieces = FP8 ? 16 : 8;
-      bool gone = false;
-      for (int k = kb; k < end && !gone; ++k) {
+      const int rows = (s.n + 7) & ~7;
+      int y[4];  // of this lane's copy
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int pos = s.pos + min(lane * 4 + q, s.n - 1);  // what fills up to eight is multiplied and not used
+        y[q] = DOWN ? r.order[pos] : r.token[pos];
+      }
+      // the scales of 32 blocks at a time, one per lane. Down: of the rows. Up: of the gate rows, of the first up rows, of the up rows
+      // that lie in the next block.
+      const float* const scale = FP8 ? (DOWN ? d.down_scale : d.gate_up_scale) + (int64_t)s.expert * sr * sk : nullptr;
+      float sc[DOWN ? 1 : 3];
+      for (int k = kb; k < end; ++k) {
+        if (FP8 && (k - kb) % 32 == 0) {
+#pragma unroll
+          for (int q = 0; q < (DOWN ? 1 : 3); ++q) {
+            const int row = DOWN ? s.tile : q == 0 ? s.tile * 64 / 128 : min((d.inner + s.tile * 64) / 128 + q - 1, sr - 1);
+            sc[q] = k + lane < end ? __ldg(scale + (int64_t)row * sk + k + lane) : 0.f;
+          }
+        }
         gone = __any_sync(0xffffffffu, !mbar_wait(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
         if (gone) break;
-        const uint32_t dst = ring.x + ring.s * ring.x_bytes;
-        for (int i = lane; i < rows * pieces; i += 32) {
-          const int row = i / pieces, piece = i % pieces, at = k * per_block + piece * 8;
-          const bool some = row < s.n && at < K;
-          const int pos = s.pos + (row < s.n ? row : 0);
-          const __nv_bfloat16* src = DOWN ? p.h + (int64_t)r.order[pos] * d.inner : (const __nv_bfloat16*)d.x + (int64_t)r.token[pos] * d.x_stride;
-          const int swizzled = FP8 ? piece ^ ((row & 3) << 1) : piece ^ (row & 7);
-          cp_async_16(dst + row * (pieces * 16) + swizzled * 16, src + (some ? at : 0), some ? 16 : 0);
+        const uint32_t bar = ring.full + 16 * ring.s, dst = ring.x + ring.s * ring.x_bytes;
+        if (FP8) {
+          float v[3];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) v[q] = __shfl_sync(0xffffffffu, sc[DOWN ? 0 : q], (k - kb) % 32);
+          if (lane == 0) asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %3};" ::"r"(ring.scales + 16 * ring.s), "f"(v[0]), "f"(v[1]), "f"(v[2]) : "memory");
         }
-        if (FP8 && lane < (DOWN ? 1 : 3)) {
-          // down: the scale of the rows; up: the gate rows', the first up rows', those of the up rows in the next block
-          const int row = DOWN ? s.tile : lane == 0 ? s.tile * 64 / 128 : min((d.inner + s.tile * 64) / 128 + lane - 1, sr - 1);
-          cp_async_4(ring.scales + 16 * ring.s + 4 * lane, (DOWN ? d.down_scale : d.gate_up_scale) + ((int64_t)s.expert * sr + row) * sk + k);
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)rows * (FP8 ? 256 : 128));
+        __syncwarp();
+        if (lane < rows / 4) {
+          tma_gather_4(dst + lane * 512, &x_map, bar, k * per_block, y);
+          if (FP8) tma_gather_4(dst + ring.x_bytes / 2 + lane * 512, &x_map, bar, k * per_block + 64, y);
         }
-        cp_async_arrive(ring.full + 16 * ring.s);
         ring.next();
       }
-      if (gone) break;
       b += end - kb;
     }
-    cp_async_wait_all();
+    if (gone && lane == 0) {  // as above
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
   } else {
     // ---- products ----
     if (DOWN) wait_for_launch_before();
@@ -672,6 +625,16 @@ static XpEncodeFn xp_encode() {
   }();
   return fn;
 }
+// [rows][cols] bfloat16, rows `stride` elements apart, of which copies gather 128 bytes of single rows
+static int xp_map_rows(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint64_t stride) {
+  const XpEncodeFn fn = xp_encode();
+  if (!fn) return EUX_ERR_UNSUPPORTED;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
+  const cuuint32_t box[2] = {64, 1}, step[2] = {1, 1};
+  const CUresult rc = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? 0 : EUX_ERR_BAD_ARG;
+}
 // [slices][rows][cols], boxes of box_rows x 128 bytes, 128-byte swizzle; what lies outside is read as zero
 static int xp_map(CUtensorMap* m, const void* base, bool fp8, uint64_t slices, uint64_t rows, uint64_t cols, uint32_t box_rows) {
   const XpEncodeFn fn = xp_encode();
@@ -689,7 +652,7 @@ static int experts_check(const eux_experts_desc* d) {
   if (d->n_experts < 1 || d->n_experts > EUX_EXPERTS_MAX_EXPERTS || d->hidden < 1 || d->inner < 1) return EUX_ERR_BAD_ARG;
   if (d->hidden > (1 << 20) || d->inner > (1 << 20)) return EUX_ERR_BAD_ARG;
   const int unit = d->fp8 ? 16 : 8;  // rows of weights begin on 16 bytes
-  if (d->hidden % unit || d->inner % unit || d->x_stride % 8 || d->out_stride % 8) return EUX_ERR_BAD_ARG;
+  if (d->hidden % unit || d->inner % unit || d->x_stride % 8 || d->out_stride % 8 || d->x_stride < 0 || d->out_stride < 0) return EUX_ERR_BAD_ARG;
   return 0;
 }
 static int xp_part_rows(const eux_experts_desc* d) { return std::max(64, d->n_tokens); }
@@ -703,13 +666,13 @@ static int xp_sms(int* dev) {
 }
 
 template <bool FP8, bool DOWN>
-static int xp_launch(const CUtensorMap& map, XpParams p, int dev, int sms, cudaStream_t st) {
+static int xp_launch(const CUtensorMap& map, const CUtensorMap& x_map, const XpParams& p, int dev, int sms, cudaStream_t st) {
   const eux_experts_desc& d = p.d;
   // the ring holds a block of every group; the routing's counts lie where the ring will be
   const int room = xp_layout(DOWN, d.n_tokens, d.n_experts, d.n_tokens * d.topk).room, most = FP8 ? 32 : 64;
   if (xp_stages(room, most, most * (FP8 ? 256 : 128)) < kXpGroups || kXpThreads / 32 * d.n_experts * 4 > room) return EUX_ERR_TOO_LARGE;
   if (cudaError_t e = allow_smem<moe_experts_kernel<FP8, DOWN>>(dev, kXpDynamic); e != cudaSuccess) return (int)e;
-  return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, kXpDynamic, st, map, p);
+  return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, kXpDynamic, st, map, x_map, p);
 }
 
 }  // namespace eux
@@ -744,8 +707,11 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   p.part_rows = xp_part_rows(d);
   int dev = 0;
   const int sms = xp_sms(&dev);
-  if (int rc = d->fp8 ? xp_launch<true, false>(*up, p, dev, sms, st) : xp_launch<false, false>(*up, p, dev, sms, st)) return rc;
-  return d->fp8 ? xp_launch<true, true>(*down, p, dev, sms, st) : xp_launch<false, true>(*down, p, dev, sms, st);
+  CUtensorMap x, h;
+  if (int rc = xp_map_rows(&x, d->x, d->n_tokens, d->hidden, std::max<int64_t>(d->x_stride, d->hidden))) return rc;
+  if (int rc = xp_map_rows(&h, p.h, (uint64_t)d->n_tokens * d->topk, d->inner, d->inner)) return rc;
+  if (int rc = d->fp8 ? xp_launch<true, false>(*up, x, p, dev, sms, st) : xp_launch<false, false>(*up, x, p, dev, sms, st)) return rc;
+  return d->fp8 ? xp_launch<true, true>(*down, h, p, dev, sms, st) : xp_launch<false, true>(*down, h, p, dev, sms, st);
 }
 
 extern "C" int eux_experts_preload(void) {
