@@ -14,7 +14,8 @@
 //   form a tile is 128 rows of the output with all experts, so the weighted sum over a token's experts is made in shared
 //   memory, and only what an SM's share cuts goes through the workspace.
 // * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp the tokens' values beside them
-//   the same way (rows are gathered, four by a copy: any tokens, any order), twelve warps multiply. The ring runs on
+//   the same way (rows are gathered, four by a copy: any tokens, any order), twelve warps multiply, and two make
+//   results of the sums while those go on. The ring runs on
 //   over the borders of segments; the down form's starts before the up form has ended (programmatic dependent launch), since
 //   weights wait for nobody.
 // * The weights are the first operand of mma.sync m16n8k16 and the tokens the second: 8 columns are the smallest padding for
@@ -34,12 +35,13 @@
 namespace eux {
 
 constexpr int kXpGroups = 3;                        // of warps that multiply: each takes the blocks of every third stage ...
-constexpr int kXpWarps = kXpGroups * 4;             // ... and each of its four warps 32 rows of it
-constexpr int kXpConsumers = kXpWarps * 32;
-constexpr int kXpThreads = kXpConsumers + 64;       // and one that fetches weights, one that fetches tokens
+constexpr int kXpWarps = kXpGroups * 4;             // ... and each of its four warps 32 rows of them
+constexpr int kXpEndThreads = 64;                   // two warps that see to the results
+constexpr int kXpThreads = kXpWarps * 32 + kXpEndThreads + 64;  // and a warp that fetches weights, one that fetches tokens
 constexpr int kXpRows = 128;                        // rows of weights in a block
 constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
 constexpr int kXpMaxStages = 13;
+constexpr int kXpSumBars = 64;                      // bytes: for each of two sums, each group's and the results' barrier
 constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
 constexpr int kXpMaxGrid = 160;
 constexpr size_t kXpDynamic = 226 * 1024;           // shared memory of a launch; the kernel declares a little more itself
@@ -50,10 +52,11 @@ struct XpParams {
   __nv_bfloat16* h;      // [entries, inner]
   float* part;           // [grid][2][part_rows][128]
   int part_rows;
+  int token_of;          // ceil(2^20 / topk): entry * token_of >> 20 is entry / topk, for less than 2^20 / topk entries
 };
 
 // Shared memory: the ring of weights (128-byte swizzle: on 1024 bytes), behind it the tokens' values of each stage, the sums
-// of a segment; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
+// of a segment, twice where they are small; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
 // many stages there is room for, is known when the entries have been counted.
 struct XpLayout {
   int acc, scales, bars, tables;  // from the beginning
@@ -62,15 +65,16 @@ struct XpLayout {
 __host__ __device__ inline XpLayout xp_layout(bool down, int n_tokens, int n_experts, int entries) {
   XpLayout l;
   int at = (int)kXpDynamic;
-  at -= ((n_experts + 1) * 8 + entries * 4 + 15) & ~15, l.tables = at;
-  at -= kXpMaxStages * 16, l.bars = at;
+  at -= ((n_experts + 1) * 8 + entries * (down ? 8 : 4) + 31) & ~15, l.tables = at;
+  at -= kXpMaxStages * 16 + kXpSumBars, l.bars = at;
   at -= kXpMaxStages * 16, l.scales = at;
   at -= down ? n_tokens * kXpLd * 4 : 0, l.acc = at;
   l.room = at;
   return l;
 }
+__host__ __device__ inline int xp_sums(int cap) { return cap <= 32 ? 2 : 1; }
 __host__ __device__ inline int xp_stages(int room, int cap, int x_bytes) {
-  const int n = (room - cap * kXpLd * 4) / (kXpBlock + x_bytes);
+  const int n = (room - xp_sums(cap) * cap * kXpLd * 4) / (kXpBlock + x_bytes);
   return n < kXpMaxStages ? n : kXpMaxStages;
 }
 
@@ -86,6 +90,30 @@ __device__ __forceinline__ void tma_gather_4(uint32_t dst, const CUtensorMap* ma
       "l"(map), "r"(bar), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
       : "memory");
 }
+// mbar_wait by a warp that has nothing else to do: it asks to be left asleep until the phase ends, for up to 20 us, instead of
+// asking again and again, which takes issue slots from the warps that multiply.
+__device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t timeout_ns) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 0; it < 0x7fffffffu; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if ((it & 15u) == 15u) {
+      if (*abort) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > (timeout_ns ? timeout_ns : 2000000000ull)) break;
+    }
+  }
+  *abort = 1;
+  return false;
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -97,7 +125,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpConsumers) : "memory"); }
+__device__ __forceinline__ void end_warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpEndThreads) : "memory"); }
 
 // Four e4m3 values as bfloat16, bytes 0 and 2 in `even` and 1 and 3 in `odd`: sign, exponent and mantissa are moved to their places,
 // which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and multiplied by
@@ -122,6 +150,7 @@ struct XpTables {
   uint16_t* expert;  // [named]
   uint16_t* order;   // [entries]
   uint16_t* token;   // [entries]: of order
+  float* weight;     // [entries]: of order (down; else null)
   int named;
 };
 
@@ -166,11 +195,47 @@ struct XpWalk {
 // The tables. Returns the tokens that a segment takes at most: 8, 16, 32 or 64, as the expert with the most needs and `most`
 // allows. `counts` is scratch, [warps][n_experts]; `out` has room for 4 and two words per warp. Entries are counted per warp and
 // expert, and their places follow: by expert and then by entry, the same in every CTA.
-__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpTables& r, int* counts, int* out) {
+__device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of, int most, XpTables& r, int* counts, int* out) {
   const int E = d.n_experts, n = d.n_tokens * d.topk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int W = kXpThreads / 32;
   const uint32_t below = (1u << lane) - 1u;
   int *const sums = out + 4, *const heads = sums + W;
+  if (n <= 32) {  // one warp, by comparing
+    if (warp == 0) {
+      const int e0 = lane < n ? d.topk_idx[lane] : -1, e = (uint32_t)e0 < (uint32_t)E ? e0 : E;  // not here: behind all others
+      int at = 0;
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        const int o = __shfl_sync(0xffffffffu, e, j);
+        at += o < e || (o == e && j < lane);
+      }
+      const uint32_t same = __match_any_sync(0xffffffffu, lane < n ? e : -1);
+      const bool head = lane < n && e < E && (same & below) == 0;
+      const int count = head ? __popc(same) : 0;
+      if (lane < n && e < E) {
+        r.order[at] = (uint16_t)lane, r.token[at] = (uint16_t)((uint32_t)lane * token_of >> 20);
+        if (r.weight) r.weight[at] = d.topk_w[lane];
+      }
+      // heads in the order of their places
+      int named = 0, chunks = 0, top = __reduce_max_sync(0xffffffffu, count), cap = 8;
+      while (cap < top && cap < most) cap *= 2;
+      const int ch = (count + cap - 1) >> (31 - __clz(cap));
+      uint32_t all = __ballot_sync(0xffffffffu, head);
+      int before = 0, first = 0;
+#pragma unroll 1
+      for (uint32_t m = all; m; m &= m - 1) {
+        const int j = __ffs(m) - 1, oe = __shfl_sync(0xffffffffu, e, j), oc = __shfl_sync(0xffffffffu, ch, j);
+        before += oe < e, first += oe < e ? oc : 0;
+        ++named, chunks += oc;
+      }
+      if (head) r.expert[before] = (uint16_t)e, r.start[before] = at, r.first[before] = (uint16_t)first;
+      const int here = __popc(__ballot_sync(0xffffffffu, lane < n && e < E));
+      if (lane == 0) r.start[named] = here, r.first[named] = (uint16_t)chunks, out[0] = named, out[1] = cap;
+    }
+    __syncthreads();
+    r.named = out[0];
+    return out[1];
+  }
   const int used = min(W, (n + 31) / 32);  // warps that have entries
   const int each = ((n + used - 1) / used + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
   const int e_first = lo + lane < hi ? d.topk_idx[lo + lane] : -1;
@@ -200,7 +265,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
     if (e < E)
       for (int w = 0; w < used; ++w) c += counts[w * E + e];
     const uint32_t has = __ballot_sync(0xffffffffu, c > 0);
-    const int v = c | ((c + cap - 1) / cap) << 16;
+    const int v = c | ((c + cap - 1) >> (31 - __clz(cap))) << 16;
     int sum = v;
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, sum, o);
@@ -234,7 +299,8 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
     const int before = __popc(same & below);
     if (here) {
       const int at = counts[warp * E + e] + before;
-      r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)(i / d.topk);
+      r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)((uint32_t)i * token_of >> 20);
+      if (r.weight) r.weight[at] = d.topk_w[i];
     }
     __syncwarp();
     if (here && before == 0) counts[warp * E + e] += __popc(same);
@@ -244,6 +310,15 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int most, XpT
   r.named = named;
   return cap;
 }
+
+// Equal shares of the line of blocks, the first `more` of them one longer. (A line has fewer than 2^31 blocks: 180 GB of weights are
+// 12 million, and no expert has more than 128 chunks.)
+struct XpShares {
+  int each, more;
+  __device__ XpShares(int blocks, int grid) : each(blocks / grid), more(blocks % grid) {}
+  __device__ int begin(int i) const { return i * each + min(i, more); }
+  __device__ int owner(int block) const { return block < more * (each + 1) ? block / (each + 1) : more + (block - more * (each + 1)) / each; }
+};
 
 // What the warps that multiply share.
 struct XpRing {
@@ -256,18 +331,19 @@ struct XpRing {
   }
   // Of a group, which has the stages group, group + kXpGroups, ... A stage must not change hands: its barrier tells two phases
   // apart, and a group that came to it from elsewhere, ahead of a load that is late, would take the phase before the last for it.
-  __device__ __forceinline__ void next_of_group(int group, int64_t& block) {
+  __device__ __forceinline__ void next_of_group(int group, int& block) {
     block += kXpGroups;
     if ((s += kXpGroups) >= stages) block += group + stages - s, s = group, ph ^= 1u;
   }
 };
 
 // The blocks of a segment up to number `end` of this SM's line times the segment's tokens: those in this group's stages, `mine`
-// the next of them, and this warp's 32 rows. All groups' sums are left in `sum` [token][row], which all of them may read when this
-// returns. Groups by blocks and not by parts of one: a block takes a warp some hundred clocks from its arrival to its release,
-// one thing after the other, and so three are under way at once.
+// the next of them, and this warp's 32 rows. The groups' sums are added up in `sum` [token][row], one group after the other: each
+// waits for the barrier in front of its own in `bars` (the first for the last, that the results made of an earlier segment's
+// sums are done), and the warps that see to the results for the last group's. Groups by blocks and not by parts of one: a block
+// takes a warp some hundred clocks from its arrival to its release, one thing after the other, and so three are under way at once.
 template <bool FP8, bool DOWN, int NB>
-__device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t end, int up_border, float* sum, int warp, int lane,
+__device__ __forceinline__ void xp_segment(XpRing& ring, int& mine, int end, int up_border, float* sum, uint32_t bars, uint32_t bars_ph, int warp, int lane,
                                            volatile int* abort, uint64_t timeout_ns) {
   const int rows = (warp & 3) * 32, group = warp >> 2, g = lane >> 2, c = lane & 3;
   // Which of eight tokens a column of the product is. With e4m3 weights a half of a warp reads 32 bytes of four tokens at a time: of
@@ -277,7 +353,7 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
   while (mine < end) {
     // A wait that ran out raises `abort`; the warps then finish on whatever lies there, so that they meet at every barrier, and the
     // status word says that the result is none.
-    mbar_wait(ring.full + 16 * ring.s, ring.ph, abort, timeout_ns);
+    mbar_sleep(ring.full + 16 * ring.s, ring.ph, abort, timeout_ns);
     __syncwarp();
     const uint32_t w = ring.w + ring.s * kXpBlock, x = ring.x + ring.s * ring.x_bytes;
     if constexpr (!FP8) {
@@ -364,26 +440,101 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int64_t& mine, int64_t 
     if (lane == 0) mbar_arrive(ring.empty + 16 * ring.s);
     ring.next_of_group(group, mine);
   }
-  for (int h = 0; h < kXpGroups; ++h) {
-    if (group == h) {
+  mbar_sleep(bars + (group ? 8 * (group - 1) : 8 * kXpGroups), group ? bars_ph : bars_ph ^ 1u, abort, timeout_ns);
+  __syncwarp();
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+  for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float* at = sum + (j * 8 + column(2 * c + (q & 1))) * kXpLd + rows + m * 16 + g + (q >> 1) * 8;
-            *at = h == 0 ? acc[m][j][q] : *at + acc[m][j][q];
-          }
-    }
-    consumers_meet();
-  }
+      for (int q = 0; q < 4; ++q) {
+        float* at = sum + (j * 8 + column(2 * c + (q & 1))) * kXpLd + rows + m * 16 + g + (q >> 1) * 8;
+        *at = group ? *at + acc[m][j][q] : acc[m][j][q];
+      }
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bars + 8 * group);
 }
 
 __device__ __forceinline__ float4 ldcg_f4(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void cta_meets() { __syncthreads(); }
+
+// The end of a tile of results, or of this SM's part of it: the sums `from` [token][row], which THREADS threads have, that meet with
+// `meet`. The parts of a tile that begin in the middle of it come early in their SMs' shares, and the first part comes last in its
+// own: where the others are there already, which it sees from their count, it need not leave its part in the workspace and count itself.
+template <bool DOWN, int THREADS, typename Meet>
+__device__ __forceinline__ void xp_tile_end(const XpParams& p, const XpTables& r, const XpSegment& s, int first, int last, int me, const float* from,
+                                            int tid, int* s_last, Meet meet) {
+  const eux_experts_desc& d = p.d;
+  const int rows = DOWN ? d.n_tokens : s.n;
+  uint32_t* const counter = d.counters + (DOWN ? kXpMaxGrid : 0) + first;
+  constexpr int Q = DOWN ? kXpRows / 4 : 16;  // four rows of results per thread and step
+  bool own_here = first == last;
+  if (first != last && me == first) {
+    if (tid == 0) {
+      *s_last = ld_acquire_gpu(counter) == (unsigned)(last - first);
+      if (*s_last) *counter = 0;
+    }
+    meet();
+    own_here = *s_last != 0;
+    meet();
+  }
+  if (!own_here) {
+    float* const part = p.part + ((int64_t)me * 2 + (me == first)) * p.part_rows * kXpRows;
+    for (int i = tid; i < rows * (kXpRows / 4); i += THREADS)
+      __stcg(reinterpret_cast<float4*>(part) + i, *reinterpret_cast<const float4*>(from + (i / (kXpRows / 4)) * kXpLd + (i % (kXpRows / 4)) * 4));
+    __threadfence();
+    meet();
+    // counts up to the number of parts and starts again: ready for the next launch
+    if (tid == 0) *s_last = atomicInc(counter, (unsigned)(last - first)) == (unsigned)(last - first);
+    meet();
+    const bool all_there = *s_last != 0;
+    meet();
+    if (!all_there) return;
+    __threadfence();
+  }
+  for (int i = tid; i < rows * Q; i += THREADS) {
+    const int j = i / Q, q = (i % Q) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+    auto add = [](float4& to, const float4& a) { to.x += a.x, to.y += a.y, to.z += a.z, to.w += a.w; };
+    int k = first;
+    if (own_here) {
+      add(v, *reinterpret_cast<const float4*>(from + j * kXpLd + q));
+      if (!DOWN) add(u, *reinterpret_cast<const float4*>(from + j * kXpLd + 64 + q));
+      ++k;
+    }
+    constexpr int AT_ONCE = DOWN ? 6 : 3;
+    for (; k <= last; k += AT_ONCE) {  // in the order of the SMs, several loads under way
+      float4 a[AT_ONCE], o[AT_ONCE];
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n) {
+        const int c = min(k + n, last);
+        const float* const part = p.part + (((int64_t)c * 2 + (c == first)) * p.part_rows + j) * kXpRows + q;
+        a[n] = ldcg_f4(part);
+        if (!DOWN) o[n] = ldcg_f4(part + 64);
+      }
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n)
+        if (k + n <= last) {
+          add(v, a[n]);
+          if (!DOWN) add(u, o[n]);
+        }
+    }
+    if (DOWN) {
+      const int at = s.tile * kXpRows + q;
+      if (at < d.hidden) *reinterpret_cast<uint2*>((__nv_bfloat16*)d.out + j * d.out_stride + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    } else {
+      const int at = s.tile * 64 + q;
+      auto gated = [](float g, float w) { return g / (1.f + expf(-g)) * w; };
+      if (at < d.inner)
+        *reinterpret_cast<uint2*>(p.h + (int64_t)r.order[s.pos + j] * d.inner + at) =
+            make_uint2(pack_bf16(gated(v.x, u.x), gated(v.y, u.y)), pack_bf16(gated(v.z, u.z), gated(v.w, u.w)));
+    }
+  }
 }
 
 template <bool FP8, bool DOWN>
@@ -397,12 +548,14 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   const uint32_t smem = smem_u32(xp_smem);
   XpRing ring;
   ring.w = smem, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;
+  const uint32_t sum_bars = smem + l.bars + kXpMaxStages * 16;
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int i = 0; i < kXpMaxStages; ++i) {
       mbar_init(ring.full + 16 * i, 2);   // weights and tokens
       mbar_init(ring.empty + 16 * i, 4);  // the warps of a group
     }
+    for (int i = 0; i < 2 * (kXpGroups + 1); ++i) mbar_init(sum_bars + 8 * i, i % (kXpGroups + 1) < kXpGroups ? 4 : kXpEndThreads / 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
@@ -416,33 +569,41 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   r.expert = r.first + d.n_experts + 1;
   r.order = r.expert + d.n_experts + 1;
   r.token = r.order + entries;
-  const int cap = xp_route(d, FP8 ? 32 : 64, r, reinterpret_cast<int*>(xp_smem), s_route);
+  r.weight = DOWN ? reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(r.token + entries) + 3) & ~(uintptr_t)3) : nullptr;
+  const int cap = xp_route(d, p.token_of, FP8 ? 32 : 64, r, reinterpret_cast<int*>(xp_smem), s_route);
   ring.x_bytes = cap * (FP8 ? 256 : 128);
   ring.stages = xp_stages(l.room, cap, ring.x_bytes);
   ring.x = smem + ring.stages * kXpBlock;
-  // the counts lay where weights are about to land
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
-
   const int K = DOWN ? d.inner : d.hidden, per_block = FP8 ? 128 : 64;
   const int nk = (K + per_block - 1) / per_block;
   const int tiles = DOWN ? (d.hidden + kXpRows - 1) / kXpRows : (d.inner + 63) / 64;
   const int chunks = r.first[r.named];
-  const int64_t blocks = (int64_t)tiles * chunks * nk;
-  const int grid = (int)min((int64_t)gridDim.x, max((int64_t)1, blocks / kXpMinBlocks));
+  const int blocks = tiles * chunks * nk;
+  const int grid = min((int)gridDim.x, max(1, blocks / kXpMinBlocks));
   const int me = blockIdx.x;
-  const int64_t b0 = me < grid ? blocks * me / grid : blocks, b1 = me < grid ? blocks * (me + 1) / grid : blocks;
+  const XpShares shares(blocks, grid);
+  const int b0 = me < grid ? shares.begin(me) : blocks, b1 = me < grid ? shares.begin(me + 1) : blocks;
+  const int seg0 = b0 / nk, kb0 = b0 - seg0 * nk;  // the segment that the share begins in, and where
+  float* const sums = reinterpret_cast<float*>(xp_smem + ring.stages * (kXpBlock + ring.x_bytes));
+  const int n_sums = xp_sums(cap);
+  float* const acc = reinterpret_cast<float*>(xp_smem + l.acc);
+  if (DOWN)
+    for (int i = threadIdx.x; i < d.n_tokens * (kXpLd / 4); i += kXpThreads) reinterpret_cast<float4*>(acc)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // the counts lay where weights are about to land
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
   volatile int* abort = &s_abort;
   XpWalk<DOWN> walk(r, tiles);
 
-  if (warp == kXpWarps) {
+  constexpr int kWeights = kXpThreads / 32 - 2, kTokens = kWeights + 1;
+  if (warp == kWeights) {
     // ---- weights ----
     if (lane == 0) {
-      for (int64_t b = b0; b < b1 && !*abort;) {
-        const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+      for (int b = b0, seg = seg0, kb = kb0; b < b1 && !*abort; ++seg, kb = 0) {
+        const int end = min(nk, kb + (b1 - b));
         const XpSegment s = walk.at(seg);
         for (int k = kb; k < end; ++k) {
-          if (!mbar_wait(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns)) break;
+          if (!mbar_sleep(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns)) break;
           const uint32_t bar = ring.full + 16 * ring.s, dst = ring.w + ring.s * kXpBlock;
           mbar_expect_tx(bar, kXpBlock);
           if (DOWN) {
@@ -461,14 +622,14 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       }
       allow_next_launch();
     }
-  } else if (warp == kXpWarps + 1) {
+  } else if (warp == kTokens) {
     // ---- the tokens' values (down: their h) and the scales ----
     if (DOWN) wait_for_launch_before();
     asm volatile("fence.proxy.async;" ::: "memory");  // written by ordinary stores, read by copies
     const int sr = ((DOWN ? d.hidden : 2 * d.inner) + 127) / 128, sk = (K + 127) / 128;
     bool gone = false;
-    for (int64_t b = b0; b < b1 && !gone;) {
-      const int seg = (int)(b / nk), kb = (int)(b - (int64_t)seg * nk), end = (int)min((int64_t)nk, kb + (b1 - b));
+    for (int b = b0, seg = seg0, kb = kb0; b < b1 && !gone; ++seg, kb = 0) {
+      const int end = min(nk, kb + (b1 - b));
       const XpSegment s = walk.at(seg);
       const int rows = (s.n + 7) & ~7;
       int y[4];  // of this lane's copy
@@ -489,7 +650,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
             sc[q] = k + lane < end ? __ldg(scale + (int64_t)row * sk + k + lane) : 0.f;
           }
         }
-        gone = __any_sync(0xffffffffu, !mbar_wait(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
+        gone = __any_sync(0xffffffffu, !mbar_sleep(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
         if (gone) break;
         const uint32_t bar = ring.full + 16 * ring.s, dst = ring.x + ring.s * ring.x_bytes;
         if (FP8) {
@@ -512,102 +673,88 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       const uint64_t t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-  } else {
+  } else if (warp < kXpWarps) {
     // ---- products ----
-    if (DOWN) wait_for_launch_before();
-    float* const sum = reinterpret_cast<float*>(xp_smem + ring.stages * (kXpBlock + ring.x_bytes));
-    float* const acc = reinterpret_cast<float*>(xp_smem + l.acc);
-    const int tid = threadIdx.x;
-    const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
-    const int64_t tile_blocks = (int64_t)tile_segs * nk;
-    const int width = DOWN ? d.n_tokens : 0;  // rows of a part (up: the segment's tokens)
-    if (DOWN && blocks == 0) {  // no expert is named: the result is zero
-      for (int64_t i = (int64_t)blockIdx.x * kXpConsumers + tid; i < (int64_t)d.n_tokens * (d.hidden / 8); i += (int64_t)gridDim.x * kXpConsumers)
-        st_u4((__nv_bfloat16*)d.out + (i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
-    }
-    int64_t mine = b0 + (warp >> 2);
+    int mine = b0 + (warp >> 2), sum_at = 0;
+    uint32_t sum_ph = 0;
     ring.s = warp >> 2;
-    for (int64_t b = b0; b < b1;) {
-      const int seg = (int)(b / nk);
-      const int64_t end = min((int64_t)(seg + 1) * nk, b1);
+    for (int b = b0, seg = seg0; b < b1; ++seg) {
+      const int end = min((seg + 1) * nk, b1);
       const XpSegment s = walk.at(seg);
-      const int tile = seg / tile_segs;
-      const int64_t tile0 = tile * tile_blocks;
-      if (DOWN && (b == b0 || b == tile0)) {
-        for (int i = tid; i < d.n_tokens * kXpLd; i += kXpConsumers) acc[i] = 0.f;
-      }
       const int up_border = 128 - (d.inner + s.tile * 64) % 128;
       const int nb = (s.n + 7) >> 3;
-      if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
-      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, mine, end, up_border, sum, warp, lane, abort, d.wait_timeout_ns);
+      float* const sum = sums + sum_at * cap * kXpLd;
+      const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
+      if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      if (++sum_at == n_sums) sum_at = 0, sum_ph ^= 1u;
       b = end;
+    }
+  } else {
+    // ---- results ----
+    if (DOWN) wait_for_launch_before();
+    const int tid = threadIdx.x - kXpWarps * 32;
+    const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
+    const int tile_blocks = tile_segs * nk;
+    if (DOWN && blocks == 0) {  // no expert is named: the result is zero
+      for (int i = blockIdx.x * kXpEndThreads + tid; i < d.n_tokens * (d.hidden / 8); i += gridDim.x * kXpEndThreads)
+        st_u4((__nv_bfloat16*)d.out + (int64_t)(i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
+    }
+    int sum_at = 0, tile = b0 < b1 ? seg0 / tile_segs : 0;
+    uint32_t sum_ph = 0;
+    for (int b = b0, seg = seg0; b < b1; ++seg) {
+      const XpSegment s = walk.at(seg);
+      const int tile0 = tile * tile_blocks, tile1 = tile0 + tile_blocks;
+      float* const sum = sums + sum_at * cap * kXpLd;
+      const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
+      if (DOWN && b == tile0 && b != b0) {
+        for (int i = tid; i < d.n_tokens * (kXpLd / 4); i += kXpEndThreads) reinterpret_cast<float4*>(acc)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        end_warps_meet();
+      }
+      mbar_sleep(bars + 8 * (kXpGroups - 1), sum_ph, abort, d.wait_timeout_ns);
+      __syncwarp();
+      b = min((seg + 1) * nk, b1);
       if (DOWN) {
-        // A thread has a row and every third token: entries of the same token, also twice of the same expert, are added by one
-        // thread, in order.
-        const int row = tid & 127, third = tid >> 7;
-        for (int j = 0; j < s.n; ++j) {
-          const int entry = r.order[s.pos + j], t = r.token[s.pos + j];
-          if (t % kXpGroups == third) acc[t * kXpLd + row] = fmaf(__ldg(d.topk_w + entry), sum[j * kXpLd + row], acc[t * kXpLd + row]);
-        }
-        consumers_meet();
-      }
-      if (b != b1 && b != tile0 + tile_blocks) continue;
-      // ---- the end of a tile, or of this SM's part of it ----
-      const int first = (int)(((tile0 + 1) * grid - 1) / blocks), last = (int)(((tile0 + tile_blocks) * grid - 1) / blocks);
-      const int rows = DOWN ? width : s.n;
-      const float* const from = DOWN ? acc : sum;
-      bool all_there = true;
-      if (first != last) {
-        float* const part = p.part + ((int64_t)me * 2 + (me == first)) * p.part_rows * kXpRows;
-        for (int i = tid; i < rows * (kXpRows / 4); i += kXpConsumers)
-          __stcg(reinterpret_cast<float4*>(part) + i, *reinterpret_cast<const float4*>(from + (i / (kXpRows / 4)) * kXpLd + (i % (kXpRows / 4)) * 4));
-        __threadfence();
-        consumers_meet();
-        // counts up to the number of parts and starts again: ready for the next launch
-        if (tid == 0) s_last = atomicInc(d.counters + (DOWN ? kXpMaxGrid : 0) + first, (unsigned)(last - first)) == (unsigned)(last - first);
-        consumers_meet();
-        all_there = s_last != 0;
-        if (all_there) __threadfence();
-      }
-      if (all_there) {
-        constexpr int Q = DOWN ? kXpRows / 4 : 16;  // four rows of results per thread and step
-        for (int i = tid; i < rows * Q; i += kXpConsumers) {
-          const int j = i / Q, q = (i % Q) * 4;
-          float4 v, u;
-          if (first == last) {
-            v = *reinterpret_cast<const float4*>(from + j * kXpLd + q);
-            if (!DOWN) u = *reinterpret_cast<const float4*>(from + j * kXpLd + 64 + q);
-          } else {
-            v = u = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = first; k <= last; ++k) {
-              const float* part = p.part + (((int64_t)k * 2 + (k == first)) * p.part_rows + j) * kXpRows + q;
-              const float4 a = ldcg_f4(part);
-              v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-              if (!DOWN) {
-                const float4 o = ldcg_f4(part + 64);
-                u.x += o.x, u.y += o.y, u.z += o.z, u.w += o.w;
-              }
+        // A thread has two rows: entries of the same token, also twice of the same expert, are added by one thread, in order.
+        for (int j0 = 0; j0 < s.n; j0 += 4) {
+          float2 v[4];
+          float w[4];
+          int t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = min(j0 + i, s.n - 1);
+            v[i] = reinterpret_cast<const float2*>(sum + j * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j0 + i < s.n) {
+              float2* const at = reinterpret_cast<float2*>(acc + t[i] * kXpLd) + tid;
+              *at = make_float2(fmaf(w[i], v[i].x, at->x), fmaf(w[i], v[i].y, at->y));
             }
-          }
-          if (DOWN) {
-            const int at = s.tile * kXpRows + q;
-            if (at < d.hidden)
-              *reinterpret_cast<uint2*>((__nv_bfloat16*)d.out + j * d.out_stride + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-          } else {
-            const int at = s.tile * 64 + q;
-            auto gated = [](float g, float w) { return g / (1.f + expf(-g)) * w; };
-            if (at < d.inner)
-              *reinterpret_cast<uint2*>(p.h + (int64_t)r.order[s.pos + j] * d.inner + at) =
-                  make_uint2(pack_bf16(gated(v.x, u.x), gated(v.y, u.y)), pack_bf16(gated(v.z, u.z), gated(v.w, u.w)));
-          }
         }
       }
-      consumers_meet();  // what was read is written over next
+      if (!DOWN || b == b1 || b == tile1) {
+        // ---- the end of a tile, or of this SM's part of it ----
+        end_warps_meet();  // acc is complete
+        if (b == b1) break;  // the end of the share is everybody's
+        xp_tile_end<DOWN, kXpEndThreads>(p, r, s, shares.owner(tile0), shares.owner(tile1 - 1), me, DOWN ? acc : sum, tid, &s_last, end_warps_meet);
+        if (DOWN) end_warps_meet();  // acc is written over next
+        if (b == tile1) ++tile;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + 8 * kXpGroups);
+      if (++sum_at == n_sums) sum_at = 0, sum_ph ^= 1u;
     }
   }
   __syncthreads();
+  if (b0 < b1) {
+    const int seg = (b1 - 1) / nk, tile_segs = DOWN ? chunks : 1, tile = seg / tile_segs, tile0 = tile * tile_segs * nk;
+    const XpSegment s = walk.at(seg);
+    xp_tile_end<DOWN, kXpThreads>(p, r, s, shares.owner(tile0), shares.owner(tile0 + tile_segs * nk - 1), me,
+                                  DOWN ? acc : sums + (seg - seg0) % n_sums * cap * kXpLd, threadIdx.x, &s_last, cta_meets);
+  }
   if (threadIdx.x == 0 && s_abort) set_status(d.status, EUX_ST_TIMEOUT, DOWN ? 2 : 1);
 }
 
@@ -705,6 +852,7 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   p.h = (__nv_bfloat16*)d->workspace;
   p.part = (float*)((char*)d->workspace + xp_h_bytes(d));
   p.part_rows = xp_part_rows(d);
+  p.token_of = ((1 << 20) + d->topk - 1) / d->topk;
   int dev = 0;
   const int sms = xp_sms(&dev);
   CUtensorMap x, h;
