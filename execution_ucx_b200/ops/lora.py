@@ -85,7 +85,7 @@ class LoraAdapters:
                                                 ws.row_stride(y), ws.row_stride(out)), stream)
         if rc:
             _native.check(rc, "eux_lora_launch")
-        _launches += 1
+        _launches += 2 if t <= 64 else 3
         return out
 
     def _desc(self, tokens, x=0, ids=0, y=0, out=0, workspace=0, x_stride=0, y_stride=0, out_stride=0):
