@@ -4,16 +4,19 @@
 //
 // What bounds it: with many tokens x, y and out go through HBM once, 2 (K + 2N) bytes per token for 2 r (K + N) operations, at
 // ranks up to 128 still less than the tensor cores do in that time; with few tokens the adapters that are named, and latency.
-// Two kernels, `shrink` (x to v) and `expand` (v to out):
+// Two kernels, `shrink` (x to v) and `expand` (v to out), and for many tokens one in front:
 //
-// * Tokens come in tiles that share an adapter. Up to kLoraPlain tokens each token is a tile: nothing is sorted, and requests that
-//   share an adapter read it again from the L2. With more, a third kernel in front orders the tokens by adapter, in one CTA.
-// * shrink: a CTA has a tile and a part of K. x and A go through a ring of stages with cp.async; its four warps share the tile's
-//   rows (16 each) or, where the tile is one row, the part's K. v stays float32, one slice per part of K: nothing is added with
-//   atomics, expand adds the slices in their order.
-// * expand: a warp has 16 tokens and runs over a part of N, 32 columns at a time. v is its first operand, two bfloat16 numbers that add
-//   up to it (what is lost is 2^-16 of it, nothing beside the result's rounding), made in registers; B comes from L1 and L2 straight
-//   into registers, y is fetched before the product and out written behind it, 16 bytes per lane.
+// * Up to kLoraPlain tokens each stands for itself: nothing is sorted, and requests that share an adapter read it again from the L2.
+//   lora_shrink_one: a warp has some rows of A and a part of K, both straight into registers; parts of K are added up by expand.
+//   lora_expand_one: a row of B is read by as many lanes as it has 16-byte pieces; a lane group makes eight columns side by side.
+//   All in float32, no shared memory in the way: the chain id, A, v, B is four round trips to memory, and that is the time.
+// * With more, lora_order orders the tokens by adapter, in one CTA, and cuts them into tiles of up to kLoraTile that share one.
+//   lora_shrink: a cluster of CTAs has a tile, each a part of K; x and A go through a ring of stages with cp.async, four warps have
+//   16 rows each. The parts are added up through the cluster's shared memory, in order: v is written once, nothing is added with
+//   atomics.
+//   lora_expand: a warp has 16 tokens and runs over a part of N, 32 columns at a time. v is its first operand, two bfloat16 numbers that
+//   add up to it (what is lost is 2^-16 of it, nothing beside the result's rounding), made in registers; B comes from L1 and L2
+//   straight into registers. The next columns' y and B are fetched before the product of these.
 #include <algorithm>
 
 #include "eux_device.cuh"
@@ -24,17 +27,18 @@ constexpr int kLoraPlain = 64;        // tokens up to which each is a tile of it
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
 constexpr int kLoraStages = 4;
-constexpr int kLoraMaxSlices = 32;
+constexpr int kLoraMaxSlices = 16;    // parts of K of a token
+constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
 struct LoraParams {
   eux_lora_desc d;
-  float* v;          // [slices][n_tokens][rank]
-  int4* tiles;       // {adapter, first place in order, tokens, -} of each tile; null: tile t is token t
+  float* v;          // [slices][n_tokens][rank]; with tiles [n_tokens][rank] in the order of the tokens' places
+  int4* tiles;       // {adapter, first place in order, tokens, -} of each tile
   int* order;        // tokens, those of an adapter side by side
   int* n_tiles;
   int slices;        // parts of K
-  int per_slice;     // of K, a multiple of 64
-  int per_cta;       // of N, a multiple of 32
+  int per_slice;     // of K, a multiple of 256
+  int per_cta;       // of N, a multiple of 128
 };
 
 __device__ __forceinline__ uint32_t lora_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -60,48 +64,165 @@ constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr size_t kOrderSmem = 200 * 1024;  // for the counts, where they fit
 
-// Where a tile's tokens are.
-struct LoraTile {
-  int adapter, first, n;
-};
-__device__ __forceinline__ bool lora_tile(const LoraParams& p, int i, LoraTile* t) {
-  const eux_lora_desc& d = p.d;
-  if (!p.tiles) {
-    const int id = d.ids[i];
-    t->adapter = (uint32_t)id < (uint32_t)d.n_adapters ? id : d.n_adapters, t->first = i, t->n = 1;
-    return true;
-  }
-  if (i >= *p.n_tiles) return false;
-  const int4 v = p.tiles[i];
-  t->adapter = v.x, t->first = v.y, t->n = v.z;
-  return true;
+__device__ __forceinline__ int lora_adapter(const eux_lora_desc& d, int64_t token) {  // n_adapters: none
+  const int id = d.ids[token];
+  return (uint32_t)id < (uint32_t)d.n_adapters ? id : d.n_adapters;
 }
 
+// ---- a token at a time ----
+
+__device__ __forceinline__ void lora_floats(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* const h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __bfloat1622float2(h[i]);
+    f[2 * i] = t.x, f[2 * i + 1] = t.y;
+  }
+}
+
+// Grid: tokens, parts of K, ranks in 32s. A warp has eight rows of A.
+__global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __grid_constant__ LoraParams p) {
+  const eux_lora_desc& d = p.d;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t token = blockIdx.x;
+  const int r0 = blockIdx.z * 32 + warp * 8;
+  wait_for_launch_before();
+  const int adapter = lora_adapter(d, token);
+  const int k0 = blockIdx.y * p.per_slice, k1 = min(d.k, k0 + p.per_slice);
+  if (r0 < d.rank && adapter < d.n_adapters) {
+    const __nv_bfloat16* const x = (const __nv_bfloat16*)d.x + token * d.x_stride;
+    const __nv_bfloat16* const a = (const __nv_bfloat16*)d.a + ((int64_t)adapter * d.rank + r0) * d.k;
+    float acc[8] = {};
+    for (int k = k0 + lane * 8; k < k1; k += 256) {
+      const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + k));
+      uint4 av[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) av[r] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)r * d.k + k));
+      float xf[8];
+      lora_floats(xv, xf);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float af[8];
+        lora_floats(av[r], af);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r] = fmaf(af[i], xf[i], acc[r]);
+      }
+    }
+    // row `lane & 7` is added up in lanes that have it, halving what each has
+#pragma unroll
+    for (int o = 4; o; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < o) {
+          const bool upper = lane & o;
+          const float give = upper ? acc[r] : acc[r + o], keep = upper ? acc[r + o] : acc[r];
+          acc[r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    float v = acc[0];
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    if (lane < 8) p.v[((int64_t)blockIdx.y * d.n_tokens + token) * d.rank + r0 + lane] = v;
+  }
+  allow_next_launch();
+}
+
+// Grid: tokens, parts of N. LANES: that share a row of B, a power of two of at least rank / 8.
+template <int LANES>
+__global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __grid_constant__ LoraParams p) {
+  const eux_lora_desc& d = p.d;
+  __shared__ float parts[kLoraMaxSlices][EUX_LORA_MAX_RANK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t token = blockIdx.x;
+  const int sub = lane % LANES, group = lane / LANES;
+  const int n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta);
+  wait_for_launch_before();
+  const int adapter = lora_adapter(d, token);
+  const bool has = adapter < d.n_adapters;
+  float v[8] = {};
+  if (has) {
+    for (int i = threadIdx.x; i < p.slices * d.rank; i += kLoraThreads) {
+      const int s = i / d.rank, r = i - s * d.rank;
+      parts[s][r] = __ldcg(p.v + ((int64_t)s * d.n_tokens + token) * d.rank + r);
+    }
+    __syncthreads();
+    const float scale = d.scale[adapter];
+    if (sub * 8 < d.rank) {
+      for (int s = 0; s < p.slices; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += parts[s][sub * 8 + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= scale;
+  }
+  const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? adapter : 0) * d.n * d.rank;
+  constexpr int GROUPS = 32 / LANES;
+  for (int n = n0 + (warp * GROUPS + group) * 8; n < n1; n += 4 * GROUPS * 8) {  // n1 is a multiple of 8: a group is all there or not at all
+    uint4 y;
+    if (sub == 0) y = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.y + token * d.y_stride + n);
+    float acc[8] = {};
+    if (has && sub * 8 < d.rank) {
+      uint4 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)(n + i) * d.rank + sub * 8));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+        lora_floats(w[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i] = fmaf(f[j], v[j], acc[i]);
+      }
+    }
+    const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (group * LANES);
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor_sync(mask, acc[i], o);
+    if (sub == 0) {
+      if (has) {
+        __nv_bfloat162* const y2 = reinterpret_cast<__nv_bfloat162*>(&y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __bfloat1622float2(y2[i]);
+          y2[i] = __floats2bfloat162_rn(f.x + acc[2 * i], f.y + acc[2 * i + 1]);
+        }
+      }
+      st_u4((__nv_bfloat16*)d.out + token * d.out_stride + n, y);
+    }
+  }
+  allow_next_launch();
+}
+
+// ---- tiles of tokens that share an adapter ----
+
 // Tokens ordered by adapter, those without one behind all (as adapter n_adapters: expand copies their rows), and the tiles. One CTA,
-// whose warps each count a run of tokens per adapter, `counts` [n_adapters + 1][warps]: null if they lie in shared memory.
+// whose warps each count a run of tokens per adapter, `counts` [warps][n_adapters + 1]: null if they lie in shared memory.
 __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_constant__ LoraParams p, int* counts) {
   extern __shared__ int order_smem[];
-  if (!counts) counts = order_smem;
   __shared__ int sums[kOrderWarps], tile_sums[kOrderWarps];
+  if (!counts) counts = order_smem;
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, A = d.n_adapters + 1;
-  const int each = ((d.n_tokens + kOrderWarps - 1) / kOrderWarps + 31) & ~31, lo = min(d.n_tokens, warp * each), hi = min(d.n_tokens, lo + each);
+  const int used = min(kOrderWarps, (d.n_tokens + 31) / 32);
+  const int each = ((d.n_tokens + used - 1) / used + 31) & ~31, lo = min(d.n_tokens, warp * each), hi = min(d.n_tokens, lo + each);
   const uint32_t below = (1u << lane) - 1u;
+  int* const mine = counts + (int64_t)warp * A;
+  for (int64_t i = threadIdx.x; i < (int64_t)A * used; i += kOrderThreads) counts[i] = 0;
   wait_for_launch_before();
-  for (int i = threadIdx.x; i < A * kOrderWarps; i += kOrderThreads) counts[i] = 0;
+  const int first = lo + lane < hi ? lora_adapter(d, lo + lane) : -1;
   __syncthreads();
-  auto adapter = [&](int i) {
-    const int id = i < hi ? d.ids[i] : -1;
-    return (uint32_t)id < (uint32_t)d.n_adapters ? id : d.n_adapters;
-  };
-  for (int i = lo + lane; i < hi; i += 32) atomicAdd(counts + adapter(i) * kOrderWarps + warp, 1);
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane, a = i0 == lo ? first : i < hi ? lora_adapter(d, i) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, a);
+    if (a >= 0 && (same & below) == 0) mine[a] += __popc(same);
+    __syncwarp();
+  }
   __syncthreads();
   int all = 0, tiles = 0;
   for (int a0 = 0; a0 < A; a0 += kOrderThreads) {
     const int a = a0 + threadIdx.x;
     int c = 0;
     if (a < A)
-      for (int w = 0; w < kOrderWarps; ++w) c += counts[a * kOrderWarps + w];
+      for (int w = 0; w < used; ++w) c += counts[(int64_t)w * A + a];
     const int t = (c + kLoraTile - 1) / kLoraTile;
     int sum = c, tsum = t;
     for (int o = 1; o < 32; o <<= 1) {
@@ -117,12 +238,11 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
     }
     at += sum - c, tile += tsum - t;
     if (c) {
-      // tiles of equal size
-      const int n = (c + t - 1) / t;
+      const int n = (c + t - 1) / t;  // tiles of equal size
       for (int i = 0; i < t; ++i) p.tiles[tile + i] = make_int4(a, at + i * n, min(n, c - i * n), 0);
-      for (int w = 0; w < kOrderWarps; ++w) {  // from counts to places
-        const int m = counts[a * kOrderWarps + w];
-        counts[a * kOrderWarps + w] = at;
+      for (int w = 0; w < used; ++w) {  // from counts to places
+        const int m = counts[(int64_t)w * A + a];
+        counts[(int64_t)w * A + a] = at;
         at += m;
       }
     }
@@ -130,59 +250,83 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
   }
   if (threadIdx.x == 0) *p.n_tiles = tiles;
   for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane, a = adapter(i);
-    const uint32_t same = __match_any_sync(0xffffffffu, i < hi ? a : -1);
+    const int i = i0 + lane, a = i0 == lo ? first : i < hi ? lora_adapter(d, i) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, a);
     const int before = __popc(same & below);
-    if (i < hi) p.order[counts[a * kOrderWarps + warp] + before] = i;
+    if (a >= 0) p.order[mine[a] + before] = i;
     __syncwarp();
-    if (i < hi && before == 0) counts[a * kOrderWarps + warp] += __popc(same);
+    if (a >= 0 && before == 0) mine[a] += __popc(same);
     __syncwarp();
   }
   allow_next_launch();
 }
 
-// What a stage of shrink holds.
-template <int R8, bool ONE>
-struct LoraStage {
-  static constexpr int KS = ONE && R8 == 16 ? 2 : 4;           // of K: 16s per warp
-  static constexpr int STEP = ONE ? KS * 64 : KS * 16;         // of K: a token's is shared by the warps
-  static constexpr int ROWS = ONE ? 1 : kLoraTile;             // of x
-  static constexpr int X = ROWS * STEP * 2, BYTES = X + R8 * 8 * STEP * 2;
+struct LoraTile {
+  int adapter, first, n;
 };
+__device__ __forceinline__ bool lora_tile(const LoraParams& p, int i, LoraTile* t) {
+  if (i >= *p.n_tiles) return false;
+  const int4 v = p.tiles[i];
+  t->adapter = v.x, t->first = v.y, t->n = v.z;
+  return true;
+}
 
-// R8: ranks in eights, rounded up to a power of two. ONE: tiles of one token, whose warps share K.
-template <int R8, bool ONE>
+__device__ __forceinline__ void lora_cluster_meets() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 lora_ld_cluster(uint32_t at, uint32_t cta) {
+  uint32_t there;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+  return v;
+}
+
+// R8: ranks in eights, rounded up to a power of two.
+template <int R8>
 __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  using S = LoraStage<R8, ONE>;
-  constexpr int STEP = S::STEP, ROWS = S::ROWS, X = S::X, PIECES = STEP / 8;  // 16-byte pieces of a row
+  constexpr int STEP = 64, PIECES = STEP / 8;  // of K in a stage; 16-byte pieces of a row
+  constexpr int X = kLoraTile * STEP * 2, STAGE = X + R8 * 8 * STEP * 2;
+  constexpr int LD = R8 * 8 + 4;               // floats between the tile's rows when it is added up
   extern __shared__ __align__(1024) unsigned char lora_smem_raw[];
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   wait_for_launch_before();
   LoraTile t;
-  if (!lora_tile(p, blockIdx.x, &t) || t.adapter == d.n_adapters) {
+  if (!lora_tile(p, blockIdx.x, &t) || t.adapter == d.n_adapters) {  // all CTAs of the cluster
     allow_next_launch();
     return;
   }
-  const int k0 = blockIdx.y * p.per_slice, k1 = min(d.k, k0 + p.per_slice), steps = (k1 - k0 + STEP - 1) / STEP;
+  const int k0 = blockIdx.y * p.per_slice, k1 = min(d.k, k0 + p.per_slice), steps = max(0, (k1 - k0 + STEP - 1) / STEP);
   const uint32_t smem = lora_smem(lora_smem_raw);
-  const __nv_bfloat16* const a = (const __nv_bfloat16*)d.a + (int64_t)t.adapter * d.rank * d.k;
-  // a row's pieces are swizzled within 128 bytes
-  auto place = [](int row, int piece) { return row * (STEP * 2) + (piece & ~7) * 16 + (((piece ^ row) & 7) << 4); };
+  auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
+  // What this thread fetches of every stage: a piece of each sixteenth row of x and of A.
+  constexpr int XR = kLoraTile / 16, AR = (R8 * 8 + 15) / 16;
+  const int row = threadIdx.x / PIECES, piece = threadIdx.x % PIECES;
+  const __nv_bfloat16 *x[XR], *a[AR];
+#pragma unroll
+  for (int i = 0; i < XR; ++i) {
+    const int r = row + 16 * i;
+    x[i] = r < t.n ? (const __nv_bfloat16*)d.x + p.order[t.first + r] * d.x_stride : nullptr;
+  }
+#pragma unroll
+  for (int i = 0; i < AR; ++i) {
+    const int r = row + 16 * i;
+    a[i] = r < d.rank ? (const __nv_bfloat16*)d.a + ((int64_t)t.adapter * d.rank + r) * d.k : nullptr;
+  }
   auto fetch = [&](int step) {
     if (step < steps) {
-      const uint32_t at = smem + step % kLoraStages * S::BYTES;
-      const int k = k0 + step * STEP;
-      for (int i = threadIdx.x; i < ROWS * PIECES; i += kLoraThreads) {
-        const int row = i / PIECES, piece = i % PIECES;
-        const bool some = row < t.n && k + piece * 8 < k1;
-        const int64_t token = some ? (p.tiles ? p.order[t.first + row] : t.first) : 0;
-        lora_cp_16(at + place(row, piece), (const __nv_bfloat16*)d.x + token * d.x_stride + (some ? k + piece * 8 : 0), some);
+      const uint32_t at = smem + step % kLoraStages * STAGE;
+      const int k = k0 + step * STEP + piece * 8;
+#pragma unroll
+      for (int i = 0; i < XR; ++i) {
+        const bool some = x[i] && k < k1;
+        lora_cp_16(at + place(row + 16 * i, piece), some ? x[i] + k : (const __nv_bfloat16*)d.x, some);
       }
-      for (int i = threadIdx.x; i < R8 * 8 * PIECES; i += kLoraThreads) {
-        const int row = i / PIECES, piece = i % PIECES;
-        const bool some = row < d.rank && k + piece * 8 < k1;
-        lora_cp_16(at + X + place(row, piece), a + (some ? (int64_t)row * d.k + k + piece * 8 : 0), some);
+#pragma unroll
+      for (int i = 0; i < AR; ++i) {
+        const bool some = a[i] && k < k1;
+        if (row + 16 * i < R8 * 8) lora_cp_16(at + X + place(row + 16 * i, piece), some ? a[i] + k : (const __nv_bfloat16*)d.a, some);
       }
     }
     lora_cp_commit();
@@ -193,32 +337,22 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     lora_cp_wait<kLoraStages - 2>();
     __syncthreads();
     fetch(s + kLoraStages - 1);
-    const uint32_t x = smem + s % kLoraStages * S::BYTES, w = x + X;
-    if (ONE || warp * 16 < t.n) {
+    const uint32_t xs = smem + s % kLoraStages * STAGE, w = xs + X;
+    if (warp * 16 < t.n) {
 #pragma unroll
-      for (int ks = 0; ks < S::KS; ++ks) {
-        const int piece = (ONE ? warp * S::KS * 2 : 0) + ks * 2;
+      for (int ks = 0; ks < STEP / 16; ++ks) {
         uint32_t av[4];
-        if (ONE) {
-          // the token is row 0, which lanes 0 to 3 hold; the others hold zeros
-          av[0] = av[1] = av[2] = av[3] = 0;
-          if (g == 0) {
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(av[0]) : "r"(x + place(0, piece) + 4 * c) : "memory");
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(av[2]) : "r"(x + place(0, piece + 1) + 4 * c) : "memory");
-          }
-        } else {
-          lora_ldsm_x4(av, x + place(warp * 16 + (lane & 15), piece + (lane >> 4)));
-        }
+        lora_ldsm_x4(av, xs + place(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)));
 #pragma unroll
         for (int j = 0; j < R8; j += 2) {
           if (R8 > 1) {
             uint32_t b[4];
-            lora_ldsm_x4(b, w + place(j * 8 + (lane & 7) + ((lane >> 4) << 3), piece + ((lane >> 3) & 1)));
+            lora_ldsm_x4(b, w + place(j * 8 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
             lora_mma(acc[j], av, b[0], b[1]);
             lora_mma(acc[j + (R8 > 1)], av, b[2], b[3]);
           } else {
             uint32_t b0, b1;
-            lora_ldsm_x2(b0, b1, w + place(lane & 7, piece + ((lane >> 3) & 1)));
+            lora_ldsm_x2(b0, b1, w + place(lane & 7, ks * 2 + ((lane >> 3) & 1)));
             lora_mma(acc[j], av, b0, b1);
           }
         }
@@ -226,31 +360,32 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     }
   }
   lora_cp_wait<0>();
-  float* const v = p.v + (int64_t)blockIdx.y * d.n_tokens * d.rank;
-  if (ONE) {
-    __shared__ float part[4][R8 * 8];
-    if (g == 0)
+  __syncthreads();
+  float* const tile = reinterpret_cast<float*>(lora_smem_raw);
 #pragma unroll
-      for (int j = 0; j < R8; ++j) part[warp][j * 8 + 2 * c] = acc[j][0], part[warp][j * 8 + 2 * c + 1] = acc[j][1];
-    __syncthreads();
-    for (int i = threadIdx.x; i < d.rank; i += kLoraThreads) v[(int64_t)t.first * d.rank + i] = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-  } else {
-    // by place, not by token: expand reads a tile's rows side by side
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = warp * 16 + g + 8 * h;
-      if (row < t.n)
-#pragma unroll
-        for (int j = 0; j < R8; ++j)
-          if (j * 8 < d.rank) *reinterpret_cast<float2*>(v + (int64_t)(t.first + row) * d.rank + j * 8 + 2 * c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+    for (int j = 0; j < R8; ++j)
+      *reinterpret_cast<float2*>(tile + (warp * 16 + g + 8 * h) * LD + j * 8 + 2 * c) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+  lora_cluster_meets();
+  // each CTA adds up its share of the tile's rows, by the parts of K in their order; rows lie by place, not by token
+  const int slices = p.slices, q = d.rank / 4;
+  for (int i = threadIdx.x + blockIdx.y * kLoraThreads; i < t.n * q; i += kLoraThreads * slices) {
+    const int r = i / q, e = i % q * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < slices; ++s) {
+      const float4 o = lora_ld_cluster(smem + (r * LD + e) * 4, s);
+      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
     }
+    *reinterpret_cast<float4*>(p.v + (int64_t)(t.first + r) * d.rank + e) = v;
   }
+  lora_cluster_meets();  // the others have read this one's
   allow_next_launch();
 }
 
 // K32: ranks in 32s. A lane's eight values of K are side by side (the order of K is the product's own affair), and so are its eight
 // columns of 32 (column 2c + i of the product's n-th eight is 8c + 2n + i of the 32).
-template <int K32, bool ONE>
+template <int K32>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
@@ -261,18 +396,38 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     return;
   }
   const bool has = t.adapter < d.n_adapters;
-  // a tile of one token: the warps share the columns
-  const int row0 = ONE ? 0 : warp * 16, n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta);
+  const int row0 = warp * 16, n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta);
   if (row0 < t.n) {
     // this lane's rows: g and g + 8 of the warp's
-    int64_t token[2];
+    const __nv_bfloat16* y_row[2];
+    __nv_bfloat16* out_row[2];
     bool row[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = row0 + g + 8 * h;
       row[h] = r < t.n;
-      token[h] = row[h] ? (p.tiles ? p.order[t.first + r] : t.first) : 0;
+      const int64_t token = row[h] ? p.order[t.first + r] : 0;
+      y_row[h] = (const __nv_bfloat16*)d.y + token * d.y_stride, out_row[h] = (__nv_bfloat16*)d.out + token * d.out_stride;
     }
+    const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? t.adapter : 0) * d.n * d.rank;
+    constexpr bool AHEAD = K32 <= 2;  // B of the next columns: there are registers for it
+    uint4 y[2], next_y[2], w[4][K32];
+    auto fetch_y = [&](uint4 (&to)[2], int n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (row[h] && n + c * 8 < n1) to[h] = *reinterpret_cast<const uint4*>(y_row[h] + n + c * 8);
+    };
+    auto fetch_w = [&](int n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = n + (g >> 1) * 8 + j * 2 + (g & 1);  // the row of B for this lane's column
+#pragma unroll
+        for (int k = 0; k < K32; ++k)
+          w[j][k] = has && at < n1 && k * 32 + c * 8 < d.rank ? __ldg(reinterpret_cast<const uint4*>(b + (int64_t)at * d.rank + k * 32 + c * 8)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    fetch_y(next_y, n0);
+    if (AHEAD) fetch_w(n0);
     uint32_t hi[K32][2][4], lo[K32][2][4];  // first operands of 16 of K
     if (has) {
       const float scale = d.scale[t.adapter];
@@ -280,60 +435,54 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
       for (int k = 0; k < K32; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float v[8] = {};
+          float4 q0 = make_float4(0.f, 0.f, 0.f, 0.f), q1 = q0;
           if (row[h] && k * 32 + c * 8 < d.rank) {
-            const float* at = p.v + (int64_t)(t.first + row0 + g + 8 * h) * d.rank + k * 32 + c * 8;
-            for (int s = 0; s < p.slices; ++s, at += (int64_t)d.n_tokens * d.rank) {
-              const float4 q0 = __ldcg(reinterpret_cast<const float4*>(at)), q1 = __ldcg(reinterpret_cast<const float4*>(at) + 1);
-              v[0] += q0.x, v[1] += q0.y, v[2] += q0.z, v[3] += q0.w, v[4] += q1.x, v[5] += q1.y, v[6] += q1.z, v[7] += q1.w;
-            }
+            const float* const at = p.v + (int64_t)(t.first + row0 + g + 8 * h) * d.rank + k * 32 + c * 8;
+            q0 = __ldcg(reinterpret_cast<const float4*>(at)), q1 = __ldcg(reinterpret_cast<const float4*>(at) + 1);
           }
+          const float v[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const float v0 = v[2 * q] * scale, v1 = v[2 * q + 1] * scale;
             const __nv_bfloat162 u = __floats2bfloat162_rn(v0, v1);
             const float2 f = __bfloat1622float2(u);
             // nothing is lost of an infinity
-            const __nv_bfloat162 w = __floats2bfloat162_rn(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
+            const __nv_bfloat162 l = __floats2bfloat162_rn(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
             // pairs 0 and 1 are the first 16's k = 2c and 2c + 8, pairs 2 and 3 the second's
             hi[k][q >> 1][(q & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&u);
-            lo[k][q >> 1][(q & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&w);
+            lo[k][q >> 1][(q & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&l);
           }
         }
     }
-    const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? t.adapter : 0) * d.n * d.rank;
-    for (int n = n0 + (ONE ? warp * 32 : 0); n < n1; n += ONE ? 128 : 32) {
-      uint4 y[2];
-      const int col = n + c * 8;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (row[h] && col < d.n) y[h] = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.y + token[h] * d.y_stride + col);
+    for (int n = n0; n < n1; n += 32) {
+      y[0] = next_y[0], y[1] = next_y[1];
+      fetch_y(next_y, n + 32);
+      if (!AHEAD) fetch_w(n);
+      float acc[4][4] = {};
       if (has) {
-        float acc[4][4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = n + (g >> 1) * 8 + j * 2 + (g & 1);  // the row of B for this lane's column
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int k = 0; k < K32; ++k) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (at < d.n && k * 32 + c * 8 < d.rank) w = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)at * d.rank + k * 32 + c * 8));
-            lora_mma(acc[j], hi[k][0], w.x, w.y), lora_mma(acc[j], hi[k][1], w.z, w.w);
-            lora_mma(acc[j], lo[k][0], w.x, w.y), lora_mma(acc[j], lo[k][1], w.z, w.w);
+            const uint4 b4 = w[j][k];
+            lora_mma(acc[j], hi[k][0], b4.x, b4.y), lora_mma(acc[j], hi[k][1], b4.z, b4.w);
+            lora_mma(acc[j], lo[k][0], b4.x, b4.y), lora_mma(acc[j], lo[k][1], b4.z, b4.w);
           }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          __nv_bfloat162* const y2 = reinterpret_cast<__nv_bfloat162*>(&y[h]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = __bfloat1622float2(y2[j]);
-            y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
-          }
-        }
+        if (AHEAD) fetch_w(n + 32);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (row[h] && col < d.n) st_u4((__nv_bfloat16*)d.out + token[h] * d.out_stride + col, y[h]);
+        if (row[h] && n + c * 8 < n1) {
+          if (has) {
+            __nv_bfloat162* const y2 = reinterpret_cast<__nv_bfloat162*>(&y[h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = __bfloat1622float2(y2[j]);
+              y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
+            }
+          }
+          st_u4(out_row[h] + n + c * 8, y[h]);
+        }
     }
   }
   allow_next_launch();
@@ -358,67 +507,56 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
   constexpr int kSms = 148;
   s.one = d->n_tokens <= kLoraPlain;
   s.tiles = s.one ? d->n_tokens : (int)std::min<int64_t>(d->n_tokens, d->n_tokens / kLoraTile + (int64_t)d->n_adapters + 1);
-  const int likely = s.one ? d->n_tokens : (d->n_tokens + kLoraTile - 1) / kLoraTile;
-  // Parts of K for about four CTAs per SM, of 256 (512: a token's) at least
-  const int step = s.one ? 512 : 256;
-  int want = std::max(1, std::min(kLoraMaxSlices, 4 * kSms / likely));
-  want = std::min(want, (d->k + step - 1) / step);
+  // Parts of K and of N for about four CTAs per SM
+  const int likely = s.one ? d->n_tokens : (d->n_tokens + kLoraTile - 1) / kLoraTile, most = s.one ? kLoraMaxSlices : kLoraCluster;
+  int want = std::max(1, std::min({most, 4 * kSms / likely, (d->k + 255) / 256}));
+  if (!s.one)
+    while (want & (want - 1)) want &= want - 1;  // a cluster
   s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
-  s.slices = (d->k + s.per_slice - 1) / s.per_slice;
-  // Parts of N likewise, of 128 at least
-  int parts = std::max(1, std::min(4 * kSms / likely, (d->n + 127) / 128));
+  s.slices = s.one ? (d->k + s.per_slice - 1) / s.per_slice : want;
+  const int parts = std::max(1, std::min(4 * kSms / likely, (d->n + 127) / 128));
   s.per_cta = ((d->n + parts - 1) / parts + 127) / 128 * 128;
   s.parts = (d->n + s.per_cta - 1) / s.per_cta;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  s.v_bytes = up((size_t)s.slices * d->n_tokens * d->rank * 4);
+  s.v_bytes = up((size_t)(s.one ? s.slices : 1) * d->n_tokens * d->rank * 4);
   s.tile_bytes = s.one ? 0 : up(((size_t)s.tiles + 1) * 16);
   s.order_bytes = s.one ? 0 : up((size_t)d->n_tokens * 4);
   s.count_bytes = s.one ? 0 : up(((size_t)d->n_adapters + 1) * kOrderWarps * 4);
   return s;
 }
 
-template <int R8, bool ONE>
+// A launch that may begin while the kernel before it ends, of clusters of `cluster` CTAs along y.
+static int lora_launch(void (*kernel)(LoraParams), dim3 grid, int cluster, size_t smem, cudaStream_t st, const LoraParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = dim3(kLoraThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1, attr[1].val.clusterDim.y = (unsigned)cluster, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, p);
+}
+template <int R8>
 static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
-  constexpr size_t smem = (size_t)kLoraStages * LoraStage<R8, ONE>::BYTES;
+  constexpr size_t smem = std::max<size_t>(kLoraStages * (kLoraTile + R8 * 8) * 128, (size_t)kLoraTile * (R8 * 8 + 4) * 4);
   if (smem > 48 * 1024)
-    if (cudaError_t e = allow_smem<lora_shrink_kernel<R8, ONE>>(dev, smem); e != cudaSuccess) return (int)e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(s.tiles, s.slices), cfg.blockDim = dim3(kLoraThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, lora_shrink_kernel<R8, ONE>, p);
-}
-template <int K32, bool ONE>
-static int lora_expand(const LoraParams& p, const LoraShape& s, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(s.tiles, s.parts), cfg.blockDim = dim3(kLoraThreads), cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, lora_expand_kernel<K32, ONE>, p);
+    if (cudaError_t e = allow_smem<lora_shrink_kernel<R8>>(dev, smem); e != cudaSuccess) return (int)e;
+  return lora_launch(lora_shrink_kernel<R8>, dim3(s.tiles, s.slices), s.slices, smem, st, p);
 }
 
-template <bool ONE>
-static int lora_run(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
+static int lora_run_one(const LoraParams& p, const LoraShape& s, cudaStream_t st) {
   const int r = p.d.rank;
-  int rc = r <= 8 ? lora_shrink<1, ONE>(p, s, dev, st) : r <= 16 ? lora_shrink<2, ONE>(p, s, dev, st) : r <= 32 ? lora_shrink<4, ONE>(p, s, dev, st)
-           : r <= 64 ? lora_shrink<8, ONE>(p, s, dev, st) : lora_shrink<16, ONE>(p, s, dev, st);
-  if (rc) return rc;
-  return r <= 32 ? lora_expand<1, ONE>(p, s, st) : r <= 64 ? lora_expand<2, ONE>(p, s, st) : lora_expand<4, ONE>(p, s, st);
+  if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, s.slices, (r + 31) / 32), 1, 0, st, p)) return rc;
+  return lora_launch(r <= 8 ? lora_expand_one_kernel<1> : r <= 16 ? lora_expand_one_kernel<2> : r <= 32 ? lora_expand_one_kernel<4>
+                     : r <= 64 ? lora_expand_one_kernel<8> : lora_expand_one_kernel<16>, dim3(s.tiles, s.parts), 1, 0, st, p);
 }
-
-template <bool ONE>
-static int lora_preload() {
-  cudaFuncAttributes a;
-  const void* kernels[] = {(const void*)lora_shrink_kernel<1, ONE>, (const void*)lora_shrink_kernel<2, ONE>, (const void*)lora_shrink_kernel<4, ONE>,
-                           (const void*)lora_shrink_kernel<8, ONE>, (const void*)lora_shrink_kernel<16, ONE>, (const void*)lora_expand_kernel<1, ONE>,
-                           (const void*)lora_expand_kernel<2, ONE>, (const void*)lora_expand_kernel<4, ONE>, (const void*)lora_order_kernel};
-  for (const void* k : kernels)
-    if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;
-  return 0;
+static int lora_run_tiles(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
+  const int r = p.d.rank;
+  const int rc = r <= 8 ? lora_shrink<1>(p, s, dev, st) : r <= 16 ? lora_shrink<2>(p, s, dev, st) : r <= 32 ? lora_shrink<4>(p, s, dev, st)
+                 : r <= 64 ? lora_shrink<8>(p, s, dev, st) : lora_shrink<16>(p, s, dev, st);
+  if (rc) return rc;
+  return lora_launch(r <= 32 ? lora_expand_kernel<1> : r <= 64 ? lora_expand_kernel<2> : lora_expand_kernel<4>, dim3(s.tiles, s.parts), 1, 0, st, p);
 }
 
 }  // namespace eux
@@ -446,17 +584,24 @@ extern "C" int eux_lora_launch(const eux_lora_desc* d, void* stream) {
   p.slices = s.slices, p.per_slice = s.per_slice, p.per_cta = s.per_cta;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (s.one) return lora_run<true>(p, s, dev, st);
+  if (s.one) return lora_run_one(p, s, st);
   p.n_tiles = (int*)at, p.tiles = (int4*)at + 1, at += s.tile_bytes;
   p.order = (int*)at, at += s.order_bytes;
   const size_t count_bytes = ((size_t)d->n_adapters + 1) * kOrderWarps * 4;
   const bool in_smem = count_bytes <= kOrderSmem;
   if (cudaError_t e = allow_smem<lora_order_kernel>(dev, kOrderSmem); e != cudaSuccess) return (int)e;
   if (int rc = launch_early(lora_order_kernel, 1, kOrderThreads, in_smem ? count_bytes : 0, st, p, in_smem ? (int*)nullptr : (int*)at)) return rc;
-  return lora_run<false>(p, s, dev, st);
+  return lora_run_tiles(p, s, dev, st);
 }
 
 extern "C" int eux_lora_preload(void) {
-  if (int rc = lora_preload<true>()) return rc;
-  return lora_preload<false>();
+  cudaFuncAttributes a;
+  const void* kernels[] = {(const void*)lora_shrink_one_kernel, (const void*)lora_expand_one_kernel<1>, (const void*)lora_expand_one_kernel<2>,
+                           (const void*)lora_expand_one_kernel<4>, (const void*)lora_expand_one_kernel<8>, (const void*)lora_expand_one_kernel<16>,
+                           (const void*)lora_order_kernel, (const void*)lora_shrink_kernel<1>, (const void*)lora_shrink_kernel<2>,
+                           (const void*)lora_shrink_kernel<4>, (const void*)lora_shrink_kernel<8>, (const void*)lora_shrink_kernel<16>,
+                           (const void*)lora_expand_kernel<1>, (const void*)lora_expand_kernel<2>, (const void*)lora_expand_kernel<4>};
+  for (const void* k : kernels)
+    if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;
+  return 0;
 }
