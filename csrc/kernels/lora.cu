@@ -27,7 +27,7 @@ constexpr int kLoraPlain = 64;        // tokens up to which each is a tile of it
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
 constexpr int kLoraStages = 4;
-constexpr int kLoraMaxSlices = 16;    // parts of K of a token
+constexpr int kLoraMaxSlices = 32;    // parts of K of a token
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
 struct LoraParams {
@@ -38,7 +38,7 @@ struct LoraParams {
   int* n_tiles;
   int slices;        // parts of K
   int per_slice;     // of K, a multiple of 256
-  int per_cta;       // of N, a multiple of 128
+  int per_cta;       // of N, a multiple of 64; with tiles of 128
 };
 
 __device__ __forceinline__ uint32_t lora_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -65,7 +65,7 @@ constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr size_t kOrderSmem = 200 * 1024;  // for the counts, where they fit
 
 __device__ __forceinline__ int lora_adapter(const eux_lora_desc& d, int64_t token) {  // n_adapters: none
-  const int id = d.ids[token];
+  const int id = __ldcg(d.ids + token);
   return (uint32_t)id < (uint32_t)d.n_adapters ? id : d.n_adapters;
 }
 
@@ -80,15 +80,16 @@ __device__ __forceinline__ void lora_floats(const uint4& v, float (&f)[8]) {
   }
 }
 
-// Grid: tokens, parts of K, ranks in 32s. A warp has eight rows of A.
+// Grid: tokens, and the warps that a token takes, each with eight rows of A and a part of K.
 __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __grid_constant__ LoraParams p) {
   const eux_lora_desc& d = p.d;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, unit = blockIdx.y * (kLoraThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = blockIdx.x;
-  const int r0 = blockIdx.z * 32 + warp * 8;
+  const int slice = unit % p.slices, r0 = unit / p.slices * 8;
   wait_for_launch_before();
+  allow_next_launch();  // expand's CTAs find room beside these, and have much to fetch that does not come from here
   const int adapter = lora_adapter(d, token);
-  const int k0 = blockIdx.y * p.per_slice, k1 = min(d.k, k0 + p.per_slice);
+  const int k0 = slice * p.per_slice, k1 = min(d.k, k0 + p.per_slice);
   if (r0 < d.rank && adapter < d.n_adapters) {
     const __nv_bfloat16* const x = (const __nv_bfloat16*)d.x + token * d.x_stride;
     const __nv_bfloat16* const a = (const __nv_bfloat16*)d.a + ((int64_t)adapter * d.rank + r0) * d.k;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __g
         for (int i = 0; i < 8; ++i) acc[r] = fmaf(af[i], xf[i], acc[r]);
       }
     }
-    // row `lane & 7` is added up in lanes that have it, halving what each has
+    // row `lane & 7` is added up in the lanes that have this number, halving what each has
 #pragma unroll
     for (int o = 4; o; o >>= 1)
 #pragma unroll
@@ -121,9 +122,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __g
     float v = acc[0];
     v += __shfl_xor_sync(0xffffffffu, v, 8);
     v += __shfl_xor_sync(0xffffffffu, v, 16);
-    if (lane < 8) p.v[((int64_t)blockIdx.y * d.n_tokens + token) * d.rank + r0 + lane] = v;
+    if (lane < 8) p.v[((int64_t)slice * d.n_tokens + token) * d.rank + r0 + lane] = v;
   }
-  allow_next_launch();
 }
 
 // Grid: tokens, parts of N. LANES: that share a row of B, a power of two of at least rank / 8.
@@ -134,10 +134,25 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __g
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t token = blockIdx.x;
   const int sub = lane % LANES, group = lane / LANES;
-  const int n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta);
-  wait_for_launch_before();
+  constexpr int GROUPS = 32 / LANES;
+  const int n0 = blockIdx.y * p.per_cta + (warp * GROUPS + group) * 8, n1 = min(d.n, blockIdx.y * p.per_cta + p.per_cta);
+  // Shrink was through with its wait for whatever is in front when it let this in: all but v is there, in the L2 (an L1 may hold what
+  // was there before).
   const int adapter = lora_adapter(d, token);
-  const bool has = adapter < d.n_adapters;
+  const bool has = adapter < d.n_adapters, some = has && sub * 8 < d.rank;
+  const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? adapter : 0) * d.n * d.rank + sub * 8;
+  uint4 y, w[8];
+  auto fetch = [&](int n) {  // n1 is a multiple of 8: eight columns are all there or not at all
+    if (n < n1) {
+      if (sub == 0) y = ld_cg_u4((const __nv_bfloat16*)d.y + token * d.y_stride + n);
+      if (some)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = ld_cg_u4(b + (int64_t)(n + i) * d.rank);
+    }
+  };
+  fetch(n0);
+  const float scale = has ? __ldcg(d.scale + adapter) : 0.f;
+  wait_for_launch_before();
   float v[8] = {};
   if (has) {
     for (int i = threadIdx.x; i < p.slices * d.rank; i += kLoraThreads) {
@@ -145,25 +160,17 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __g
       parts[s][r] = __ldcg(p.v + ((int64_t)s * d.n_tokens + token) * d.rank + r);
     }
     __syncthreads();
-    const float scale = d.scale[adapter];
-    if (sub * 8 < d.rank) {
+    if (some)
       for (int s = 0; s < p.slices; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += parts[s][sub * 8 + i];
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= scale;
   }
-  const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? adapter : 0) * d.n * d.rank;
-  constexpr int GROUPS = 32 / LANES;
-  for (int n = n0 + (warp * GROUPS + group) * 8; n < n1; n += 4 * GROUPS * 8) {  // n1 is a multiple of 8: a group is all there or not at all
-    uint4 y;
-    if (sub == 0) y = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.y + token * d.y_stride + n);
+  for (int n = n0; n < n1; n += 4 * GROUPS * 8) {
+    if (n != n0) fetch(n);
     float acc[8] = {};
-    if (has && sub * 8 < d.rank) {
-      uint4 w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)(n + i) * d.rank + sub * 8));
+    if (some) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float f[8];
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __g
         for (int j = 0; j < 8; ++j) acc[i] = fmaf(f[j], v[j], acc[i]);
       }
     }
-    const uint32_t mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (group * LANES);
+    const uint32_t mask = ((1u << LANES) - 1u) << (group * LANES);
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1)
 #pragma unroll
@@ -208,10 +215,21 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
   int* const mine = counts + (int64_t)warp * A;
   for (int64_t i = threadIdx.x; i < (int64_t)A * used; i += kOrderThreads) counts[i] = 0;
   wait_for_launch_before();
-  const int first = lo + lane < hi ? lora_adapter(d, lo + lane) : -1;
+  constexpr int KEPT = 8;  // a thread's first adapters, fetched at once
+  int kept[KEPT];
+#pragma unroll
+  for (int q = 0; q < KEPT; ++q) kept[q] = lo + q * 32 + lane < hi ? lora_adapter(d, lo + q * 32 + lane) : -1;
+  auto adapter_of = [&](int i0) {
+    int a = -1;
+    if (i0 - lo >= KEPT * 32) return i0 + lane < hi ? lora_adapter(d, i0 + lane) : -1;
+#pragma unroll
+    for (int q = 0; q < KEPT; ++q)
+      if (i0 == lo + q * 32) a = kept[q];
+    return a;
+  };
   __syncthreads();
   for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane, a = i0 == lo ? first : i < hi ? lora_adapter(d, i) : -1;
+    const int a = adapter_of(i0);
     const uint32_t same = __match_any_sync(0xffffffffu, a);
     if (a >= 0 && (same & below) == 0) mine[a] += __popc(same);
     __syncwarp();
@@ -232,9 +250,11 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
     if (lane == 31) sums[warp] = sum, tile_sums[warp] = tsum;
     __syncthreads();
     int at = all, tile = tiles;
-    for (int w = 0; w < kOrderWarps; ++w) {
-      if (w < warp) at += sums[w], tile += tile_sums[w];
-      all += sums[w], tiles += tile_sums[w];
+    {  // over the warps, by each warp
+      int u = sums[lane], v = tile_sums[lane];
+      const int before_u = __reduce_add_sync(0xffffffffu, lane < warp ? u : 0), before_v = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+      u = __reduce_add_sync(0xffffffffu, u), v = __reduce_add_sync(0xffffffffu, v);
+      at += before_u, tile += before_v, all += u, tiles += v;
     }
     at += sum - c, tile += tsum - t;
     if (c) {
@@ -250,7 +270,7 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
   }
   if (threadIdx.x == 0) *p.n_tiles = tiles;
   for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane, a = i0 == lo ? first : i < hi ? lora_adapter(d, i) : -1;
+    const int i = i0 + lane, a = adapter_of(i0);
     const uint32_t same = __match_any_sync(0xffffffffu, a);
     const int before = __popc(same & below);
     if (a >= 0) p.order[mine[a] + before] = i;
@@ -265,8 +285,8 @@ struct LoraTile {
   int adapter, first, n;
 };
 __device__ __forceinline__ bool lora_tile(const LoraParams& p, int i, LoraTile* t) {
-  if (i >= *p.n_tiles) return false;
-  const int4 v = p.tiles[i];
+  if (i >= __ldcg(p.n_tiles)) return false;
+  const int4 v = __ldcg(p.tiles + i);
   t->adapter = v.x, t->first = v.y, t->n = v.z;
   return true;
 }
@@ -332,6 +352,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     lora_cp_commit();
   };
   for (int s = 0; s < kLoraStages - 1; ++s) fetch(s);
+  allow_next_launch();
   float acc[R8][4] = {};
   for (int s = 0; s < steps; ++s) {
     lora_cp_wait<kLoraStages - 2>();
@@ -380,7 +401,6 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     *reinterpret_cast<float4*>(p.v + (int64_t)(t.first + r) * d.rank + e) = v;
   }
   lora_cluster_meets();  // the others have read this one's
-  allow_next_launch();
 }
 
 // K32: ranks in 32s. A lane's eight values of K are side by side (the order of K is the product's own affair), and so are its eight
@@ -389,9 +409,10 @@ template <int K32>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  wait_for_launch_before();
+  // Shrink was through with its wait for whatever is in front when it let this in: all but v is there, in the L2.
   LoraTile t;
   if (!lora_tile(p, blockIdx.x, &t)) {
+    wait_for_launch_before();  // what follows in the stream may rely on this kernel for what is in front of it
     allow_next_launch();
     return;
   }
@@ -406,7 +427,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     for (int h = 0; h < 2; ++h) {
       const int r = row0 + g + 8 * h;
       row[h] = r < t.n;
-      const int64_t token = row[h] ? p.order[t.first + r] : 0;
+      const int64_t token = row[h] ? __ldcg(p.order + t.first + r) : 0;
       y_row[h] = (const __nv_bfloat16*)d.y + token * d.y_stride, out_row[h] = (__nv_bfloat16*)d.out + token * d.out_stride;
     }
     const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? t.adapter : 0) * d.n * d.rank;
@@ -415,7 +436,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     auto fetch_y = [&](uint4 (&to)[2], int n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (row[h] && n + c * 8 < n1) to[h] = *reinterpret_cast<const uint4*>(y_row[h] + n + c * 8);
+        if (row[h] && n + c * 8 < n1) to[h] = ld_cg_u4(y_row[h] + n + c * 8);  // L1 is for B
     };
     auto fetch_w = [&](int n) {
 #pragma unroll
@@ -427,8 +448,9 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
       }
     };
     fetch_y(next_y, n0);
-    if (AHEAD) fetch_w(n0);
     uint32_t hi[K32][2][4], lo[K32][2][4];  // first operands of 16 of K
+    wait_for_launch_before();
+    if (AHEAD) fetch_w(n0);
     if (has) {
       const float scale = d.scale[t.adapter];
 #pragma unroll
@@ -481,10 +503,11 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
               y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
             }
           }
-          st_u4(out_row[h] + n + c * 8, y[h]);
+          st_stream_u4(out_row[h] + n + c * 8, y[h]);
         }
     }
   }
+  wait_for_launch_before();
   allow_next_launch();
 }
 
@@ -499,23 +522,35 @@ static int lora_check(const eux_lora_desc* d) {
 
 struct LoraShape {
   bool one;
-  int tiles, slices, per_slice, parts, per_cta;
+  int tiles, slices, per_slice, units, parts, per_cta;
   size_t v_bytes, tile_bytes, order_bytes, count_bytes;
 };
+// Columns that a CTA of lora_expand_one makes at a time.
+static int lora_width(int rank) { return rank <= 8 ? 1024 : rank <= 16 ? 512 : rank <= 32 ? 256 : rank <= 64 ? 128 : 64; }
 static LoraShape lora_shape(const eux_lora_desc* d) {
   LoraShape s;
   constexpr int kSms = 148;
   s.one = d->n_tokens <= kLoraPlain;
   s.tiles = s.one ? d->n_tokens : (int)std::min<int64_t>(d->n_tokens, d->n_tokens / kLoraTile + (int64_t)d->n_adapters + 1);
-  // Parts of K and of N for about four CTAs per SM
-  const int likely = s.one ? d->n_tokens : (d->n_tokens + kLoraTile - 1) / kLoraTile, most = s.one ? kLoraMaxSlices : kLoraCluster;
-  int want = std::max(1, std::min({most, 4 * kSms / likely, (d->k + 255) / 256}));
-  if (!s.one)
+  if (s.one) {
+    // As many warps as the SMs have places for about, each with 256 of K or a multiple; expand once over its columns, likewise.
+    const int64_t units = (int64_t)d->n_tokens * (d->rank / 8);
+    const int want = (int)std::max<int64_t>(1, std::min<int64_t>(kLoraMaxSlices, 32 * kSms / units));
+    s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
+    s.slices = (d->k + s.per_slice - 1) / s.per_slice;
+    s.units = s.slices * (d->rank / 8);
+    const int width = lora_width(d->rank), passes = (int)std::max<int64_t>(1, (int64_t)d->n_tokens * ((d->n + width - 1) / width) / (16 * kSms));
+    s.per_cta = width * passes;
+  } else {
+    // Parts of K and of N for about four CTAs per SM
+    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile;
+    int want = std::max(1, std::min({kLoraCluster, 4 * kSms / likely, (d->k + 255) / 256}));
     while (want & (want - 1)) want &= want - 1;  // a cluster
-  s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
-  s.slices = s.one ? (d->k + s.per_slice - 1) / s.per_slice : want;
-  const int parts = std::max(1, std::min(4 * kSms / likely, (d->n + 127) / 128));
-  s.per_cta = ((d->n + parts - 1) / parts + 127) / 128 * 128;
+    s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
+    s.slices = want;
+    const int parts = std::max(1, std::min(4 * kSms / likely, (d->n + 127) / 128));
+    s.per_cta = ((d->n + parts - 1) / parts + 127) / 128 * 128;
+  }
   s.parts = (d->n + s.per_cta - 1) / s.per_cta;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   s.v_bytes = up((size_t)(s.one ? s.slices : 1) * d->n_tokens * d->rank * 4);
@@ -547,7 +582,7 @@ static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStr
 
 static int lora_run_one(const LoraParams& p, const LoraShape& s, cudaStream_t st) {
   const int r = p.d.rank;
-  if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, s.slices, (r + 31) / 32), 1, 0, st, p)) return rc;
+  if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, (s.units + kLoraThreads / 32 - 1) / (kLoraThreads / 32)), 1, 0, st, p)) return rc;
   return lora_launch(r <= 8 ? lora_expand_one_kernel<1> : r <= 16 ? lora_expand_one_kernel<2> : r <= 32 ? lora_expand_one_kernel<4>
                      : r <= 64 ? lora_expand_one_kernel<8> : lora_expand_one_kernel<16>, dim3(s.tiles, s.parts), 1, 0, st, p);
 }

@@ -202,7 +202,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
   int *const sums = out + 4, *const heads = sums + W;
   if (n <= 32) {  // one warp, by comparing
     if (warp == 0) {
-      const int e0 = lane < n ? d.topk_idx[lane] : -1, e = (uint32_t)e0 < (uint32_t)E ? e0 : E;  // not here: behind all others
+      const int e0 = lane < n ? __ldcg(d.topk_idx + lane) : -1, e = (uint32_t)e0 < (uint32_t)E ? e0 : E;  // not here: behind all others
       int at = 0;
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
@@ -214,7 +214,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
       const int count = head ? __popc(same) : 0;
       if (lane < n && e < E) {
         r.order[at] = (uint16_t)lane, r.token[at] = (uint16_t)((uint32_t)lane * token_of >> 20);
-        if (r.weight) r.weight[at] = d.topk_w[lane];
+        if (r.weight) r.weight[at] = __ldcg(d.topk_w + lane);
       }
       // heads in the order of their places
       int named = 0, chunks = 0, top = __reduce_max_sync(0xffffffffu, count), cap = 8;
@@ -238,12 +238,12 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
   }
   const int used = min(W, (n + 31) / 32);  // warps that have entries
   const int each = ((n + used - 1) / used + 31) & ~31, lo = min(n, warp * each), hi = min(n, lo + each);
-  const int e_first = lo + lane < hi ? d.topk_idx[lo + lane] : -1;
+  const int e_first = lo + lane < hi ? __ldcg(d.topk_idx + lo + lane) : -1;
   for (int i = threadIdx.x; i < used * E; i += kXpThreads) counts[i] = 0;
   if (threadIdx.x == 0) out[0] = 0;
   __syncthreads();
   for (int i = lo + lane; i < hi; i += 32) {
-    const int e = i == lo + lane ? e_first : d.topk_idx[i];
+    const int e = i == lo + lane ? e_first : __ldcg(d.topk_idx + i);
     if ((uint32_t)e < (uint32_t)E) atomicAdd(&counts[warp * E + e], 1);
   }
   __syncthreads();
@@ -293,14 +293,14 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
   if (threadIdx.x == 0) r.start[named] = all & 0xffff, r.first[named] = (uint16_t)(all >> 16);
   for (int i0 = lo; i0 < hi; i0 += 32) {
     const int i = i0 + lane;
-    const int e = i0 == lo ? e_first : i < hi ? d.topk_idx[i] : -1;
+    const int e = i0 == lo ? e_first : i < hi ? __ldcg(d.topk_idx + i) : -1;
     const bool here = (uint32_t)e < (uint32_t)E;
     const uint32_t same = __match_any_sync(0xffffffffu, here ? e : -1);
     const int before = __popc(same & below);
     if (here) {
       const int at = counts[warp * E + e] + before;
       r.order[at] = (uint16_t)i, r.token[at] = (uint16_t)((uint32_t)i * token_of >> 20);
-      if (r.weight) r.weight[at] = d.topk_w[i];
+      if (r.weight) r.weight[at] = __ldcg(d.topk_w + i);
     }
     __syncwarp();
     if (here && before == 0) counts[warp * E + e] += __popc(same);
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
     asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
   }
   // The up form waits here for whatever wrote the tokens and their experts. The down form was let in by the up form, behind its
-  // wait: what both read is there, and only what the up form writes is waited for (below).
+  // wait: what both read is there, in the L2, and only what the up form writes is waited for (below).
   if (!DOWN) wait_for_launch_before();
   XpTables r;
   r.start = reinterpret_cast<int*>(xp_smem + l.tables);

@@ -137,6 +137,31 @@ def test_captured_beside_other_streams(cuda_device, t):
         assert torch.equal(third, want[2]) and all(torch.equal(outs[s], want[s]) for s in range(2))
 
 
+@pytest.mark.parametrize("t", [3, 300])
+def test_what_a_graph_writes_in_front_of_a_call_is_seen(cuda_device, t):
+    """ids, y and the adapters, written by kernels that run just before the call, replay after replay."""
+    from execution_ucx_b200.ops import lora
+    layer = lora.LoraAdapters(*adapters(6, 512, 264, 16, cuda_device))
+    x, y, ids = bf(t, 512, dev=cuda_device), bf(t, 264, dev=cuda_device), torch.zeros(t, dtype=torch.int32, device=cuda_device)
+    new = [torch.empty_like(v) for v in (x, y, ids, layer.a, layer.b)]
+    layer(x, ids, y)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for old, v in zip((x, y, ids, layer.a, layer.b), new):
+            old.copy_(v)
+        out = layer(x, ids, y)
+        out2 = layer(x, ids, out)
+    for rnd in range(5):
+        for v in new:
+            v.copy_(torch.randint(-1, 6, v.shape, device=cuda_device) if v.dtype == torch.int32 else torch.randn(v.shape, device=cuda_device))
+        g.replay()
+        torch.cuda.synchronize()
+        want, tol = plain(new[0], new[2], new[1], new[3], new[4], layer.scale)
+        assert bool(((out.double() - want).abs() <= tol).all())
+        want, tol = plain(new[0], new[2], out, new[3], new[4], layer.scale)
+        assert bool(((out2.double() - want).abs() <= tol).all())
+
+
 def test_beside_a_shared_projection(cuda_device):
     """The remote GEMM's result for tokens of several requests, and each request's adapter added to it in place."""
     from execution_ucx_b200.ops import lora

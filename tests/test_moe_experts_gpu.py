@@ -264,6 +264,34 @@ def test_weights_written_in_place_hold_for_the_next_call(cuda_device):
     check(layer, x, idx, w)
 
 
+@pytest.mark.parametrize("t", [2, 60])
+def test_what_a_graph_writes_in_front_of_a_call_is_seen(cuda_device, t):
+    """Tokens, choices, weights of choices and of experts, written by kernels that run just before the call, replay after replay."""
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(8, 256, 144, False, cuda_device))
+    x = torch.randn(t, 256, device=cuda_device).to(torch.bfloat16)
+    idx, w = routing(t, 3, 8, cuda_device, 1)
+    old = (x, idx, w, layer.w_gate_up, layer.w_down)
+    new = [v.clone() for v in old]
+    layer(x, idx, w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for a, b in zip(old, new):
+            a.copy_(b)
+        out = layer(x, idx, w)
+    for rnd in range(5):
+        new[0].copy_(torch.randn(t, 256, device=cuda_device))
+        for a, b in zip(new[1:3], routing(t, 3, 8, cuda_device, 20 + rnd, absent=0.2)):
+            a.copy_(b)
+        for b in new[3:]:
+            b.copy_(torch.randn(b.shape, device=cuda_device) * 0.07)
+        g.replay()
+        torch.cuda.synchronize()
+        layer.check_status()
+        want, tol = plain(*new)
+        assert bool(((out.double() - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("fp8_rows", [False])
 def test_route_dispatch_experts_combine(cuda_device, fp8_rows):
     """The parts as they are used across GPUs, with logical ranks on one: the router's choice, the rows sent to the experts'
