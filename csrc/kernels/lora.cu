@@ -14,9 +14,9 @@
 //   lora_shrink: a cluster of CTAs has a tile, each a part of K; x and A go through a ring of stages with cp.async, four warps have
 //   16 rows each. The parts are added up through the cluster's shared memory, in order: v is written once, nothing is added with
 //   atomics.
-//   lora_expand: a warp has 16 tokens and runs over a part of N, 32 columns at a time. v is its first operand, two bfloat16 numbers that
-//   add up to it (what is lost is 2^-16 of it, nothing beside the result's rounding), made in registers; B comes from L1 and L2
-//   straight into registers. The next columns' y and B are fetched before the product of these.
+//   lora_expand: a warp has 16 tokens and runs over a part of N. v is its first operand, two bfloat16 numbers that add up to it (what is
+//   lost is 2^-16 of it, nothing beside the result's rounding), made in registers. y and B go through a ring of stages with cp.async: B
+//   for all four warps, of y a lane fetches what it will need itself.
 #include <algorithm>
 
 #include "eux_device.cuh"
@@ -27,6 +27,7 @@ constexpr int kLoraPlain = 64;        // tokens up to which each is a tile of it
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
 constexpr int kLoraStages = 4;
+constexpr int kLoraColumns = 64;      // of N in a stage of expand
 constexpr int kLoraMaxSlices = 32;    // parts of K of a token
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
@@ -403,10 +404,18 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   lora_cluster_meets();  // the others have read this one's
 }
 
-// K32: ranks in 32s. A lane's eight values of K are side by side (the order of K is the product's own affair), and so are its eight
-// columns of 32 (column 2c + i of the product's n-th eight is 8c + 2n + i of the 32).
-template <int K32>
+// K16: ranks in 16s, rounded up to a power of two. Columns go 64 at a time, in two runs of 32. A lane's eight columns of a run lie side
+// by side, so that y and out are moved 16 bytes at a time: column 2c + i of the product's j-th eight is column 8c + 2j + i of the run,
+// and the rows of B lie in shared memory in the product's order.
+template <int K16>
+struct LoraExpand {
+  static constexpr int PITCH = K16 * 32 + 16;  // bytes between rows of B: eight rows on different banks
+  static constexpr int B = kLoraColumns * PITCH, Y = 4 * kLoraThreads * 16, STAGE = B + Y;
+};
+template <int K16>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
+  using S = LoraExpand<K16>;
+  extern __shared__ __align__(1024) unsigned char lora_smem_raw[];
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   // Shrink was through with its wait for whatever is in front when it let this in: all but v is there, in the L2.
@@ -417,97 +426,104 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     return;
   }
   const bool has = t.adapter < d.n_adapters;
-  const int row0 = warp * 16, n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta);
-  if (row0 < t.n) {
-    // this lane's rows: g and g + 8 of the warp's
-    const __nv_bfloat16* y_row[2];
-    __nv_bfloat16* out_row[2];
-    bool row[2];
+  const int row0 = warp * 16, n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta), steps = (n1 - n0 + kLoraColumns - 1) / kLoraColumns;
+  // this lane's rows: g and g + 8 of the warp's
+  const __nv_bfloat16* y_row[2];
+  __nv_bfloat16* out_row[2];
+  bool row[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = row0 + g + 8 * h;
-      row[h] = r < t.n;
-      const int64_t token = row[h] ? __ldcg(p.order + t.first + r) : 0;
-      y_row[h] = (const __nv_bfloat16*)d.y + token * d.y_stride, out_row[h] = (__nv_bfloat16*)d.out + token * d.out_stride;
-    }
-    const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? t.adapter : 0) * d.n * d.rank;
-    constexpr bool AHEAD = K32 <= 2;  // B of the next columns: there are registers for it
-    uint4 y[2], next_y[2], w[4][K32];
-    auto fetch_y = [&](uint4 (&to)[2], int n) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (row[h] && n + c * 8 < n1) to[h] = ld_cg_u4(y_row[h] + n + c * 8);  // L1 is for B
-    };
-    auto fetch_w = [&](int n) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = n + (g >> 1) * 8 + j * 2 + (g & 1);  // the row of B for this lane's column
-#pragma unroll
-        for (int k = 0; k < K32; ++k)
-          w[j][k] = has && at < n1 && k * 32 + c * 8 < d.rank ? __ldg(reinterpret_cast<const uint4*>(b + (int64_t)at * d.rank + k * 32 + c * 8)) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    fetch_y(next_y, n0);
-    uint32_t hi[K32][2][4], lo[K32][2][4];  // first operands of 16 of K
-    wait_for_launch_before();
-    if (AHEAD) fetch_w(n0);
-    if (has) {
-      const float scale = d.scale[t.adapter];
-#pragma unroll
-      for (int k = 0; k < K32; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float4 q0 = make_float4(0.f, 0.f, 0.f, 0.f), q1 = q0;
-          if (row[h] && k * 32 + c * 8 < d.rank) {
-            const float* const at = p.v + (int64_t)(t.first + row0 + g + 8 * h) * d.rank + k * 32 + c * 8;
-            q0 = __ldcg(reinterpret_cast<const float4*>(at)), q1 = __ldcg(reinterpret_cast<const float4*>(at) + 1);
-          }
-          const float v[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float v0 = v[2 * q] * scale, v1 = v[2 * q + 1] * scale;
-            const __nv_bfloat162 u = __floats2bfloat162_rn(v0, v1);
-            const float2 f = __bfloat1622float2(u);
-            // nothing is lost of an infinity
-            const __nv_bfloat162 l = __floats2bfloat162_rn(isinf(f.x) ? 0.f : v0 - f.x, isinf(f.y) ? 0.f : v1 - f.y);
-            // pairs 0 and 1 are the first 16's k = 2c and 2c + 8, pairs 2 and 3 the second's
-            hi[k][q >> 1][(q & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&u);
-            lo[k][q >> 1][(q & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&l);
-          }
-        }
-    }
-    for (int n = n0; n < n1; n += 32) {
-      y[0] = next_y[0], y[1] = next_y[1];
-      fetch_y(next_y, n + 32);
-      if (!AHEAD) fetch_w(n);
-      float acc[4][4] = {};
+  for (int h = 0; h < 2; ++h) {
+    const int r = row0 + g + 8 * h;
+    row[h] = r < t.n;
+    const int64_t token = row[h] ? __ldcg(p.order + t.first + r) : 0;
+    y_row[h] = (const __nv_bfloat16*)d.y + token * d.y_stride, out_row[h] = (__nv_bfloat16*)d.out + token * d.out_stride;
+  }
+  const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + (int64_t)(has ? t.adapter : 0) * d.n * d.rank;
+  const uint32_t smem = lora_smem(lora_smem_raw);
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      const uint32_t at = smem + step % kLoraStages * S::STAGE;
+      const int n = n0 + step * kLoraColumns;
       if (has) {
+        constexpr int PIECES = K16 * 2;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < K32; ++k) {
-            const uint4 b4 = w[j][k];
-            lora_mma(acc[j], hi[k][0], b4.x, b4.y), lora_mma(acc[j], hi[k][1], b4.z, b4.w);
-            lora_mma(acc[j], lo[k][0], b4.x, b4.y), lora_mma(acc[j], lo[k][1], b4.z, b4.w);
-          }
-        if (AHEAD) fetch_w(n + 32);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (row[h] && n + c * 8 < n1) {
-          if (has) {
-            __nv_bfloat162* const y2 = reinterpret_cast<__nv_bfloat162*>(&y[h]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = __bfloat1622float2(y2[j]);
-              y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
-            }
-          }
-          st_stream_u4(out_row[h] + n + c * 8, y[h]);
+        for (int i = threadIdx.x; i < kLoraColumns * PIECES; i += kLoraThreads) {
+          const int place = i / PIECES, piece = i % PIECES, in = place & 7, eight = place >> 3 & 3;
+          const int col = n + (place & 32) + (in >> 1) * 8 + eight * 2 + (in & 1);
+          const bool some = col < n1 && piece * 8 < d.rank;
+          lora_cp_16(at + place * S::PITCH + piece * 16, some ? b + (int64_t)col * d.rank + piece * 8 : b, some);
         }
+      }
+      // y: what this lane needs itself
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int h = q & 1, col = n + (q >> 1) * 32 + c * 8;
+        if (row[h] && col < n1) lora_cp_16(at + S::B + (q * kLoraThreads + threadIdx.x) * 16, y_row[h] + col, true);
+      }
+    }
+    lora_cp_commit();
+  };
+  for (int i = 0; i < kLoraStages - 1; ++i) fetch(i);
+  uint32_t hi[K16][4], lo[K16][4];  // first operands
+  const float scale = has ? __ldcg(d.scale + t.adapter) : 0.f;
+  wait_for_launch_before();
+#pragma unroll
+  for (int k = 0; k < K16; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // row g + 8 (q & 1), columns 2c + 8 (q >> 1) and the next
+      const int at = k * 16 + 2 * c + 8 * (q >> 1);
+      float2 v = make_float2(0.f, 0.f);
+      if (has && row[q & 1] && at < d.rank) v = __ldcg(reinterpret_cast<const float2*>(p.v + (int64_t)(t.first + row0 + g + 8 * (q & 1)) * d.rank + at));
+      v.x *= scale, v.y *= scale;
+      const __nv_bfloat162 u = __floats2bfloat162_rn(v.x, v.y);
+      const float2 f = __bfloat1622float2(u);
+      // nothing is lost of an infinity
+      const __nv_bfloat162 l = __floats2bfloat162_rn(isinf(f.x) ? 0.f : v.x - f.x, isinf(f.y) ? 0.f : v.y - f.y);
+      hi[k][q] = *reinterpret_cast<const uint32_t*>(&u), lo[k][q] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+  for (int s = 0; s < steps; ++s) {
+    lora_cp_wait<kLoraStages - 2>();
+    __syncthreads();
+    fetch(s + kLoraStages - 1);
+    const uint32_t at = smem + s % kLoraStages * S::STAGE;
+    if (row0 < t.n) {
+#pragma unroll
+      for (int run = 0; run < 2; ++run) {
+        float acc[4][4] = {};
+        if (has) {
+#pragma unroll
+          for (int k = 0; k < K16; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+              uint32_t w[4];
+              lora_ldsm_x4(w, at + (run * 32 + j * 8 + (lane & 7) + ((lane >> 4) << 3)) * S::PITCH + k * 32 + ((lane >> 3) & 1) * 16);
+              lora_mma(acc[j], hi[k], w[0], w[1]), lora_mma(acc[j + 1], hi[k], w[2], w[3]);
+              lora_mma(acc[j], lo[k], w[0], w[1]), lora_mma(acc[j + 1], lo[k], w[2], w[3]);
+            }
+        }
+        const int col = n0 + s * kLoraColumns + run * 32 + c * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (row[h] && col < n1) {
+            uint4 y;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(at + S::B + ((run * 2 + h) * kLoraThreads + threadIdx.x) * 16)
+                         : "memory");
+            if (has) {
+              __nv_bfloat162* const y2 = reinterpret_cast<__nv_bfloat162*>(&y);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 f = __bfloat1622float2(y2[j]);
+                y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
+              }
+            }
+            st_u4(out_row[h] + col, y);
+          }
+      }
     }
   }
-  wait_for_launch_before();
+  lora_cp_wait<0>();
   allow_next_launch();
 }
 
@@ -548,7 +564,7 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     while (want & (want - 1)) want &= want - 1;  // a cluster
     s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
     s.slices = want;
-    const int parts = std::max(1, std::min(4 * kSms / likely, (d->n + 127) / 128));
+    const int parts = std::max(1, std::min(12 * kSms / likely, (d->n + 127) / 128));
     s.per_cta = ((d->n + parts - 1) / parts + 127) / 128 * 128;
   }
   s.parts = (d->n + s.per_cta - 1) / s.per_cta;
@@ -580,6 +596,14 @@ static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStr
   return lora_launch(lora_shrink_kernel<R8>, dim3(s.tiles, s.slices), s.slices, smem, st, p);
 }
 
+template <int K16>
+static int lora_expand(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
+  constexpr size_t smem = (size_t)kLoraStages * LoraExpand<K16>::STAGE;
+  if (smem > 48 * 1024)
+    if (cudaError_t e = allow_smem<lora_expand_kernel<K16>>(dev, smem); e != cudaSuccess) return (int)e;
+  return lora_launch(lora_expand_kernel<K16>, dim3(s.tiles, s.parts), 1, smem, st, p);
+}
+
 static int lora_run_one(const LoraParams& p, const LoraShape& s, cudaStream_t st) {
   const int r = p.d.rank;
   if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, (s.units + kLoraThreads / 32 - 1) / (kLoraThreads / 32)), 1, 0, st, p)) return rc;
@@ -591,7 +615,7 @@ static int lora_run_tiles(const LoraParams& p, const LoraShape& s, int dev, cuda
   const int rc = r <= 8 ? lora_shrink<1>(p, s, dev, st) : r <= 16 ? lora_shrink<2>(p, s, dev, st) : r <= 32 ? lora_shrink<4>(p, s, dev, st)
                  : r <= 64 ? lora_shrink<8>(p, s, dev, st) : lora_shrink<16>(p, s, dev, st);
   if (rc) return rc;
-  return lora_launch(r <= 32 ? lora_expand_kernel<1> : r <= 64 ? lora_expand_kernel<2> : lora_expand_kernel<4>, dim3(s.tiles, s.parts), 1, 0, st, p);
+  return r <= 16 ? lora_expand<1>(p, s, dev, st) : r <= 32 ? lora_expand<2>(p, s, dev, st) : r <= 64 ? lora_expand<4>(p, s, dev, st) : lora_expand<8>(p, s, dev, st);
 }
 
 }  // namespace eux
@@ -635,7 +659,7 @@ extern "C" int eux_lora_preload(void) {
                            (const void*)lora_expand_one_kernel<4>, (const void*)lora_expand_one_kernel<8>, (const void*)lora_expand_one_kernel<16>,
                            (const void*)lora_order_kernel, (const void*)lora_shrink_kernel<1>, (const void*)lora_shrink_kernel<2>,
                            (const void*)lora_shrink_kernel<4>, (const void*)lora_shrink_kernel<8>, (const void*)lora_shrink_kernel<16>,
-                           (const void*)lora_expand_kernel<1>, (const void*)lora_expand_kernel<2>, (const void*)lora_expand_kernel<4>};
+                           (const void*)lora_expand_kernel<1>, (const void*)lora_expand_kernel<2>, (const void*)lora_expand_kernel<4>, (const void*)lora_expand_kernel<8>};
   for (const void* k : kernels)
     if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;
   return 0;
