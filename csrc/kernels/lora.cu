@@ -6,7 +6,7 @@
 // ranks up to 128 still less than the tensor cores do in that time; with few tokens the adapters that are named, and latency.
 // Two kernels, `shrink` (x to v) and `expand` (v to out), and for many tokens one in front:
 //
-// * Up to kLoraPlain tokens each stands for itself: nothing is sorted, and requests that share an adapter read it again from the L2.
+// * Few tokens each stand for themselves: nothing is sorted, and requests that share an adapter read it again from the L2.
 //   lora_shrink_one: a warp has some rows of A and a part of K, both straight into registers; parts of K are added up by expand.
 //   lora_expand_one: a row of B is read by as many lanes as it has 16-byte pieces; a lane group makes eight columns side by side.
 //   All in float32, no shared memory in the way: the chain id, A, v, B is four round trips to memory, and that is the time.
@@ -18,15 +18,16 @@
 //   lost is 2^-16 of it, nothing beside the result's rounding), made in registers. y and B go through a ring of stages with cp.async: B
 //   for all four warps, of y a lane fetches what it will need itself.
 #include <algorithm>
+#include <mutex>
 
 #include "eux_device.cuh"
 
 namespace eux {
 
-constexpr int kLoraPlain = 64;        // tokens up to which each is a tile of its own
+constexpr int kLoraPlain = 512;       // tokens up to which each may stand for itself ...
+constexpr int64_t kLoraPlainBytes = int64_t(64) << 20;  // ... if the adapters that they read then come to no more than this
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
-constexpr int kLoraStages = 4;
 constexpr int kLoraColumns = 64;      // of N in a stage of expand
 constexpr int kLoraMaxSlices = 32;    // parts of K of a token
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
@@ -62,7 +63,6 @@ __device__ __forceinline__ void lora_mma(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 constexpr int kOrderThreads = 1024;
-constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr size_t kOrderSmem = 200 * 1024;  // for the counts, where they fit
 
 __device__ __forceinline__ int lora_adapter(const eux_lora_desc& d, int64_t token) {  // n_adapters: none
@@ -202,83 +202,73 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __g
 
 // ---- tiles of tokens that share an adapter ----
 
-// Tokens ordered by adapter, those without one behind all (as adapter n_adapters: expand copies their rows), and the tiles. One CTA,
-// whose warps each count a run of tokens per adapter, `counts` [warps][n_adapters + 1]: null if they lie in shared memory.
+// Tokens ordered by adapter, those without one behind all (as adapter n_adapters: expand copies their rows), and the tiles, by one CTA.
+// `counts` [n_adapters + 1]: null if they lie in shared memory. The order of an adapter's tokens is left to chance: a token's result
+// does not depend on its place.
 __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_constant__ LoraParams p, int* counts) {
   extern __shared__ int order_smem[];
-  __shared__ int sums[kOrderWarps], tile_sums[kOrderWarps];
+  __shared__ int sums[kOrderThreads / 32], tile_sums[kOrderThreads / 32];
   if (!counts) counts = order_smem;
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, A = d.n_adapters + 1;
-  const int used = min(kOrderWarps, (d.n_tokens + 31) / 32);
-  const int each = ((d.n_tokens + used - 1) / used + 31) & ~31, lo = min(d.n_tokens, warp * each), hi = min(d.n_tokens, lo + each);
-  const uint32_t below = (1u << lane) - 1u;
-  int* const mine = counts + (int64_t)warp * A;
-  for (int64_t i = threadIdx.x; i < (int64_t)A * used; i += kOrderThreads) counts[i] = 0;
+  for (int i = threadIdx.x; i < A; i += kOrderThreads) counts[i] = 0;
   wait_for_launch_before();
   constexpr int KEPT = 8;  // a thread's first adapters, fetched at once
   int kept[KEPT];
 #pragma unroll
-  for (int q = 0; q < KEPT; ++q) kept[q] = lo + q * 32 + lane < hi ? lora_adapter(d, lo + q * 32 + lane) : -1;
-  auto adapter_of = [&](int i0) {
-    int a = -1;
-    if (i0 - lo >= KEPT * 32) return i0 + lane < hi ? lora_adapter(d, i0 + lane) : -1;
+  for (int q = 0; q < KEPT; ++q) {
+    const int i = q * kOrderThreads + threadIdx.x;
+    kept[q] = i < d.n_tokens ? lora_adapter(d, i) : -1;
+  }
+  __syncthreads();
+  // A warp's neighbours with the same adapter count, and are placed, as one: prompts are runs of one adapter.
+  auto add = [&](int a, bool place, int token) {
+    const int before = __shfl_up_sync(0xffffffffu, a, 1);
+    const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || a != before);
+    const int head = 31 - __clz(heads & (0xffffffffu >> (31 - lane)));
+    const uint32_t behind = heads & ~(0xffffffffu >> (31 - lane));
+    int at = 0;
+    if (head == lane && a >= 0) at = atomicAdd(counts + a, (behind ? __ffs(behind) - 1 : 32) - lane);
+    if (place) {
+      at = __shfl_sync(0xffffffffu, at, head) + lane - head;
+      if (a >= 0) p.order[at] = token;
+    }
+  };
+  auto over_tokens = [&](bool place) {
 #pragma unroll
     for (int q = 0; q < KEPT; ++q)
-      if (i0 == lo + q * 32) a = kept[q];
-    return a;
+      if (q * kOrderThreads < d.n_tokens) add(kept[q], place, q * kOrderThreads + threadIdx.x);
+    for (int i0 = KEPT * kOrderThreads; i0 < d.n_tokens; i0 += kOrderThreads) {
+      const int i = i0 + threadIdx.x;
+      add(i < d.n_tokens ? lora_adapter(d, i) : -1, place, i);
+    }
   };
-  __syncthreads();
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int a = adapter_of(i0);
-    const uint32_t same = __match_any_sync(0xffffffffu, a);
-    if (a >= 0 && (same & below) == 0) mine[a] += __popc(same);
-    __syncwarp();
-  }
+  over_tokens(false);
   __syncthreads();
   int all = 0, tiles = 0;
   for (int a0 = 0; a0 < A; a0 += kOrderThreads) {
-    const int a = a0 + threadIdx.x;
-    int c = 0;
-    if (a < A)
-      for (int w = 0; w < used; ++w) c += counts[(int64_t)w * A + a];
-    const int t = (c + kLoraTile - 1) / kLoraTile;
+    const int a = a0 + threadIdx.x, c = a < A ? counts[a] : 0, t = (c + kLoraTile - 1) / kLoraTile;
     int sum = c, tsum = t;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, sum, o), v = __shfl_up_sync(0xffffffffu, tsum, o);
       if (lane >= o) sum += u, tsum += v;
     }
     if (lane == 31) sums[warp] = sum, tile_sums[warp] = tsum;
     __syncthreads();
-    int at = all, tile = tiles;
-    {  // over the warps, by each warp
-      int u = sums[lane], v = tile_sums[lane];
-      const int before_u = __reduce_add_sync(0xffffffffu, lane < warp ? u : 0), before_v = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
-      u = __reduce_add_sync(0xffffffffu, u), v = __reduce_add_sync(0xffffffffu, v);
-      at += before_u, tile += before_v, all += u, tiles += v;
-    }
-    at += sum - c, tile += tsum - t;
+    const int u = sums[lane], v = tile_sums[lane];  // as many warps as lanes
+    const int at = all + __reduce_add_sync(0xffffffffu, lane < warp ? u : 0) + sum - c;
+    const int tile = tiles + __reduce_add_sync(0xffffffffu, lane < warp ? v : 0) + tsum - t;
+    all += __reduce_add_sync(0xffffffffu, u), tiles += __reduce_add_sync(0xffffffffu, v);
     if (c) {
       const int n = (c + t - 1) / t;  // tiles of equal size
       for (int i = 0; i < t; ++i) p.tiles[tile + i] = make_int4(a, at + i * n, min(n, c - i * n), 0);
-      for (int w = 0; w < used; ++w) {  // from counts to places
-        const int m = counts[(int64_t)w * A + a];
-        counts[(int64_t)w * A + a] = at;
-        at += m;
-      }
+      counts[a] = at;  // from counts to places
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) *p.n_tiles = tiles;
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane, a = adapter_of(i0);
-    const uint32_t same = __match_any_sync(0xffffffffu, a);
-    const int before = __popc(same & below);
-    if (a >= 0) p.order[mine[a] + before] = i;
-    __syncwarp();
-    if (a >= 0 && before == 0) mine[a] += __popc(same);
-    __syncwarp();
-  }
+  over_tokens(true);
   allow_next_launch();
 }
 
@@ -305,9 +295,14 @@ __device__ __forceinline__ float4 lora_ld_cluster(uint32_t at, uint32_t cta) {
 
 // R8: ranks in eights, rounded up to a power of two.
 template <int R8>
+struct LoraShrink {
+  static constexpr int STAGE = (kLoraTile + R8 * 8) * 128, STAGES = R8 >= 8 ? 3 : 4;
+  static constexpr int RING = STAGES * STAGE, SUM = kLoraTile * (R8 * 8 + 4) * 4, BYTES = RING > SUM ? RING : SUM;
+};
+template <int R8>
 __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
   constexpr int STEP = 64, PIECES = STEP / 8;  // of K in a stage; 16-byte pieces of a row
-  constexpr int X = kLoraTile * STEP * 2, STAGE = X + R8 * 8 * STEP * 2;
+  constexpr int X = kLoraTile * STEP * 2, STAGE = LoraShrink<R8>::STAGE, STAGES = LoraShrink<R8>::STAGES;
   constexpr int LD = R8 * 8 + 4;               // floats between the tile's rows when it is added up
   extern __shared__ __align__(1024) unsigned char lora_smem_raw[];
   const eux_lora_desc& d = p.d;
@@ -337,7 +332,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   }
   auto fetch = [&](int step) {
     if (step < steps) {
-      const uint32_t at = smem + step % kLoraStages * STAGE;
+      const uint32_t at = smem + step % STAGES * STAGE;
       const int k = k0 + step * STEP + piece * 8;
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
@@ -352,14 +347,16 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     }
     lora_cp_commit();
   };
-  for (int s = 0; s < kLoraStages - 1; ++s) fetch(s);
-  allow_next_launch();
+  for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+  // Expand's CTAs fetch their first y and B beside this (2048 tokens, 4096 x 4096, rank 64: 29.0 us, 30.8 without); with ranks above 64 the
+  // few that find room beside these hold it unevenly until the end (8192 tokens, rank 128: 139 us, 115 without).
+  if (R8 < 16) allow_next_launch();
   float acc[R8][4] = {};
   for (int s = 0; s < steps; ++s) {
-    lora_cp_wait<kLoraStages - 2>();
+    lora_cp_wait<STAGES - 2>();
     __syncthreads();
-    fetch(s + kLoraStages - 1);
-    const uint32_t xs = smem + s % kLoraStages * STAGE, w = xs + X;
+    fetch(s + STAGES - 1);
+    const uint32_t xs = smem + s % STAGES * STAGE, w = xs + X;
     if (warp * 16 < t.n) {
 #pragma unroll
       for (int ks = 0; ks < STEP / 16; ++ks) {
@@ -402,6 +399,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
     *reinterpret_cast<float4*>(p.v + (int64_t)(t.first + r) * d.rank + e) = v;
   }
   lora_cluster_meets();  // the others have read this one's
+  if (R8 >= 16) allow_next_launch();
 }
 
 // K16: ranks in 16s, rounded up to a power of two. Columns go 64 at a time, in two runs of 32. A lane's eight columns of a run lie side
@@ -410,7 +408,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
 template <int K16>
 struct LoraExpand {
   static constexpr int PITCH = K16 * 32 + 16;  // bytes between rows of B: eight rows on different banks
-  static constexpr int B = kLoraColumns * PITCH, Y = 4 * kLoraThreads * 16, STAGE = B + Y;
+  static constexpr int B = kLoraColumns * PITCH, Y = 4 * kLoraThreads * 16, STAGE = B + Y, STAGES = K16 >= 4 ? 3 : 4, BYTES = STAGES * STAGE;
 };
 template <int K16>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
   const uint32_t smem = lora_smem(lora_smem_raw);
   auto fetch = [&](int step) {
     if (step < steps) {
-      const uint32_t at = smem + step % kLoraStages * S::STAGE;
+      const uint32_t at = smem + step % S::STAGES * S::STAGE;
       const int n = n0 + step * kLoraColumns;
       if (has) {
         constexpr int PIECES = K16 * 2;
@@ -463,7 +461,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     }
     lora_cp_commit();
   };
-  for (int i = 0; i < kLoraStages - 1; ++i) fetch(i);
+  for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
   uint32_t hi[K16][4], lo[K16][4];  // first operands
   const float scale = has ? __ldcg(d.scale + t.adapter) : 0.f;
   wait_for_launch_before();
@@ -482,10 +480,10 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
       hi[k][q] = *reinterpret_cast<const uint32_t*>(&u), lo[k][q] = *reinterpret_cast<const uint32_t*>(&l);
     }
   for (int s = 0; s < steps; ++s) {
-    lora_cp_wait<kLoraStages - 2>();
+    lora_cp_wait<S::STAGES - 2>();
     __syncthreads();
-    fetch(s + kLoraStages - 1);
-    const uint32_t at = smem + s % kLoraStages * S::STAGE;
+    fetch(s + S::STAGES - 1);
+    const uint32_t at = smem + s % S::STAGES * S::STAGE;
     if (row0 < t.n) {
 #pragma unroll
       for (int run = 0; run < 2; ++run) {
@@ -546,7 +544,9 @@ static int lora_width(int rank) { return rank <= 8 ? 1024 : rank <= 16 ? 512 : r
 static LoraShape lora_shape(const eux_lora_desc* d) {
   LoraShape s;
   constexpr int kSms = 148;
-  s.one = d->n_tokens <= kLoraPlain;
+  // Each token for itself, or tiles of those that share an adapter (8192 x 8192, rank 16, an adapter each: 65 tokens, 34 MB, 13.5 and 22.4
+  // us; 256 tokens, 134 MB, 26.9 and 29.0, and where they share adapters tiles read fewer).
+  s.one = d->n_tokens <= kLoraPlain && (int64_t)d->n_tokens * d->rank * ((int64_t)d->k + d->n) * 2 <= kLoraPlainBytes;
   s.tiles = s.one ? d->n_tokens : (int)std::min<int64_t>(d->n_tokens, d->n_tokens / kLoraTile + (int64_t)d->n_adapters + 1);
   if (s.one) {
     // As many warps as the SMs have places for about, each with 256 of K or a multiple; expand once over its columns, likewise.
@@ -558,13 +558,17 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     const int width = lora_width(d->rank), passes = (int)std::max<int64_t>(1, (int64_t)d->n_tokens * ((d->n + width - 1) / width) / (16 * kSms));
     s.per_cta = width * passes;
   } else {
-    // Parts of K and of N for about four CTAs per SM
-    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile;
-    int want = std::max(1, std::min({kLoraCluster, 4 * kSms / likely, (d->k + 255) / 256}));
+    // Parts of K and of N that the SMs have places for at once: a second wave that is half empty costs as much as a full one.
+    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile, r = d->rank;
+    auto places = [](int smem) { return kSms * (227 * 1024 / (smem + 1024)); };
+    const int shrink = places(r <= 8 ? LoraShrink<1>::BYTES : r <= 16 ? LoraShrink<2>::BYTES : r <= 32 ? LoraShrink<4>::BYTES
+                              : r <= 64 ? LoraShrink<8>::BYTES : LoraShrink<16>::BYTES);
+    const int expand = places(r <= 16 ? LoraExpand<1>::BYTES : r <= 32 ? LoraExpand<2>::BYTES : r <= 64 ? LoraExpand<4>::BYTES : LoraExpand<8>::BYTES);
+    int want = std::max(1, std::min({kLoraCluster, shrink / likely, (d->k + 255) / 256}));
     while (want & (want - 1)) want &= want - 1;  // a cluster
     s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
     s.slices = want;
-    const int parts = std::max(1, std::min(12 * kSms / likely, (d->n + 127) / 128));
+    const int parts = std::max(1, std::min(expand / likely, (d->n + 127) / 128));
     s.per_cta = ((d->n + parts - 1) / parts + 127) / 128 * 128;
   }
   s.parts = (d->n + s.per_cta - 1) / s.per_cta;
@@ -572,7 +576,7 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
   s.v_bytes = up((size_t)(s.one ? s.slices : 1) * d->n_tokens * d->rank * 4);
   s.tile_bytes = s.one ? 0 : up(((size_t)s.tiles + 1) * 16);
   s.order_bytes = s.one ? 0 : up((size_t)d->n_tokens * 4);
-  s.count_bytes = s.one ? 0 : up(((size_t)d->n_adapters + 1) * kOrderWarps * 4);
+  s.count_bytes = s.one ? 0 : up(((size_t)d->n_adapters + 1) * 4);
   return s;
 }
 
@@ -590,7 +594,7 @@ static int lora_launch(void (*kernel)(LoraParams), dim3 grid, int cluster, size_
 }
 template <int R8>
 static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
-  constexpr size_t smem = std::max<size_t>(kLoraStages * (kLoraTile + R8 * 8) * 128, (size_t)kLoraTile * (R8 * 8 + 4) * 4);
+  constexpr size_t smem = LoraShrink<R8>::BYTES;
   if (smem > 48 * 1024)
     if (cudaError_t e = allow_smem<lora_shrink_kernel<R8>>(dev, smem); e != cudaSuccess) return (int)e;
   return lora_launch(lora_shrink_kernel<R8>, dim3(s.tiles, s.slices), s.slices, smem, st, p);
@@ -598,7 +602,7 @@ static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStr
 
 template <int K16>
 static int lora_expand(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
-  constexpr size_t smem = (size_t)kLoraStages * LoraExpand<K16>::STAGE;
+  constexpr size_t smem = LoraExpand<K16>::BYTES;
   if (smem > 48 * 1024)
     if (cudaError_t e = allow_smem<lora_expand_kernel<K16>>(dev, smem); e != cudaSuccess) return (int)e;
   return lora_launch(lora_expand_kernel<K16>, dim3(s.tiles, s.parts), 1, smem, st, p);
@@ -635,6 +639,9 @@ extern "C" int eux_lora_launch(const eux_lora_desc* d, void* stream) {
   if (!d->x || !d->ids || !d->y || !d->out || !d->a || !d->b || !d->scale || !d->workspace) return EUX_ERR_BAD_ARG;
   if (((uintptr_t)d->x | (uintptr_t)d->y | (uintptr_t)d->out | (uintptr_t)d->a | (uintptr_t)d->b | (uintptr_t)d->workspace) & 15) return EUX_ERR_BAD_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
+  // Threads that share a stream share a workspace: their launches must not mix.
+  static std::mutex launching;
+  std::lock_guard<std::mutex> lock(launching);
   const LoraShape s = lora_shape(d);
   char* at = (char*)d->workspace;
   LoraParams p = {};
@@ -646,7 +653,7 @@ extern "C" int eux_lora_launch(const eux_lora_desc* d, void* stream) {
   if (s.one) return lora_run_one(p, s, st);
   p.n_tiles = (int*)at, p.tiles = (int4*)at + 1, at += s.tile_bytes;
   p.order = (int*)at, at += s.order_bytes;
-  const size_t count_bytes = ((size_t)d->n_adapters + 1) * kOrderWarps * 4;
+  const size_t count_bytes = ((size_t)d->n_adapters + 1) * 4;
   const bool in_smem = count_bytes <= kOrderSmem;
   if (cudaError_t e = allow_smem<lora_order_kernel>(dev, kOrderSmem); e != cudaSuccess) return (int)e;
   if (int rc = launch_early(lora_order_kernel, 1, kOrderThreads, in_smem ? count_bytes : 0, st, p, in_smem ? (int*)nullptr : (int*)at)) return rc;

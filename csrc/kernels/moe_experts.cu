@@ -28,6 +28,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "eux_bulk.cuh"
 #include "eux_device.cuh"
@@ -846,6 +847,9 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   if (d->fp8 && (!d->gate_up_scale || !d->down_scale)) return EUX_ERR_BAD_ARG;
   if (((uintptr_t)d->x | (uintptr_t)d->out | (uintptr_t)d->w_gate_up | (uintptr_t)d->w_down | (uintptr_t)d->workspace) & 15 || (uintptr_t)d->maps & 63) return EUX_ERR_BAD_ARG;
   const cudaStream_t st = (cudaStream_t)stream;
+  // Threads that share a stream share a workspace: their launches must not mix.
+  static std::mutex launching;
+  std::lock_guard<std::mutex> lock(launching);
   const CUtensorMap *up = (const CUtensorMap*)d->maps, *down = up + 1;
   XpParams p = {};
   p.d = *d;

@@ -55,13 +55,22 @@ class on_device:
 
     def __enter__(self) -> int:
         self.before = torch.cuda.current_device()
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
+        torch.cuda.set_device(self.index)
         return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
+        torch.cuda.set_device(self.before)
+
+
+def launch(function, desc, index: int, what: str) -> None:
+    """One call of a launch function on device ``index`` and its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        rc = function(desc, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with on_device(index) as stream:
+            rc = function(desc, stream)
+    if rc:
+        _native.check(rc, what)
 
 
 class CallScratch:
@@ -74,33 +83,39 @@ class CallScratch:
     def __init__(self, words: int, device):
         self.words, self.device = words, device
         self._of_stream = {}
-        self._kept = []
+        self._captured, self._kept = [], []
         with on_device(device.index):
             self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0)) if words else []
             torch.cuda.current_stream().synchronize()  # captured calls run on any stream
 
-    def get(self, stream: int, need: int):
-        """The addresses of ``need`` bytes and of the words, for a call on ``stream``, the current one."""
-        if torch.cuda.is_current_stream_capturing():
+    def get(self, need: int):
+        """The addresses of ``need`` bytes and of the words, for a call on the device's current stream, whether or not the device
+        is the current one."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            with on_device(self.device.index):
+                return self.get(need)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if torch._C._cuda_isCurrentStreamCapturing():
             # In a capture a tensor's memory is the graph's; the words are zeroed by the graph itself once those that were
             # zeroed beforehand are given out.
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
             words = self._spare.pop() if self._spare else torch.zeros(self.words, dtype=torch.int32, device=self.device)
-            self._kept.append(words)
+            self._captured.append(words)
             return workspace.data_ptr(), words.data_ptr()
         mine = self._of_stream.get(stream)
         if mine is None or mine[2] < need:
+            # A smaller workspace may be another thread's, which has yet to launch with it: it is kept. Powers of two: all that are kept come
+            # to less than the largest.
+            need = 1 << (need - 1).bit_length()
             words = mine[1] if mine else torch.zeros(self.words, dtype=torch.int32, device=self.device)
+            if mine:
+                self._kept.append(mine[0])
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
             mine = self._of_stream[stream] = (workspace, words, need, (workspace.data_ptr(), words.data_ptr()))
         return mine[3]
 
     def reset(self) -> None:
         """Zeroes all words, after a kernel that gave up: with nothing in flight."""
-        for t in [m[1] for m in self._of_stream.values()] + self._kept:
+        for t in [m[1] for m in self._of_stream.values()] + self._captured:
             t.zero_()
 
-
-def check(rc: int, what: str) -> None:
-    if rc:
-        _native.check(rc, what)

@@ -69,7 +69,7 @@ class LoraAdapters:
             self._require(x, ids, y)
         t = ids.shape[0]
         if out is None:
-            out = torch.empty(t, self.N, dtype=torch.bfloat16, device=self.device)
+            out = torch.empty_strided((t, self.N), (self.N, 1), dtype=torch.bfloat16, device=self.device)
         else:
             ws.require_rows(out, "out", torch.bfloat16, cols=self.N, rows=t)
             ws.require_device(self.device, out=out)
@@ -79,13 +79,10 @@ class LoraAdapters:
         need = self._need.get(t)
         if need is None:
             need = self._need[t] = int(lib.eux_lora_workspace_bytes(self._desc(t)))
-        with ws.on_device(self._index) as stream:
-            workspace, _ = self._scratch.get(stream, need)
-            rc = lib.eux_lora_launch(self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, ws.row_stride(x),
-                                                ws.row_stride(y), ws.row_stride(out)), stream)
-        if rc:
-            _native.check(rc, "eux_lora_launch")
-        _launches += 2 if t <= 64 else 3
+        workspace, _ = self._scratch.get(need)
+        desc = self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, ws.row_stride(x), ws.row_stride(y), ws.row_stride(out))
+        ws.launch(lib.eux_lora_launch, desc, self._index, "eux_lora_launch")
+        _launches += 2 if t <= 512 and t * self.rank * (self.K + self.N) * 2 <= 64 << 20 else 3  # as the launch chooses
         return out
 
     def _desc(self, tokens, x=0, ids=0, y=0, out=0, workspace=0, x_stride=0, y_stride=0, out_stride=0):

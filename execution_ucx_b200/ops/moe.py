@@ -188,18 +188,13 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: Op
         ws.require_dense(bias, "bias", torch.float32, (e,))
         ws.require_device(device, bias=bias)
     ws.require_cuda(device)
-    # one allocation for both: the weights behind the indices
-    both = torch.empty(2, t, topk, dtype=torch.int32, device=device)
-    idx, w = both[0], both[1].view(torch.float32)
+    idx = torch.empty_strided((t, topk), (topk, 1), dtype=torch.int32, device=device)
+    w = torch.empty_strided((t, topk), (topk, 1), dtype=torch.float32, device=device)
     if t:
-        at = both.data_ptr()
         desc = _native.descriptor(_native.ROUTE_DESC, _native.RouteDesc, logits.data_ptr(), bias.data_ptr() if bias is not None else 0,
-                                  at, at + 4 * t * topk, stride, t, e, topk, _native.DT_F32 if dtype is torch.float32 else _native.DT_BF16,
+                                  idx.data_ptr(), w.data_ptr(), stride, t, e, topk, _native.DT_F32 if dtype is torch.float32 else _native.DT_BF16,
                                   int(scoring == "sigmoid"), groups, topk_groups, int(renormalize), float(scale), 0)
-        with ws.on_device(device.index) as stream:
-            rc = _native.load().eux_route_launch(desc, stream)
-        if rc:
-            _native.check(rc, "eux_route_launch")
+        ws.launch(_native.load().eux_route_launch, desc, device.index, "eux_route_launch")
         _launches += 1
     return idx, w
 
@@ -257,7 +252,7 @@ class MoeExperts:
         self._room = C.create_string_buffer(256 + 64)
         self._maps = (C.addressof(self._room) + 63) & ~63
         with ws.on_device(self._index):
-            ws.check(lib.eux_experts_maps(self._desc(1, 1), self._maps), "eux_experts_maps")
+            _native.check(lib.eux_experts_maps(self._desc(1, 1), self._maps), "eux_experts_maps")
         self._scratch = ws.CallScratch(int(lib.eux_experts_counter_words(self._desc(1, 1))), self.device)
 
     w_gate_up = property(lambda self: self._weights[0])
@@ -289,24 +284,22 @@ class MoeExperts:
             self._require(x, topk_idx, topk_w)
         t, topk = topk_idx.shape
         if out is None:
-            out = torch.empty(t, hidden, dtype=torch.bfloat16, device=self.device)
+            out = torch.empty_strided((t, hidden), (hidden, 1), dtype=torch.bfloat16, device=self.device)
         else:
             ws.require_rows(out, "out", torch.bfloat16, cols=hidden, rows=t)
             ws.require_device(self.device, out=out)
         lib = _native.load()
         xs, os_ = ws.row_stride(x), ws.row_stride(out)
-        with ws.on_device(index) as stream:
-            for first in range(0, t, self.MAX_TOKENS):
-                n = min(self.MAX_TOKENS, t - first)
-                need = self._need.get((n, topk))
-                if need is None:
-                    need = self._need[n, topk] = int(lib.eux_experts_workspace_bytes(self._desc(n, topk)))
-                workspace, counters = self._scratch.get(stream, need)
-                rc = lib.eux_experts_launch(self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk,
-                                                       topk_w.data_ptr() + 4 * first * topk, out.data_ptr() + 2 * first * os_, workspace, counters, xs, os_), stream)
-                if rc:
-                    _native.check(rc, "eux_experts_launch")
-                _launches += 2
+        for first in range(0, t, self.MAX_TOKENS):
+            n = min(self.MAX_TOKENS, t - first)
+            need = self._need.get((n, topk))
+            if need is None:
+                need = self._need[n, topk] = int(lib.eux_experts_workspace_bytes(self._desc(n, topk)))
+            workspace, counters = self._scratch.get(need)
+            desc = self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk, topk_w.data_ptr() + 4 * first * topk,
+                              out.data_ptr() + 2 * first * os_, workspace, counters, xs, os_)
+            ws.launch(lib.eux_experts_launch, desc, index, "eux_experts_launch")
+            _launches += 2
         return out
 
     def _require(self, x, topk_idx, topk_w) -> None:

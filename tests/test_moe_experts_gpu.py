@@ -208,6 +208,35 @@ def test_two_streams_at_once(cuda_device):
         assert all(torch.equal(o, want[s]) for o in got[s])
 
 
+def test_threads_that_share_a_stream(cuda_device):
+    import threading
+    from execution_ucx_b200.ops import lora, moe
+    layer = moe.MoeExperts(*weights(8, 1024, 256, False, cuda_device))
+    adapters = lora.LoraAdapters(torch.randn(4, 16, 1024, device=cuda_device).to(torch.bfloat16), torch.randn(4, 1024, 16, device=cuda_device).to(torch.bfloat16))
+    args, want, got = [], [], [[] for _ in range(4)]
+    for s in range(4):
+        t = (3, 17, 40, 100)[s]
+        x = torch.randn(t, 1024, device=cuda_device).to(torch.bfloat16)
+        ids = torch.randint(0, 4, (t,), device=cuda_device, dtype=torch.int32)
+        args.append((x, *routing(t, 3, 8, cuda_device, s), ids))
+    both = lambda a: adapters(a[0], a[3], layer(*a[:3]))  # noqa: E731
+    for a in args:
+        want.append(both(a))
+    layer2 = moe.MoeExperts(layer.w_gate_up, layer.w_down)  # whose workspaces have yet to grow
+    both2 = lambda a: adapters(a[0], a[3], layer2(*a[:3]))  # noqa: E731
+
+    def run(s):
+        for _ in range(50):
+            got[s].append(both2(args[s]))
+    threads = [threading.Thread(target=run, args=(s,)) for s in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    layer2.check_status()
+    for s in range(4):
+        assert len(got[s]) == 50 and all(torch.equal(o, want[s]) for o in got[s])
+
+
 def test_captured_calls_replayed_beside_each_other_and_plain_ones(cuda_device):
     from execution_ucx_b200.ops import moe
     layer = moe.MoeExperts(*weights(8, 1024, 256, False, cuda_device))
