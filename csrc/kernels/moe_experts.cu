@@ -35,14 +35,20 @@
 
 namespace eux {
 
-constexpr int kXpGroups = 3;                        // of warps that multiply: each takes the blocks of every third stage ...
-constexpr int kXpWarps = kXpGroups * 4;             // ... and each of its four warps 32 rows of them
-constexpr int kXpEndThreads = 64;                   // two warps that see to the results
-constexpr int kXpThreads = kXpWarps * 32 + kXpEndThreads + 64;  // and a warp that fetches weights, one that fetches tokens
+constexpr int kXpThreads = 512;
+// Two ways to multiply. With mma.sync three groups of warps do it, each takes the blocks of every third stage, and each of its four
+// warps 32 rows of them; two warps see to the results. With tcgen05 one warp does it, four see to the results, the others help at both
+// ends.
+constexpr int kXpGroups = 3;
+constexpr int kXpWarps = kXpGroups * 4;
+template <bool TC>
+constexpr int kXpEndThreads = TC ? 128 : 64;
+constexpr int kXpAccColumns = 64;                   // of TMEM: the tokens of a segment at most
+constexpr int kXpFewColumns = 16;                   // bfloat16 weights: up to so many tokens of an expert are multiplied with mma.sync
 constexpr int kXpRows = 128;                        // rows of weights in a block
 constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
 constexpr int kXpMaxStages = 13;
-constexpr int kXpSumBars = 64;                      // bytes: for each of two sums, each group's and the results' barrier
+constexpr int kXpSumBars = 96;                      // bytes: for each of two sums, each group's and the results' barrier, and of tcgen05 two
 constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
 constexpr int kXpMaxGrid = 160;
 constexpr size_t kXpDynamic = 226 * 1024;           // shared memory of a launch; the kernel declares a little more itself
@@ -60,7 +66,7 @@ struct XpParams {
 };
 
 // Shared memory: the ring of weights (128-byte swizzle: on 1024 bytes), behind it the tokens' values of each stage, the sums
-// of a segment, twice where they are small; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
+// of a segment (tcgen05) or of two; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
 // many stages there is room for, is known when the entries have been counted.
 __host__ __device__ inline int xp_table_bytes(int n_experts, int entries) { return ((n_experts + 1) * 8 + entries * 8 + 31) & ~15; }
 struct XpLayout {
@@ -71,15 +77,17 @@ __host__ __device__ inline XpLayout xp_layout(bool down, int n_tokens, int n_exp
   XpLayout l;
   int at = (int)kXpDynamic;
   at -= xp_table_bytes(n_experts, entries), l.tables = at;
-  at -= kXpMaxStages * 16 + kXpSumBars, l.bars = at;
+  at -= kXpMaxStages * 32 + kXpSumBars, l.bars = at;
   at -= kXpMaxStages * 16, l.scales = at;
   at -= down ? n_tokens * kXpLd * 4 : 0, l.acc = at;
   l.room = at;
   return l;
 }
-__host__ __device__ inline int xp_sums(int cap) { return cap <= 32 ? 2 : 1; }
-__host__ __device__ inline int xp_stages(int room, int cap, int x_bytes) {
-  const int n = (room - xp_sums(cap) * cap * kXpLd * 4) / (kXpBlock + x_bytes);
+__host__ __device__ inline bool xp_tc(bool fp8, int columns) { return !fp8 && columns > kXpFewColumns; }
+__host__ __device__ inline int xp_sums(bool fp8, int columns) { return xp_tc(fp8, columns) ? 1 : 2; }
+__host__ __device__ inline int xp_x_bytes(bool fp8, int columns) { return columns * (fp8 ? 256 : 128); }
+__host__ __device__ inline int xp_stages(bool fp8, int room, int columns) {
+  const int n = (room - xp_sums(fp8, columns) * columns * kXpLd * 4) / (kXpBlock + xp_x_bytes(fp8, columns));
   return n < kXpMaxStages ? n : kXpMaxStages;
 }
 
@@ -123,7 +131,35 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void end_warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpEndThreads) : "memory"); }
+template <bool TC>
+__device__ __forceinline__ void end_warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kXpEndThreads<TC>) : "memory"); }
+
+// ---- tcgen05 (bfloat16 weights, many tokens): the weights' 128 rows are the first operand, the tokens the second, the accumulators lie in TMEM ----
+__device__ __forceinline__ uint64_t xp_operand(uint32_t at) {  // rows of 128 bytes, swizzled, eight of them 1024 bytes apart from the next
+  return (uint64_t)((at >> 4) & 0x3fffu) | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void xp_multiply(uint32_t acc, uint64_t a, uint64_t b, int columns, bool add) {
+  // float32 += bfloat16 x bfloat16, 128 rows
+  const uint32_t what = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(columns >> 3) << 17 | (uint32_t)(kXpRows >> 4) << 24;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(acc), "l"(a), "l"(b), "r"(what), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void xp_multiplied(uint32_t bar) {  // arrives when the products so far are through
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void xp_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void xp_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void xp_acc_16(uint32_t at, float (&v)[16]) {  // of this lane's row
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(at)
+      : "memory");
+}
 
 // Four e4m3 values as bfloat16, bytes 0 and 2 in `even` and 1 and 3 in `odd`: sign, exponent and mantissa are moved to their places,
 // which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and multiplied by
@@ -364,7 +400,7 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int& mine, int end, int
   while (mine < end) {
     // A wait that ran out raises `abort`; the warps then finish on whatever lies there, so that they meet at every barrier, and the
     // status word says that the result is none.
-    mbar_sleep(ring.full + 16 * ring.s, ring.ph, abort, timeout_ns);
+    mbar_sleep(ring.full + 32 * ring.s, ring.ph, abort, timeout_ns);
     __syncwarp();
     const uint32_t w = ring.w + ring.s * kXpBlock, x = ring.x + ring.s * ring.x_bytes;
     if constexpr (!FP8) {
@@ -448,7 +484,7 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int& mine, int end, int
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(ring.empty + 16 * ring.s);
+    if (lane == 0) mbar_arrive(ring.empty + 32 * ring.s);
     ring.next_of_group(group, mine);
   }
   mbar_sleep(bars + (group ? 8 * (group - 1) : 8 * kXpGroups), group ? bars_ph : bars_ph ^ 1u, abort, timeout_ns);
@@ -550,29 +586,127 @@ __device__ __forceinline__ void xp_tile_end(const XpParams& p, const XpTables& r
   }
 }
 
+// What the warps that see to the results do.
+template <bool DOWN>
+struct XpResults {
+  const XpParams& p;
+  const XpTables& r;
+  const XpShares& shares;
+  int b0, b1, seg0, nk, chunks, me;
+  bool in_place;
+  int columns;
+  float *sums, *acc;
+  int* s_last;
+  volatile int* abort;
+
+  template <bool TC>
+  __device__ __forceinline__ void make(XpWalk<DOWN>& walk, uint32_t all_bars, uint32_t tmem, int tid) const {
+    const eux_experts_desc& d = p.d;
+    constexpr int THREADS = kXpEndThreads<TC>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
+    const int tile_blocks = tile_segs * nk;
+    if (DOWN && chunks == 0) {  // no expert is named: the result is zero
+      for (int i = blockIdx.x * THREADS + tid; i < d.n_tokens * (d.hidden / 8); i += gridDim.x * THREADS)
+        st_u4((__nv_bfloat16*)d.out + (int64_t)(i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
+    }
+    int buf = 0, tile = b0 < b1 ? seg0 / tile_segs : 0;
+    uint32_t buf_ph = 0;
+    for (int b = b0, seg = seg0; b < b1; ++seg) {
+      const XpSegment s = walk.at(seg);
+      const int tile0 = tile * tile_blocks, tile1 = tile0 + tile_blocks;
+      float* const sum = sums + (TC ? 0 : buf * columns * kXpLd);
+      const uint32_t bars = all_bars + buf * 8 * (TC ? 2 : kXpGroups + 1), free_bar = bars + 8 * (TC ? 1 : kXpGroups);
+      if (DOWN && b == tile0 && b != b0) {
+        for (int i = tid; i < d.n_tokens * (kXpLd / 4); i += THREADS) reinterpret_cast<float4*>(acc)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        end_warps_meet<TC>();
+      }
+      mbar_sleep(bars + (TC ? 0 : 8 * (kXpGroups - 1)), buf_ph, abort, d.wait_timeout_ns);
+      __syncwarp();
+      b = min((seg + 1) * nk, b1);
+      // Down: entries of the same token, also twice of the same expert, are added by one thread, which has one or two rows, in order.
+      if (TC) {
+        // A thread has a row, which is a lane of TMEM.
+        xp_fence_after();
+        for (int j0 = 0; j0 < s.n; j0 += 16) {
+          float v[16];
+          xp_acc_16(tmem + buf * kXpAccColumns + j0 + ((uint32_t)(warp * 32) << 16), v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (j0 + i < s.n) {
+              if (DOWN) {
+                float* const at = acc + r.token[s.pos + j0 + i] * kXpLd + tid;
+                *at = fmaf(r.weight[s.pos + j0 + i], v[i], *at);
+              } else {
+                sum[(j0 + i) * kXpLd + tid] = v[i];
+              }
+            }
+        }
+        xp_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(free_bar);
+      } else if (DOWN) {
+        for (int j0 = 0; j0 < s.n; j0 += 4) {
+          float2 v[4];
+          float w[4];
+          int t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = min(j0 + i, s.n - 1);
+            v[i] = reinterpret_cast<const float2*>(sum + j * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j0 + i < s.n) {
+              float2* const at = reinterpret_cast<float2*>(acc + t[i] * kXpLd) + tid;
+              *at = make_float2(fmaf(w[i], v[i].x, at->x), fmaf(w[i], v[i].y, at->y));
+            }
+        }
+      }
+      if (!DOWN || b == b1 || b == tile1) {
+        // the end of a tile, or of this SM's part of it
+        end_warps_meet<TC>();  // what they have put together is complete
+        if (b == b1) break;    // the end of the share is everybody's
+        xp_tile_end<DOWN, THREADS>(p, r, s, shares.owner(tile0), shares.owner(tile1 - 1), me, DOWN ? acc : sum, in_place, tid, s_last, end_warps_meet<TC>);
+        end_warps_meet<TC>();  // and is written over next
+        if (b == tile1) ++tile;
+      }
+      if (!TC) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(free_bar);
+      }
+      if ((buf ^= 1) == 0) buf_ph ^= 1u;
+    }
+  }
+};
+
 template <bool FP8, bool DOWN>
 __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ XpMaps x_maps, const __grid_constant__ XpParams p) {
   extern __shared__ __align__(1024) unsigned char xp_smem[];
   __shared__ int s_abort, s_last, s_route[4 + 2 * kXpThreads / 32];
+  __shared__ uint32_t s_acc;
   const eux_experts_desc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entries = d.n_tokens * d.topk;
   const XpLayout l = xp_layout(DOWN, d.n_tokens, d.n_experts, entries);
   const uint32_t smem = smem_u32(xp_smem);
   XpRing ring;
-  ring.w = smem, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;
-  const uint32_t sum_bars = smem + l.bars + kXpMaxStages * 16;
+  ring.w = smem, ring.scales = smem + l.scales, ring.full = smem + l.bars, ring.empty = smem + l.bars + 8;  // tcgen05: + 16
+  const uint32_t sum_bars = smem + l.bars + kXpMaxStages * 32, tc_bars = sum_bars + 2 * (kXpGroups + 1) * 8;
   if (threadIdx.x == 0) {
     s_abort = 0;
     for (int i = 0; i < kXpMaxStages; ++i) {
-      mbar_init(ring.full + 16 * i, 2);   // weights and tokens
-      mbar_init(ring.empty + 16 * i, 4);  // the warps of a group
+      mbar_init(ring.full + 32 * i, 2);       // weights and tokens
+      mbar_init(ring.empty + 32 * i, 4);      // the warps of a group
+      mbar_init(ring.empty + 32 * i + 8, 1);
     }
-    for (int i = 0; i < 2 * (kXpGroups + 1); ++i) mbar_init(sum_bars + 8 * i, i % (kXpGroups + 1) < kXpGroups ? 4 : kXpEndThreads / 32);
+    for (int i = 0; i < 2 * (kXpGroups + 1); ++i) mbar_init(sum_bars + 8 * i, i % (kXpGroups + 1) < kXpGroups ? 4 : kXpEndThreads<false> / 32);
+    for (int i = 0; i < 4; ++i) mbar_init(tc_bars + 8 * i, i % 2 ? kXpEndThreads<true> / 32 : 1);  // full and free, of two accumulators
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&x_maps.of[0]) : "memory");
   }
+  constexpr int kProducts = 4, kWeights = kXpThreads / 32 - 2, kTokens = kWeights + 1;  // warps
   // The up form waits here for whatever wrote the tokens and their experts. The down form was let in by the up form, behind its
   // wait: what both read is there, in the L2, and only what the up form writes is waited for (below).
   if (!DOWN) wait_for_launch_before();
@@ -584,13 +718,22 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
     r.named = (int)__ldcg(p.tables), cap = (int)__ldcg(p.tables + 1);
     __syncthreads();
   } else {
-    cap = xp_route(d, p.token_of, FP8 ? 32 : 64, r, reinterpret_cast<int*>(xp_smem), s_route);
+    cap = xp_route(d, p.token_of, FP8 ? 32 : kXpAccColumns, r, reinterpret_cast<int*>(xp_smem), s_route);
   }
   // Up to eight tokens lie where they are: each is a column of every product, whichever of them an expert has.
   const bool in_place = !DOWN && !p.x;
   const int columns = in_place ? 8 : cap;
-  ring.x_bytes = columns * (FP8 ? 256 : 128);
-  ring.stages = xp_stages(l.room, columns, ring.x_bytes);
+  // Few tokens take a tensor core little time either way, and tcgen05 draws more power for its padding to 16: the memory clock's share of
+  // it is what counts then (16 tokens, 32 experts of 7168 x 2048: 421 us with mma.sync, 439 with tcgen05; one token 115.5 and 120). With
+  // more, operands through registers are what an SM waits for (128 tokens, top-4 of 16 experts of 4096 x 2048: 187 and 160).
+  const bool tc = xp_tc(FP8, columns);
+  if (!FP8 && tc && warp == kProducts) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_acc)), "r"(2u * kXpAccColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tc) ring.empty += 8;
+  ring.x_bytes = xp_x_bytes(FP8, columns);
+  ring.stages = xp_stages(FP8, l.room, columns);
   ring.x = smem + ring.stages * kXpBlock;
   const int K = DOWN ? d.inner : d.hidden, per_block = FP8 ? 128 : 64;
   const int nk = (K + per_block - 1) / per_block;
@@ -603,17 +746,18 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   const int b0 = me < grid ? shares.begin(me) : blocks, b1 = me < grid ? shares.begin(me + 1) : blocks;
   const int seg0 = b0 / nk, kb0 = b0 - seg0 * nk;  // the segment that the share begins in, and where
   float* const sums = reinterpret_cast<float*>(xp_smem + ring.stages * (kXpBlock + ring.x_bytes));
-  const int n_sums = xp_sums(columns);
+  const int n_sums = xp_sums(FP8, columns);
   float* const acc = reinterpret_cast<float*>(xp_smem + l.acc);
   if (DOWN)
     for (int i = threadIdx.x; i < d.n_tokens * (kXpLd / 4); i += kXpThreads) reinterpret_cast<float4*>(acc)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   // the counts lay where weights are about to land
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  xp_fence_before();
   __syncthreads();
+  xp_fence_after();
   volatile int* abort = &s_abort;
   XpWalk<DOWN> walk(r, tiles);
 
-  constexpr int kWeights = kXpThreads / 32 - 2, kTokens = kWeights + 1;
   if (warp == kWeights) {
     // ---- weights ----
     if (lane == 0) {
@@ -621,8 +765,8 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
         const int end = min(nk, kb + (b1 - b));
         const XpSegment s = walk.at(seg);
         for (int k = kb; k < end; ++k) {
-          if (!mbar_sleep(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns)) break;
-          const uint32_t bar = ring.full + 16 * ring.s, dst = ring.w + ring.s * kXpBlock;
+          if (!mbar_sleep(ring.empty + 32 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns)) break;
+          const uint32_t bar = ring.full + 32 * ring.s, dst = ring.w + ring.s * kXpBlock;
           mbar_expect_tx(bar, kXpBlock);
           if (DOWN) tma_load_3d(dst, &map, bar, k * per_block, s.tile * kXpRows, s.expert);
           else tma_load_3d(dst, &map, bar, k * per_block, s.tile * 64, s.expert * 2);  // 64 gate rows, and 64 up rows behind them
@@ -658,9 +802,9 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
             sc[q] = k + lane < end ? __ldg(scale + (int64_t)block * sk + k + lane) : 0.f;
           }
         }
-        gone = __any_sync(0xffffffffu, !mbar_sleep(ring.empty + 16 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
+        gone = __any_sync(0xffffffffu, !mbar_sleep(ring.empty + 32 * ring.s, ring.ph ^ 1u, abort, d.wait_timeout_ns));
         if (gone) break;
-        const uint32_t bar = ring.full + 16 * ring.s, dst = ring.x + ring.s * ring.x_bytes;
+        const uint32_t bar = ring.full + 32 * ring.s, dst = ring.x + ring.s * ring.x_bytes;
         if (FP8) {
           float v[3];
 #pragma unroll
@@ -679,8 +823,8 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       const uint64_t t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-  } else if (warp < kXpWarps) {
-    // ---- products ----
+  } else if (!tc && warp < kXpWarps) {
+    // ---- products with mma.sync ----
     int mine = b0 + (warp >> 2), sum_at = 0;
     uint32_t sum_ph = 0;
     ring.s = warp >> 2;
@@ -692,74 +836,59 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       float* const sum = sums + sum_at * columns * kXpLd;
       const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
       if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
-      else if (nb <= 4) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
-      else if constexpr (!FP8) xp_segment<FP8, DOWN, 8>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if (!FP8 || nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if constexpr (FP8) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
       if (++sum_at == n_sums) sum_at = 0, sum_ph ^= 1u;
       b = end;
     }
-  } else {
-    // ---- results ----
-    if (DOWN) wait_for_launch_before();
-    const int tid = threadIdx.x - kXpWarps * 32;
-    const int tile_segs = DOWN ? chunks : 1;  // segments of a tile of results
-    const int tile_blocks = tile_segs * nk;
-    if (DOWN && blocks == 0) {  // no expert is named: the result is zero
-      for (int i = blockIdx.x * kXpEndThreads + tid; i < d.n_tokens * (d.hidden / 8); i += gridDim.x * kXpEndThreads)
-        st_u4((__nv_bfloat16*)d.out + (int64_t)(i / (d.hidden / 8)) * d.out_stride + (i % (d.hidden / 8)) * 8, make_uint4(0, 0, 0, 0));
-    }
-    int sum_at = 0, tile = b0 < b1 ? seg0 / tile_segs : 0;
-    uint32_t sum_ph = 0;
-    for (int b = b0, seg = seg0; b < b1; ++seg) {
-      const XpSegment s = walk.at(seg);
-      const int tile0 = tile * tile_blocks, tile1 = tile0 + tile_blocks;
-      float* const sum = sums + sum_at * columns * kXpLd;
-      const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
-      if (DOWN && b == tile0 && b != b0) {
-        for (int i = tid; i < d.n_tokens * (kXpLd / 4); i += kXpEndThreads) reinterpret_cast<float4*>(acc)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        end_warps_meet();
-      }
-      mbar_sleep(bars + 8 * (kXpGroups - 1), sum_ph, abort, d.wait_timeout_ns);
-      __syncwarp();
-      b = min((seg + 1) * nk, b1);
-      if (DOWN) {
-        // A thread has two rows: entries of the same token, also twice of the same expert, are added by one thread, in order.
-        for (int j0 = 0; j0 < s.n; j0 += 4) {
-          float2 v[4];
-          float w[4];
-          int t[4];
+  } else if (!FP8 && tc && warp == kProducts) {
+    // ---- products with tcgen05 ----
+    if (lane == 0) {
+      int buf = 0;
+      uint32_t buf_ph = 0;
+      bool gone = false;
+      for (int b = b0, seg = seg0; b < b1 && !gone; ++seg) {
+        const int end = min((seg + 1) * nk, b1);
+        const XpSegment s = walk.at(seg);
+        const int n = s.n <= 16 ? 16 : s.n <= 32 ? 32 : 64;  // 16 are the fewest
+        const uint32_t bars = tc_bars + buf * 16, acc = s_acc + buf * kXpAccColumns;
+        gone = !mbar_sleep(bars + 8, buf_ph ^ 1u, abort, d.wait_timeout_ns);
+        xp_fence_after();
+        for (int k = b; k < end && !gone; ++k) {
+          if ((gone = !mbar_sleep(ring.full + 32 * ring.s, ring.ph, abort, d.wait_timeout_ns))) break;
+          xp_fence_after();
+          const uint64_t w = xp_operand(ring.w + ring.s * kXpBlock), x = xp_operand(ring.x + ring.s * ring.x_bytes);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = min(j0 + i, s.n - 1);
-            v[i] = reinterpret_cast<const float2*>(sum + j * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (j0 + i < s.n) {
-              float2* const at = reinterpret_cast<float2*>(acc + t[i] * kXpLd) + tid;
-              *at = make_float2(fmaf(w[i], v[i].x, at->x), fmaf(w[i], v[i].y, at->y));
-            }
+          for (int i = 0; i < 4; ++i) xp_multiply(acc, w + 2 * i, x + 2 * i, n, k > b || i > 0);  // 16 of K, 32 bytes, each
+          xp_multiplied(ring.empty + 32 * ring.s);
+          ring.next();
         }
+        if (!gone) xp_multiplied(bars);
+        if ((buf ^= 1) == 0) buf_ph ^= 1u;
+        b = end;
       }
-      if (!DOWN || b == b1 || b == tile1) {
-        // ---- the end of a tile, or of this SM's part of it ----
-        end_warps_meet();  // acc is complete
-        if (b == b1) break;  // the end of the share is everybody's
-        xp_tile_end<DOWN, kXpEndThreads>(p, r, s, shares.owner(tile0), shares.owner(tile1 - 1), me, DOWN ? acc : sum, in_place, tid, &s_last, end_warps_meet);
-        if (DOWN) end_warps_meet();  // acc is written over next
-        if (b == tile1) ++tile;
+      if (gone) {  // products that were begun still write TMEM and read shared memory
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars + 8 * kXpGroups);
-      if (++sum_at == n_sums) sum_at = 0, sum_ph ^= 1u;
     }
+  } else if (!tc || warp < kXpEndThreads<true> / 32) {
+    if (DOWN) wait_for_launch_before();
+    const XpResults<DOWN> results{p, r, shares, b0, b1, seg0, nk, chunks, me, in_place, columns, sums, acc, &s_last, abort};
+    if (!tc) results.template make<false>(walk, sum_bars, 0, threadIdx.x - kXpWarps * 32);
+    else if constexpr (!FP8) results.template make<true>(walk, tc_bars, s_acc, threadIdx.x);
   }
+  xp_fence_before();
   __syncthreads();
   if (b0 < b1) {
     const int seg = (b1 - 1) / nk, tile_segs = DOWN ? chunks : 1, tile = seg / tile_segs, tile0 = tile * tile_segs * nk;
     const XpSegment s = walk.at(seg);
     xp_tile_end<DOWN, kXpThreads>(p, r, s, shares.owner(tile0), shares.owner(tile0 + tile_segs * nk - 1), me,
                                   DOWN ? acc : sums + (seg - seg0) % n_sums * columns * kXpLd, in_place, threadIdx.x, &s_last, cta_meets);
+  }
+  if (!FP8 && tc && warp == kProducts) {
+    xp_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_acc), "r"(2u * kXpAccColumns) : "memory");
   }
   if (threadIdx.x == 0 && s_abort) set_status(d.status, EUX_ST_TIMEOUT, DOWN ? 2 : 1);
 }
@@ -866,8 +995,8 @@ template <bool FP8, bool DOWN>
 static int xp_launch(const CUtensorMap& map, const XpMaps& x_maps, const XpParams& p, int dev, int sms, cudaStream_t st) {
   const eux_experts_desc& d = p.d;
   // the ring holds a block of every group; the routing's counts lie where the ring will be
-  const int room = xp_layout(DOWN, d.n_tokens, d.n_experts, d.n_tokens * d.topk).room, most = FP8 ? 32 : 64;
-  if (xp_stages(room, most, most * (FP8 ? 256 : 128)) < kXpGroups || kXpThreads / 32 * d.n_experts * 4 > room) return EUX_ERR_TOO_LARGE;
+  const int room = xp_layout(DOWN, d.n_tokens, d.n_experts, d.n_tokens * d.topk).room;
+  if (xp_stages(FP8, room, FP8 ? 32 : kXpAccColumns) < kXpGroups || xp_stages(FP8, room, kXpFewColumns) < kXpGroups || kXpThreads / 32 * d.n_experts * 4 > room) return EUX_ERR_TOO_LARGE;
   if (cudaError_t e = allow_smem<moe_experts_kernel<FP8, DOWN>>(dev, kXpDynamic); e != cudaSuccess) return (int)e;
   return launch_early(moe_experts_kernel<FP8, DOWN>, sms, kXpThreads, kXpDynamic, st, map, x_maps, p);
 }
@@ -925,7 +1054,7 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
     if (cudaError_t e = allow_smem<moe_experts_sort_kernel>(dev, 200 * 1024); e != cudaSuccess) return (int)e;
     const int64_t pieces = (int64_t)entries * (p.x_pitch / 8);
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(sms, pieces / kXpThreads));
-    if (int rc = launch_early(moe_experts_sort_kernel, grid, kXpThreads, smem, st, p, d->fp8 ? 32 : 64)) return rc;
+    if (int rc = launch_early(moe_experts_sort_kernel, grid, kXpThreads, smem, st, p, d->fp8 ? 32 : kXpAccColumns)) return rc;
   }
   if (int rc = d->fp8 ? xp_launch<true, false>(*up, x, p, dev, sms, st) : xp_launch<false, false>(*up, x, p, dev, sms, st)) return rc;
   return d->fp8 ? xp_launch<true, true>(*down, h, p, dev, sms, st) : xp_launch<false, true>(*down, h, p, dev, sms, st);
