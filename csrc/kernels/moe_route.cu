@@ -31,11 +31,6 @@ __device__ __forceinline__ double key_value(uint64_t k) {
 }
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
-  return ((uint64_t)hi << 32) | lo;
-}
 __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -51,21 +46,47 @@ __device__ __forceinline__ float route_logit(const eux_route_desc& d, int64_t t,
                                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(d.logits)[at]);
 }
 
-// The largest key of the warp's registers and its expert (0 and any: none left). KEEP: it stays.
+// A lane's largest key and where it is, from its registers.
 template <int NV, typename Key>
-__device__ __forceinline__ int take_best(Key (&key)[NV], int lane, Key* best) {
-  Key mine = 0;
-  int at = 0;
+__device__ __forceinline__ void lane_best(const Key (&key)[NV], Key& mine, int& at) {
+  mine = 0, at = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (key[i] > mine) mine = key[i], at = i;
-  const Key m = warp_max(mine);
-  *best = m;
-  const uint32_t e = __reduce_min_sync(0xffffffffu, m != 0 && mine == m ? (uint32_t)(at * 32 + lane) : 0xffffffffu);
+}
+// The warp's largest key, of equal ones that of the lowest expert, is taken out; its expert, -1 if there is none. `mine` and `at` are the
+// lanes' largest.
+template <int NV>
+__device__ __forceinline__ int take_best(uint32_t (&key)[NV], uint32_t& mine, int& at, int lane) {
+  const uint32_t top = warp_max(mine);
+  const uint32_t e = __reduce_min_sync(0xffffffffu, mine == top ? (uint32_t)(at * 32 + lane) : 0xffffffffu);
+  if (top == 0) return -1;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if ((uint32_t)(i * 32 + lane) == e) key[i] = 0;
-  return m != 0 ? (int)e : -1;
+  lane_best<NV>(key, mine, at);
+  return (int)e;
+}
+// With 64-bit keys the upper halves nearly always tell; only where they do not are the lower ones, and then the experts, asked, and only
+// the lane that had it looks for its next one.
+template <int NV>
+__device__ __forceinline__ int take_best(uint64_t (&key)[NV], uint64_t& mine, int& at, int lane) {
+  const uint32_t top = warp_max((uint32_t)(mine >> 32));
+  uint32_t who = __ballot_sync(0xffffffffu, mine != 0 && (uint32_t)(mine >> 32) == top);
+  if (who == 0) return -1;
+  if (who & (who - 1)) {
+    const uint32_t low = warp_max((who >> lane) & 1u ? (uint32_t)mine : 0u);
+    who = __ballot_sync(0xffffffffu, ((who >> lane) & 1u) && (uint32_t)mine == low);
+    who = 1u << (__reduce_min_sync(0xffffffffu, (who >> lane) & 1u ? (uint32_t)(at * 32 + lane) : 0xffffffffu) & 31u);
+  }
+  const int winner = __ffs(who) - 1, e = __shfl_sync(0xffffffffu, at, winner) * 32 + winner;
+  if (lane == winner) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i == at) key[i] = 0;
+    lane_best<NV>(key, mine, at);
+  }
+  return e;
 }
 
 // WIDE: scores and keys in 64 bits (bias or groups).
@@ -74,6 +95,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
   using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
   using Real = typename std::conditional<WIDE, double, float>::type;
   wait_for_launch_before();
+  __shared__ uint64_t keys[WIDE ? kRouteWarps : 1][WIDE ? NV * 32 : 1];
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
   if (t < d.n_tokens) {
@@ -111,7 +133,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
       if (l[i] > -INFINITY) {
         if constexpr (WIDE) {
           const float b = d.bias ? d.bias[e] : 0.f;
-          const double s = d.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : ex[i] / sum;
+          const double s = d.sigmoid ? __drcp_rn(1.0 + exp(-(double)l[i])) : ex[i] / sum;
           if (b > -INFINITY) key[i] = order_key(s + (double)b);
         } else {
           key[i] = order_key(route_logit(d, t, e));  // with +inf above the largest number
@@ -120,19 +142,25 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
     }
     if constexpr (WIDE) {
       if (d.groups > 1) {
-        const int size = E / d.groups;
-        double score = -INFINITY;  // of the group with this lane's number
-        for (int g = 0; g < d.groups; ++g) {
-          uint64_t in[NV], b1, b2;
+        // As many lanes as there are for each group look through its experts, in shared memory, for the two largest.
+        const int size = E / d.groups, per = 32 / d.groups, lanes = per >= 16 ? 16 : per >= 8 ? 8 : per >= 4 ? 4 : per >= 2 ? 2 : 1;
+        uint64_t* const mine = keys[threadIdx.x >> 5];
 #pragma unroll
-          for (int i = 0; i < NV; ++i) {
-            const int e = i * 32 + lane;
-            in[i] = e >= g * size && e < (g + 1) * size ? key[i] : 0;
+        for (int i = 0; i < NV; ++i) mine[i * 32 + lane] = key[i];
+        __syncwarp();
+        const int g0 = lane / lanes;
+        uint64_t b1 = 0, b2 = 0;
+        if (g0 < d.groups)
+          for (int e = lane % lanes; e < size; e += lanes) {
+            const uint64_t k = mine[g0 * size + e], low = min(k, b1);
+            b1 = max(k, b1), b2 = max(low, b2);
           }
-          take_best<NV>(in, lane, &b1);
-          take_best<NV>(in, lane, &b2);
-          if (lane == g && b1) score = key_value(b1) + (b2 ? key_value(b2) : 0.0);
+        for (int o = 1; o < lanes; o <<= 1) {
+          const uint64_t o1 = __shfl_xor_sync(0xffffffffu, b1, o), o2 = __shfl_xor_sync(0xffffffffu, b2, o);
+          b2 = max(min(b1, o1), max(b2, o2)), b1 = max(b1, o1);
         }
+        const double of_mine = b1 ? key_value(b1) + (b2 ? key_value(b2) : 0.0) : -INFINITY;
+        const double score = __shfl_sync(0xffffffffu, of_mine, min(lane, d.groups - 1) * lanes);  // of the group with this lane's number
         int ahead = 0;
         for (int g = 0; g < d.groups; ++g) {
           const double other = __shfl_sync(0xffffffffu, score, g);
@@ -146,16 +174,17 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
         }
       }
     }
-    int mine = -1;  // lane j: the expert in place j
+    int mine = -1, at;  // lane j: the expert in place j
+    Key best;
+    lane_best<NV>(key, best, at);
     for (int j = 0; j < d.topk; ++j) {
-      Key best;
-      const int e = take_best<NV>(key, lane, &best);
+      const int e = take_best<NV>(key, best, at, lane);
       if (lane == j) mine = e;
     }
     Real s = 0;
     if (mine >= 0) {
       const float v = fminf(route_logit(d, t, mine), 3.402823466e38f);
-      if constexpr (WIDE) s = d.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)peak) / sum;
+      if constexpr (WIDE) s = d.sigmoid ? __drcp_rn(1.0 + exp(-(double)v)) : exp((double)v - (double)peak) / sum;
       else s = d.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - peak) / sum;
     }
     if (d.renormalize) {
