@@ -261,6 +261,8 @@ typedef struct eux_experts_desc {
   int32_t n_tokens, hidden, inner, n_experts, topk;
   int32_t fp8;                 /* 0: bf16 weights; 1: e4m3 weights with one fp32 scale per 128 x 128 block */
 } eux_experts_desc;
+/* Stores 1 to `found` (device memory) if one of the e4m3 values is NaN: such weights the kernels do not multiply as what they are. */
+EUX_API int eux_experts_find_nan(const void* e4m3, size_t bytes, uint32_t* found, void* stream);
 #define EUX_EXPERTS_MAPS_BYTES 256
 /* What the launches need to know of where the weights lie, into EUX_EXPERTS_MAPS_BYTES of host memory on 64 bytes; made once
  * for weights that stay where they are. */

@@ -917,6 +917,16 @@ __global__ void __launch_bounds__(kXpThreads) moe_experts_sort_kernel(const __gr
   allow_next_launch();
 }
 
+// Whether one of n 16-byte pieces holds an e4m3 NaN (0x7f or 0xff).
+__global__ void __launch_bounds__(512) moe_experts_nan_kernel(const uint4* q, size_t n, uint32_t* found) {
+  uint32_t any = 0;
+  for (size_t i = (size_t)blockIdx.x * 512 + threadIdx.x; i < n; i += (size_t)gridDim.x * 512) {
+    const uint4 v = ld_stream_u4(q + i);
+    any |= ((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u) | ((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u);
+  }
+  if (any & 0x80808080u) *found = 1;
+}
+
 // ---- host ----
 
 typedef CUresult (*XpEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1019,6 +1029,15 @@ extern "C" int eux_experts_maps(const eux_experts_desc* d, void* maps) {
 }
 extern "C" size_t eux_experts_counter_words(const eux_experts_desc* d) { return experts_check(d) ? 0 : 2 * kXpMaxGrid; }
 
+extern "C" int eux_experts_find_nan(const void* e4m3, size_t bytes, uint32_t* found, void* stream) {
+  if (!e4m3 || !found || (uintptr_t)e4m3 & 15 || bytes % 16) return EUX_ERR_BAD_ARG;
+  if (bytes == 0) return 0;
+  int dev = 0;
+  const size_t n = bytes / 16;
+  moe_experts_nan_kernel<<<(int)std::min<size_t>((n + 511) / 512, 8 * xp_sms(&dev)), 512, 0, (cudaStream_t)stream>>>((const uint4*)e4m3, n, found);
+  return (int)cudaGetLastError();
+}
+
 extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   if (int rc = experts_check(d)) return rc;
   if (d->n_tokens == 0) return 0;
@@ -1064,7 +1083,7 @@ extern "C" int eux_experts_preload(void) {
   cudaFuncAttributes a;
   const void* kernels[] = {(const void*)moe_experts_kernel<false, false>, (const void*)moe_experts_kernel<false, true>,
                            (const void*)moe_experts_kernel<true, false>, (const void*)moe_experts_kernel<true, true>,
-                           (const void*)moe_experts_sort_kernel};
+                           (const void*)moe_experts_sort_kernel, (const void*)moe_experts_nan_kernel};
   for (const void* k : kernels)
     if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;
   return 0;

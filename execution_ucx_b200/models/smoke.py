@@ -44,6 +44,7 @@ def run(device: torch.device) -> None:
     from ..ops import remote_gemm
     remote_gemm.smoke(device)
     _fp8_block_gemm(device)
+    _experts_and_adapters(device)
     _data_plane_echo_and_pingpong(device)
     _axon_round_trip(device)
 
@@ -60,6 +61,32 @@ def _fp8_block_gemm(device: torch.device) -> None:
     torch.cuda.synchronize()
     gemm.check_status()
     torch.testing.assert_close(y.float(), g.dequantized_reference(xq, xs, gemm.w_q_t, gemm.w_scale), rtol=3e-2, atol=3e-2)
+
+
+def _experts_and_adapters(device: torch.device) -> None:
+    """The choice of experts, the expert layer (few and many tokens of an expert, bf16 and e4m3) and adapters of several requests."""
+    from ..ops import lora, moe
+    from ..ops.remote_gemm import quantize_blocks_128x128
+    gate_up = (torch.randn(4, 256, 256, device=device) * 0.06).to(torch.bfloat16)
+    down = (torch.randn(4, 256, 128, device=device) * 0.09).to(torch.bfloat16)
+    quantized = [[torch.stack(v) for v in zip(*(quantize_blocks_128x128(e) for e in w))] for w in (gate_up, down)]
+    layers = [(moe.MoeExperts(gate_up, down), (gate_up, down)),
+              (moe.MoeExperts(quantized[0][0], quantized[1][0], quantized[0][1], quantized[1][1]),
+               (quantized[0][0], quantized[1][0], quantized[0][1], quantized[1][1]))]
+    for t in (1, 64):
+        x = torch.randn(t, 256, device=device).to(torch.bfloat16)
+        idx, w = moe.route(torch.randn(t, 4, device=device), 2, scoring="sigmoid", bias=torch.zeros(4, device=device), groups=2, topk_groups=2)
+        for layer, weights in layers:
+            out = layer(x, idx, w)
+            torch.cuda.synchronize()
+            layer.check_status()
+            torch.testing.assert_close(out.double(), moe.reference_experts(x, idx, w, *weights), rtol=2e-2, atol=2e-2)
+    for t in (2, 600):
+        a, b = torch.randn(3, 16, 512, device=device).to(torch.bfloat16), torch.randn(3, 4096, 16, device=device).to(torch.bfloat16)
+        adapters = lora.LoraAdapters(a * 512 ** -0.5, b * 0.25, torch.ones(3, device=device))
+        x, y = torch.randn(t, 512, device=device).to(torch.bfloat16), torch.randn(t, 4096, device=device).to(torch.bfloat16)
+        ids = torch.arange(t, device=device, dtype=torch.int32) % 4 - 1
+        torch.testing.assert_close(adapters(x, ids, y).double(), lora.reference(x, ids, y, adapters.a, adapters.b, adapters.scale), rtol=2e-2, atol=2e-2)
 
 
 def _data_plane_echo_and_pingpong(device: torch.device) -> None:

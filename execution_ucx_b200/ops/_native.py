@@ -163,6 +163,7 @@ def load():
     for op in ("route", "experts", "lora"):
         getattr(lib, f"eux_{op}_launch").argtypes = [P, P]
     lib.eux_experts_maps.argtypes = [P, P]
+    lib.eux_experts_find_nan.argtypes = [P, C.c_size_t, P, P]
     for size in ("eux_experts_workspace_bytes", "eux_experts_counter_words", "eux_lora_workspace_bytes"):
         getattr(lib, size).argtypes = [P]
         getattr(lib, size).restype = C.c_size_t

@@ -239,16 +239,19 @@ class MoeExperts:
         ws.require_device(self.device, w_gate_up=w_gate_up, gate_up_scale=gate_up_scale, down_scale=down_scale)
         ws.require_cuda(self.device)
         ws.require((w_gate_up.data_ptr() | w_down.data_ptr()) % 16 == 0, "weights must begin on 16 bytes")
-        if self.fp8:
-            # the kernels widen e4m3 by moving bits, which has no place for NaN
-            nan = sum(((w[j].view(torch.uint8) & 0x7F) == 0x7F).any() for w in (w_gate_up, w_down) for j in range(e))
-            ws.require(int(nan) == 0, "e4m3 weights must not be NaN")
         self._weights = (w_gate_up, w_down, gate_up_scale, down_scale)
         self._weight_ptrs = tuple(w.data_ptr() if w is not None else 0 for w in self._weights)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status_ptr, self._index = self.status.data_ptr(), self.device.index
         self._need = {}
         lib = _native.load()
+        if self.fp8:
+            # the kernels widen e4m3 by moving bits, which has no place for NaN
+            found = torch.zeros(1, dtype=torch.int32, device=self.device)
+            with ws.on_device(self._index) as stream:
+                for w in (w_gate_up, w_down):
+                    _native.check(lib.eux_experts_find_nan(w.data_ptr(), w.numel(), found.data_ptr(), stream), "eux_experts_find_nan")
+                ws.require(int(found.item()) == 0, "e4m3 weights must not be NaN")
         self._room = C.create_string_buffer(256 + 64)
         self._maps = (C.addressof(self._room) + 63) & ~63
         with ws.on_device(self._index):

@@ -53,6 +53,7 @@ def test_launches_refuse_without_a_gpu(native_build):
     for launch, size in ((lib.eux_route_launch, None), (lib.eux_experts_launch, lib.eux_experts_workspace_bytes), (lib.eux_lora_launch, lib.eux_lora_workspace_bytes)):
         assert launch(None, None) == bad
         assert lib.eux_experts_maps(None, None) == bad
+        assert lib.eux_experts_find_nan(None, 16, None, None) == bad
         assert size is None or size(None) == 0
     good = dict(n_tokens=2, n_experts=16, topk=2, dtype=n.DT_F32, groups=1, topk_groups=1)
     for change in (dict(n_experts=0), dict(n_experts=1025), dict(topk=17), dict(topk=33, n_experts=64), dict(groups=3), dict(groups=2, topk_groups=3), dict(dtype=n.DT_F16),
