@@ -2,6 +2,8 @@
 zeroed words for kernels that count their CTAs."""
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _native
@@ -84,6 +86,7 @@ class CallScratch:
         self.words, self.device = words, device
         self._of_stream = {}
         self._captured, self._kept = [], []
+        self._lock = threading.Lock()  # two threads that find nothing for their stream must not both make it
         with on_device(device.index):
             self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0)) if words else []
             torch.cuda.current_stream().synchronize()  # captured calls run on any stream
@@ -94,6 +97,10 @@ class CallScratch:
         if torch._C._cuda_getDevice() != self.device.index:
             with on_device(self.device.index):
                 return self.get(need)
+        with self._lock:
+            return self._get(need)
+
+    def _get(self, need: int):
         stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         if torch._C._cuda_isCurrentStreamCapturing():
             # In a capture a tensor's memory is the graph's; the words are zeroed by the graph itself once those that were
@@ -118,4 +125,3 @@ class CallScratch:
         """Zeroes all words, after a kernel that gave up: with nothing in flight."""
         for t in [m[1] for m in self._of_stream.values()] + self._captured:
             t.zero_()
-

@@ -237,6 +237,31 @@ def test_threads_that_share_a_stream(cuda_device):
         assert len(got[s]) == 50 and all(torch.equal(o, want[s]) for o in got[s])
 
 
+def test_threads_that_call_an_object_for_the_first_time_share_one_workspace(cuda_device):
+    import threading
+    from execution_ucx_b200.ops import _workspace
+    scratch = _workspace.CallScratch(8, cuda_device)
+    made, begin = [], threading.Barrier(8)
+    ordinary = torch.zeros
+
+    def slow(*a, **kw):  # the other threads come while the first is making its words
+        import time
+        time.sleep(0.05)
+        return ordinary(*a, **kw)
+
+    def run():
+        begin.wait()
+        made.append(scratch.get(1 << 16))
+    threads = [threading.Thread(target=run) for _ in range(8)]
+    torch.zeros = slow
+    try:
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        torch.zeros = ordinary
+    assert len(made) == 8 and len(set(made)) == 1
+
+
 def test_captured_calls_replayed_beside_each_other_and_plain_ones(cuda_device):
     from execution_ucx_b200.ops import moe
     layer = moe.MoeExperts(*weights(8, 1024, 256, False, cuda_device))
