@@ -240,7 +240,7 @@ EUX_API int eux_route_preload(void);
 
 /* ---- a whole expert layer for a few tokens (moe_experts.cu) ----
  * out[t] = sum_k topk_w[t,k] * W_down[e] (silu(W_gate[e] x[t]) * (W_up[e] x[t])), e = topk_idx[t,k]; entries with e outside
- * [0, n_experts) add nothing. Two launches; topk_idx and topk_w are read by both. */
+ * [0, n_experts) add nothing. Two launches, with more than eight tokens or a hidden that is no multiple of 128 one more in front. */
 #define EUX_EXPERTS_MAX_TOKENS 128
 #define EUX_EXPERTS_MAX_EXPERTS 1024
 typedef struct eux_experts_desc {

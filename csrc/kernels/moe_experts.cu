@@ -13,18 +13,24 @@
 //   results, it leaves its part in a workspace, and the last to come adds the parts up, in the order of the SMs. For the down
 //   form a tile is 128 rows of the output with all experts, so the weighted sum over a token's experts is made in shared
 //   memory, and only what an SM's share cuts goes through the workspace.
-// * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp the tokens' values beside them
-//   the same way (rows are gathered, four by a copy: any tokens, any order), twelve warps multiply, and two make
-//   results of the sums while those go on. The ring runs on
-//   over the borders of segments; the down form's starts before the up form has ended (programmatic dependent launch), since
-//   weights wait for nobody.
-// * The weights are the first operand of mma.sync m16n8k16 and the tokens the second: 8 columns are the smallest padding for
-//   one token. At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks per block, of which
-//   eight tokens take about 130, so operands through registers cost nothing here, and they let e4m3 weights be multiplied with
-//   bfloat16 tokens: widened on the way, exactly (see widen).
+// * One thread fetches blocks with TMA into a ring of up to a dozen stages, one warp the tokens' values beside them, others
+//   multiply, and others again make results of the sums while those go on. The ring runs on over the borders of segments; the
+//   down form's starts before the up form has ended (programmatic dependent launch), since weights wait for nobody.
+// * An expert's tokens lie side by side, so that one copy takes them: up to eight tokens of the call do as they are (every
+//   token is a column of every product), more are put into the experts' order by a kernel in front, once for both forms.
+// * The weights are the first operand, 128 rows of them, and the tokens the second: a token costs a column and not a row.
+//   With few tokens, and with e4m3 weights, that is mma.sync m16n8k16, whose 8 columns are the smallest padding for one token and whose
+//   operands go through registers, where e4m3 weights are widened to the tokens' bfloat16, exactly (see widen). With bfloat16 weights and
+//   more than kXpFewColumns tokens of an expert it is tcgen05, straight from the stages into TMEM.
 //
-// Sums are float32 throughout. h is rounded to bfloat16, which its product takes; its error, 2^-9 of each term on average, is
-// that of the result's own rounding.
+// At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks for a block. Measured, in a graph, of
+// the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 418 us (1.00), e4m3 247 us (0.84); one
+// token, 8 experts of that size: 115 us (0.93) and 77 us (0.69); one token, 8 experts of 2048 x 768, bf16: 24 us (0.48: two launches'
+// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 161 us (0.76), e4m3 201 us (0.31: widening
+// and mma.sync are the bound, 32 tokens to an expert).
+//
+// Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, which
+// stays below that of the result's own rounding on average.
 #include <cuda.h>
 
 #include <algorithm>
@@ -164,8 +170,7 @@ __device__ __forceinline__ void xp_acc_16(uint32_t at, float (&v)[16]) {  // of 
 // Four e4m3 values as bfloat16, bytes 0 and 2 in `even` and 1 and 3 in `odd`: sign, exponent and mantissa are moved to their places,
 // which gives the value times 2^-120 (the exponents' biases are 7 and 127; subnormal ones stay subnormal), and multiplied by
 // 2^120. Both steps are exact. NaN (0x7f) would become 480: weights with NaN are refused when they are given.
-// The shifts to the left are written as products, which the pipe that multiplies can take: integer logic runs at half of a
-// warp's rate, and with six such instructions for four values instead of eight a block keeps an SM busy for ...
+// The shifts to the left are written as products, which the pipe that multiplies takes: integer logic has half its rate.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd) {
   const uint32_t w4 = w * 16u, w8 = w * 256u, r4 = w >> 4;
   const uint32_t e = (w4 & 0x07f007f0u) | (w8 & 0x80008000u), o = (r4 & 0x07f007f0u) | (w & 0x80008000u);

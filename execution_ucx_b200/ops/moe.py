@@ -163,7 +163,8 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: Op
     With ``groups`` the experts are that many equal runs, and only those of the ``topk_groups`` runs with the largest sum
     of two scores are chosen from. ``renormalize`` divides a token's weights by their sum (a sum of zero gives weights of
     zero), ``scale`` multiplies them. An expert whose logit or bias is -inf or NaN is never chosen; where fewer than
-    ``topk`` are left, the last places are expert -1 with weight 0. A logit of +inf weighs as the largest number does."""
+    ``topk`` are left, the last places are expert -1 with weight 0. A logit of +inf weighs as the largest number does. For
+    inference: the weights have no gradient."""
     global _launches
     ws.require(isinstance(logits, torch.Tensor) and logits.dim() == 2, "logits must be a matrix")
     dtype = logits.dtype
@@ -212,7 +213,8 @@ class MoeExperts:
     (16 for e4m3), e4m3 weights no NaN (checked when they are given).
 
     Made for few tokens, where the layer is as fast as the weights of the named experts can be read: rows beyond
-    ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again."""
+    ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again. For inference: the result has no
+    gradient. An object is made outside of graph captures; its calls may be captured, and made by several threads."""
 
     MAX_TOKENS = 128
     MAX_EXPERTS = 1024
@@ -274,7 +276,8 @@ class MoeExperts:
         per token. An entry whose expert is not in ``[0, experts)`` adds nothing: with the experts of one of several GPUs, pass
         the indices less the number of its first expert, and add up the GPUs' results. A token without entries gets zeros.
         ``out`` may be ``x`` itself; the rows of both may lie apart. Sums are in float32; what lies between the two products is
-        rounded to bfloat16. The same arguments give the same bits."""
+        rounded to bfloat16. The same arguments give the same bits. A wait in the kernels that runs out (two seconds) is told by
+        ``check_status``; the result is none then."""
         global _launches
         index, hidden = self._index, self.hidden
         # what a call usually brings, with as few questions as tell it from everything else
