@@ -276,8 +276,8 @@ struct LoraTile {
   int adapter, first, n;
 };
 __device__ __forceinline__ bool lora_tile(const LoraParams& p, int i, LoraTile* t) {
+  const int4 v = __ldcg(p.tiles + i);  // there is room for one per CTA: fetched together with the number that are filled
   if (i >= __ldcg(p.n_tiles)) return false;
-  const int4 v = __ldcg(p.tiles + i);
   t->adapter = v.x, t->first = v.y, t->n = v.z;
   return true;
 }
@@ -293,16 +293,18 @@ __device__ __forceinline__ float4 lora_ld_cluster(uint32_t at, uint32_t cta) {
   return v;
 }
 
-// R8: ranks in eights, rounded up to a power of two.
-template <int R8>
+// R8: ranks in eights, rounded up to a power of two. WIDE: stages of twice the size, half as many rounds of the CTA, for two CTAs of an SM.
+template <int R8, bool WIDE>
 struct LoraShrink {
-  static constexpr int STAGE = (kLoraTile + R8 * 8) * 128, STAGES = R8 >= 8 ? 3 : 4;
+  static constexpr int STEP = WIDE ? 128 : 64;  // of K in a stage
+  static constexpr int STAGE = (kLoraTile + R8 * 8) * STEP * 2, STAGES = WIDE ? (R8 >= 16 ? 2 : 3) : (R8 >= 8 ? 3 : 4);
   static constexpr int RING = STAGES * STAGE, SUM = kLoraTile * (R8 * 8 + 4) * 4, BYTES = RING > SUM ? RING : SUM;
 };
-template <int R8>
+template <int R8, bool WIDE>
 __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int STEP = 64, PIECES = STEP / 8;  // of K in a stage; 16-byte pieces of a row
-  constexpr int X = kLoraTile * STEP * 2, STAGE = LoraShrink<R8>::STAGE, STAGES = LoraShrink<R8>::STAGES;
+  using S = LoraShrink<R8, WIDE>;
+  constexpr int STEP = S::STEP, PIECES = STEP / 8;  // 16-byte pieces of a row
+  constexpr int X = kLoraTile * STEP * 2, STAGE = S::STAGE, STAGES = S::STAGES;
   constexpr int LD = R8 * 8 + 4;               // floats between the tile's rows when it is added up
   extern __shared__ __align__(1024) unsigned char lora_smem_raw[];
   const eux_lora_desc& d = p.d;
@@ -315,19 +317,19 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   }
   const int k0 = blockIdx.y * p.per_slice, k1 = min(d.k, k0 + p.per_slice), steps = max(0, (k1 - k0 + STEP - 1) / STEP);
   const uint32_t smem = lora_smem(lora_smem_raw);
-  auto place = [](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); };
-  // What this thread fetches of every stage: a piece of each sixteenth row of x and of A.
-  constexpr int XR = kLoraTile / 16, AR = (R8 * 8 + 15) / 16;
+  auto place = [](int row, int piece) { return row * (STEP * 2) + ((piece ^ (row & 7)) << 4); };
+  // What this thread fetches of every stage: a piece of some rows of x and of A.
+  constexpr int ROWS = kLoraThreads / PIECES, XR = kLoraTile / ROWS, AR = (R8 * 8 + ROWS - 1) / ROWS;
   const int row = threadIdx.x / PIECES, piece = threadIdx.x % PIECES;
   const __nv_bfloat16 *x[XR], *a[AR];
 #pragma unroll
   for (int i = 0; i < XR; ++i) {
-    const int r = row + 16 * i;
+    const int r = row + ROWS * i;
     x[i] = r < t.n ? (const __nv_bfloat16*)d.x + p.order[t.first + r] * d.x_stride : nullptr;
   }
 #pragma unroll
   for (int i = 0; i < AR; ++i) {
-    const int r = row + 16 * i;
+    const int r = row + ROWS * i;
     a[i] = r < d.rank ? (const __nv_bfloat16*)d.a + ((int64_t)t.adapter * d.rank + r) * d.k : nullptr;
   }
   auto fetch = [&](int step) {
@@ -337,12 +339,12 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
         const bool some = x[i] && k < k1;
-        lora_cp_16(at + place(row + 16 * i, piece), some ? x[i] + k : (const __nv_bfloat16*)d.x, some);
+        lora_cp_16(at + place(row + ROWS * i, piece), some ? x[i] + k : (const __nv_bfloat16*)d.x, some);
       }
 #pragma unroll
       for (int i = 0; i < AR; ++i) {
         const bool some = a[i] && k < k1;
-        if (row + 16 * i < R8 * 8) lora_cp_16(at + X + place(row + 16 * i, piece), some ? a[i] + k : (const __nv_bfloat16*)d.a, some);
+        if (row + ROWS * i < R8 * 8) lora_cp_16(at + X + place(row + ROWS * i, piece), some ? a[i] + k : (const __nv_bfloat16*)d.a, some);
       }
     }
     lora_cp_commit();
@@ -392,10 +394,13 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   for (int i = threadIdx.x + blockIdx.y * kLoraThreads; i < t.n * q; i += kLoraThreads * slices) {
     const int r = i / q, e = i % q * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < slices; ++s) {
-      const float4 o = lora_ld_cluster(smem + (r * LD + e) * 4, s);
-      v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-    }
+    float4 o[kLoraCluster];  // all under way at once
+#pragma unroll
+    for (int s = 0; s < kLoraCluster; ++s)
+      if (s < slices) o[s] = lora_ld_cluster(smem + (r * LD + e) * 4, s);
+#pragma unroll
+    for (int s = 0; s < kLoraCluster; ++s)
+      if (s < slices) v.x += o[s].x, v.y += o[s].y, v.z += o[s].z, v.w += o[s].w;
     *reinterpret_cast<float4*>(p.v + (int64_t)(t.first + r) * d.rank + e) = v;
   }
   lora_cluster_meets();  // the others have read this one's
@@ -418,11 +423,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   // Shrink was through with its wait for whatever is in front when it let this in: all but v is there, in the L2.
   LoraTile t;
-  if (!lora_tile(p, blockIdx.x, &t)) {
-    wait_for_launch_before();  // what follows in the stream may rely on this kernel for what is in front of it
-    allow_next_launch();
-    return;
-  }
+  if (!lora_tile(p, blockIdx.x, &t)) return;  // the others, there are some, wait for what is in front: whatever follows may rely on that
   const bool has = t.adapter < d.n_adapters;
   const int row0 = warp * 16, n0 = blockIdx.y * p.per_cta, n1 = min(d.n, n0 + p.per_cta), steps = (n1 - n0 + kLoraColumns - 1) / kLoraColumns;
   // this lane's rows: g and g + 8 of the warp's
@@ -535,7 +536,7 @@ static int lora_check(const eux_lora_desc* d) {
 }
 
 struct LoraShape {
-  bool one;
+  bool one, wide;
   int tiles, slices, per_slice, units, parts, per_cta;
   size_t v_bytes, tile_bytes, order_bytes, count_bytes;
 };
@@ -561,11 +562,19 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     // Parts of K and of N that the SMs have places for at once: a second wave that is half empty costs as much as a full one.
     const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile, r = d->rank;
     auto places = [](int smem) { return kSms * (227 * 1024 / (smem + 1024)); };
-    const int shrink = places(r <= 8 ? LoraShrink<1>::BYTES : r <= 16 ? LoraShrink<2>::BYTES : r <= 32 ? LoraShrink<4>::BYTES
-                              : r <= 64 ? LoraShrink<8>::BYTES : LoraShrink<16>::BYTES);
+    const int shrink = places(r <= 8 ? LoraShrink<1, false>::BYTES : r <= 16 ? LoraShrink<2, false>::BYTES : r <= 32 ? LoraShrink<4, false>::BYTES
+                              : r <= 64 ? LoraShrink<8, false>::BYTES : LoraShrink<16, false>::BYTES);
     const int expand = places(r <= 16 ? LoraExpand<1>::BYTES : r <= 32 ? LoraExpand<2>::BYTES : r <= 64 ? LoraExpand<4>::BYTES : LoraExpand<8>::BYTES);
-    int want = std::max(1, std::min({kLoraCluster, shrink / likely, (d->k + 255) / 256}));
-    while (want & (want - 1)) want &= want - 1;  // a cluster
+    auto cluster = [&](int all) {
+      int n = std::max(1, std::min({kLoraCluster, all / likely, (d->k + 255) / 256}));
+      while (n & (n - 1)) n &= n - 1;
+      return n;
+    };
+    // Wide stages where the tiles have places for them even if every adapter has one that is not full (777 tokens, 7168 x 2056, rank 40,
+    // 24 adapters: 19.4 us, 22.5 with narrow ones; 8192 tokens, 4096 x 4096, rank 128: 110 and 113; but 256 tokens with 64 adapters
+    // of rank 64: 33.8 and 31.1). Up to rank 32 a stage is mostly x, and narrow ones are as fast.
+    s.wide = r > 32 && s.tiles * cluster(2 * kSms) <= 2 * kSms;
+    const int want = cluster(s.wide ? 2 * kSms : shrink);
     s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
     s.slices = want;
     const int parts = std::max(1, std::min(expand / likely, (d->n + 127) / 128));
@@ -592,12 +601,12 @@ static int lora_launch(void (*kernel)(LoraParams), dim3 grid, int cluster, size_
   cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
   return (int)cudaLaunchKernelEx(&cfg, kernel, p);
 }
-template <int R8>
+template <int R8, bool WIDE>
 static int lora_shrink(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
-  constexpr size_t smem = LoraShrink<R8>::BYTES;
+  constexpr size_t smem = LoraShrink<R8, WIDE>::BYTES;
   if (smem > 48 * 1024)
-    if (cudaError_t e = allow_smem<lora_shrink_kernel<R8>>(dev, smem); e != cudaSuccess) return (int)e;
-  return lora_launch(lora_shrink_kernel<R8>, dim3(s.tiles, s.slices), s.slices, smem, st, p);
+    if (cudaError_t e = allow_smem<lora_shrink_kernel<R8, WIDE>>(dev, smem); e != cudaSuccess) return (int)e;
+  return lora_launch(lora_shrink_kernel<R8, WIDE>, dim3(s.tiles, s.slices), s.slices, smem, st, p);
 }
 
 template <int K16>
@@ -616,8 +625,10 @@ static int lora_run_one(const LoraParams& p, const LoraShape& s, cudaStream_t st
 }
 static int lora_run_tiles(const LoraParams& p, const LoraShape& s, int dev, cudaStream_t st) {
   const int r = p.d.rank;
-  const int rc = r <= 8 ? lora_shrink<1>(p, s, dev, st) : r <= 16 ? lora_shrink<2>(p, s, dev, st) : r <= 32 ? lora_shrink<4>(p, s, dev, st)
-                 : r <= 64 ? lora_shrink<8>(p, s, dev, st) : lora_shrink<16>(p, s, dev, st);
+  const int rc = r <= 8 ? lora_shrink<1, false>(p, s, dev, st) : r <= 16 ? lora_shrink<2, false>(p, s, dev, st)
+                 : r <= 32 ? lora_shrink<4, false>(p, s, dev, st)
+                 : r <= 64 ? (s.wide ? lora_shrink<8, true>(p, s, dev, st) : lora_shrink<8, false>(p, s, dev, st))
+                           : (s.wide ? lora_shrink<16, true>(p, s, dev, st) : lora_shrink<16, false>(p, s, dev, st));
   if (rc) return rc;
   return r <= 16 ? lora_expand<1>(p, s, dev, st) : r <= 32 ? lora_expand<2>(p, s, dev, st) : r <= 64 ? lora_expand<4>(p, s, dev, st) : lora_expand<8>(p, s, dev, st);
 }
@@ -664,8 +675,9 @@ extern "C" int eux_lora_preload(void) {
   cudaFuncAttributes a;
   const void* kernels[] = {(const void*)lora_shrink_one_kernel, (const void*)lora_expand_one_kernel<1>, (const void*)lora_expand_one_kernel<2>,
                            (const void*)lora_expand_one_kernel<4>, (const void*)lora_expand_one_kernel<8>, (const void*)lora_expand_one_kernel<16>,
-                           (const void*)lora_order_kernel, (const void*)lora_shrink_kernel<1>, (const void*)lora_shrink_kernel<2>,
-                           (const void*)lora_shrink_kernel<4>, (const void*)lora_shrink_kernel<8>, (const void*)lora_shrink_kernel<16>,
+                           (const void*)lora_order_kernel, (const void*)lora_shrink_kernel<1, false>, (const void*)lora_shrink_kernel<2, false>,
+                           (const void*)lora_shrink_kernel<4, false>, (const void*)lora_shrink_kernel<8, false>, (const void*)lora_shrink_kernel<8, true>,
+                           (const void*)lora_shrink_kernel<16, false>, (const void*)lora_shrink_kernel<16, true>,
                            (const void*)lora_expand_kernel<1>, (const void*)lora_expand_kernel<2>, (const void*)lora_expand_kernel<4>, (const void*)lora_expand_kernel<8>};
   for (const void* k : kernels)
     if (cudaError_t e = cudaFuncGetAttributes(&a, k); e != cudaSuccess) return (int)e;

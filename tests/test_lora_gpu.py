@@ -63,6 +63,18 @@ def test_against_plain(cuda_device, t, k, n, rank, count, run):
     assert torch.equal(out, layer(x, ids, y)), "the same arguments give the same bits"
 
 
+@pytest.mark.parametrize("rank", [40, 64, 104, 128])
+@pytest.mark.parametrize("count", [3, 80])
+def test_larger_ranks_with_few_and_with_many_adapters(cuda_device, rank, count):
+    from execution_ucx_b200.ops import lora
+    layer = lora.LoraAdapters(*adapters(count, 2056, 200, rank, cuda_device, seed=rank))
+    g = torch.Generator(device=cuda_device).manual_seed(count)
+    ids = torch.randint(-1, count, (650,), generator=g, device=cuda_device, dtype=torch.int32)
+    x, y = bf(650, 2056, dev=cuda_device), bf(650, 200, dev=cuda_device)
+    out = check(layer, x, ids, y)
+    assert torch.equal(out, layer(x, ids, y))
+
+
 @pytest.mark.parametrize("t", [1, 40, 300])
 def test_tokens_without_an_adapter(cuda_device, t):
     from execution_ucx_b200.ops import lora
