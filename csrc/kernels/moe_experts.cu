@@ -26,7 +26,7 @@
 // At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks for a block. Measured, in a graph, of
 // the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 418 us (1.00), e4m3 247 us (0.84); one
 // token, 8 experts of that size: 115 us (0.93) and 77 us (0.69); one token, 8 experts of 2048 x 768, bf16: 24 us (0.48: two launches'
-// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 161 us (0.76), e4m3 201 us (0.31: widening
+// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 161 us (0.76), e4m3 200 us (0.31: widening
 // and mma.sync are the bound, 32 tokens to an expert).
 //
 // Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, which
@@ -463,7 +463,7 @@ __device__ __forceinline__ void xp_segment(XpRing& ring, int& mine, int end, int
           for (int j = 0; j < NB; ++j) {
             uint32_t x0, x1;
             const int st = step + ks;
-            lds_64(x0, x1, x + (st >> 2) * (NB * 1024) + (j * 8 + column(g)) * 128 + ((((st & 3) * 2 + (c >> 1)) ^ column(g)) << 4) + (c & 1) * 8);
+            lds_64(x0, x1, x + (st >> 2) * ((NB == 3 ? 4 : NB) * 1024) + (j * 8 + column(g)) * 128 + ((((st & 3) * 2 + (c >> 1)) ^ column(g)) << 4) + (c & 1) * 8);
             const uint32_t b0 = __byte_perm(x0, x1, 0x5410), b1 = __byte_perm(x0, x1, 0x7632);
 #pragma unroll
             for (int m = 0; m < 2; ++m) mma_bf16(part[m][j], wa[m][0], wa[m][1], wa[m][2], wa[m][3], b0, b1);
@@ -842,7 +842,10 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
       if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
       else if (!FP8 || nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
-      else if constexpr (FP8) xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      else if constexpr (FP8) {  // 32 tokens at most; three eights are worth a form of their own (64 tokens, 8 experts of 4096 x 8192: 209 us, 231 without)
+        if (nb == 3) xp_segment<FP8, DOWN, 3>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+        else xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
+      }
       if (++sum_at == n_sums) sum_at = 0, sum_ph ^= 1u;
       b = end;
     }

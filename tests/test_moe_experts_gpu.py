@@ -104,6 +104,18 @@ def test_all_tokens_to_one_expert_and_the_same_expert_twice(cuda_device, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [7, 8, 9, 15, 16, 17, 24, 25, 31, 32, 33, 45, 48, 49, 63, 64, 65, 97, 128])
+def test_every_number_of_tokens_that_an_expert_can_have(cuda_device, fp8, t):
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(3, 272, 208, fp8, cuda_device))
+    idx = torch.ones(t, 1, dtype=torch.int32, device=cuda_device)
+    idx[:2] = 2  # and another expert with two
+    x = torch.randn(t, 272, device=cuda_device).to(torch.bfloat16)
+    check(layer, x, idx, torch.rand(t, 1, device=cuda_device))
+    layer.check_status()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_entries_without_an_expert(cuda_device, fp8):
     from execution_ucx_b200.ops import moe
     layer = moe.MoeExperts(*weights(6, 256, 144, fp8, cuda_device))
