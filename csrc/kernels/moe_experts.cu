@@ -58,7 +58,7 @@ constexpr int kXpSumBars = 96;                      // bytes: for each of two su
 constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
 constexpr int kXpMaxGrid = 160;
 constexpr size_t kXpDynamic = 226 * 1024;           // shared memory of a launch; the kernel declares a little more itself
-constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer cost more to add up than they save
+constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer cost more to add up than they save; none may cost more than all of these (xp_cost)
 
 struct XpParams {
   eux_experts_desc d;
@@ -74,7 +74,7 @@ struct XpParams {
 // Shared memory: the ring of weights (128-byte swizzle: on 1024 bytes), behind it the tokens' values of each stage, the sums
 // of a segment (tcgen05) or of two; from the end the parts whose sizes the launch knows. How many tokens a segment takes (`cap`), and with it how
 // many stages there is room for, is known when the entries have been counted.
-__host__ __device__ inline int xp_table_bytes(int n_experts, int entries) { return ((n_experts + 1) * 8 + entries * 8 + 31) & ~15; }
+__host__ __device__ inline int xp_table_bytes(int n_experts, int entries) { return ((n_experts + 1) * 10 + entries * 8 + 31) & ~15; }
 struct XpLayout {
   int acc, scales, bars, tables;  // from the beginning
   int room;                       // bytes in front of these
@@ -183,10 +183,12 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& even, uint32_t& odd)
 //   start[a]   where the entries of the a-th named expert begin in `order` (the experts in order, entries of one in order)
 //   first[a]   number of the first chunk (of up to `cap` entries) of that expert; first[named] is their number
 //   expert[a]
+//   cost[a]    what the chunks in front of that expert cost; only where they are made uneven (XpLine)
 struct XpTables {
   int* start;        // [named + 1]
   uint16_t* first;   // [named + 1]
   uint16_t* expert;  // [named]
+  uint16_t* cost;    // [named + 1]
   uint16_t* order;   // [entries]
   uint16_t* token;   // [entries]: of order
   float* weight;     // [entries]: of order
@@ -195,11 +197,35 @@ struct XpTables {
     start = reinterpret_cast<int*>(at);
     first = reinterpret_cast<uint16_t*>(start + n_experts + 1);
     expert = first + n_experts + 1;
-    order = expert + n_experts + 1;
+    cost = expert + n_experts + 1;
+    order = cost + n_experts + 1;
     token = order + entries;
     weight = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(token + entries) + 3) & ~(uintptr_t)3);
   }
 };
+
+// What a block of e4m3 weights costs an SM with so many eights of tokens, in quarters of what its bytes take; with more than one it is
+// the products that count. Tried: 4, 4, 7, 9 and 4, 5, 8, 11 and 4, 4, 6, 8 (2 to 4 % slower over the sizes below).
+__device__ __forceinline__ int xp_cost(int eights) { return eights <= 1 ? 4 : eights == 2 ? 5 : eights == 3 ? 7 : 9; }
+__device__ __forceinline__ void xp_costs(XpTables& r, int lane) {  // by a warp
+  int all = 0;
+  for (int a0 = 0; a0 < r.named; a0 += 32) {
+    const int a = a0 + lane;
+    int c = 0;
+    if (a < r.named) {
+      const int count = r.start[a + 1] - r.start[a], chunks = r.first[a + 1] - r.first[a];
+      c = chunks * xp_cost(((count + chunks - 1) / chunks + 7) >> 3);
+    }
+    int sum = c;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    if (a < r.named) r.cost[a] = (uint16_t)(all + sum - c);
+    all += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) r.cost[r.named] = (uint16_t)all;
+}
 
 struct XpSegment {
   int expert, tile, pos, n;
@@ -358,13 +384,54 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
   return cap;
 }
 
-// Equal shares of the line of blocks, the first `more` of them one longer. (A line has fewer than 2^31 blocks: 180 GB of weights are
-// 12 million, and no expert has more than 128 chunks.)
+// Equal shares of a line, the first `more` of them one longer. (A line is shorter than 2^31: 180 GB of weights are 12 million blocks
+// that cost 9 at most, and no expert has more than 128 chunks.)
 struct XpShares {
   int each, more;
-  __device__ XpShares(int blocks, int grid) : each(blocks / grid), more(blocks % grid) {}
+  __device__ XpShares(int length, int grid) : each(length / grid), more(length % grid) {}
   __device__ int begin(int i) const { return i * each + min(i, more); }
-  __device__ int owner(int block) const { return block < more * (each + 1) ? block / (each + 1) : more + (block - more * (each + 1)) / each; }
+  __device__ int owner(int at) const { return at < more * (each + 1) ? at / (each + 1) : more + (at - more * (each + 1)) / each; }
+};
+
+// The line that is shared out: of blocks, or where e4m3 weights meet experts of more than 8 tokens, of what the blocks cost. An expert's
+// blocks stand side by side, so that in equal numbers a few SMs would get all the dear ones, and the others wait (128 tokens, top-8 of 256
+// experts of 7168 x 2048, of which 23 to 25 of this GPU's 32: one has 17 tokens, 225 us, 289 by number; two have 9 or 10, 210 and 221; 64
+// tokens, top-2 of 8 experts of 4096 x 8192: 196 and 209). A block belongs to the share in which it begins; with kXpMinBlocks to a share
+// each has one.
+template <bool FP8, bool DOWN>
+struct XpLine {
+  const XpTables& r;
+  int tiles, nk;
+  bool by_cost;
+  __device__ int each(int a) const { return (r.cost[a + 1] - r.cost[a]) / (r.first[a + 1] - r.first[a]); }
+  __device__ int length() const { return tiles * nk * (FP8 && by_cost ? r.cost[r.named] : r.first[r.named]); }
+  // The first block that begins at `at` or behind it. By whole warps.
+  __device__ int block(int at) const {
+    if (!FP8 || !by_cost) return at;
+    const int all = r.first[r.named], lane = threadIdx.x & 31;
+    if (at >= length()) return tiles * nk * all;
+    const int of_tile = nk * r.cost[r.named], tile = DOWN ? at / of_tile : 0, unit = DOWN ? nk : nk * tiles;
+    at -= tile * of_tile;
+    int a = 0;
+    for (;; a += 32) {
+      const uint32_t behind = __ballot_sync(0xffffffffu, a + lane < r.named && unit * r.cost[min(a + lane, r.named - 1) + 1] > at);
+      if (behind) {
+        a += __ffs(behind) - 1;
+        break;
+      }
+    }
+    const int c = each(a);
+    return nk * tile * all + unit * r.first[a] + (at - unit * r.cost[a] + c - 1) / c;
+  }
+  // Where the first and the last block of a tile of results begin; up: a tile is a segment, of the a-th expert.
+  __device__ int tile_first(int tile, int a) const {
+    if (!FP8 || !by_cost) return tile * nk * (DOWN ? r.first[r.named] : 1);
+    return DOWN ? tile * nk * r.cost[r.named] : nk * (tiles * r.cost[a] + (tile - tiles * r.first[a]) * each(a));
+  }
+  __device__ int tile_last(int tile, int a) const {
+    if (!FP8 || !by_cost) return (tile + 1) * nk * (DOWN ? r.first[r.named] : 1) - 1;
+    return DOWN ? (tile + 1) * nk * r.cost[r.named] - each(r.named - 1) : tile_first(tile, a) + (nk - 1) * each(a);
+  }
 };
 
 // Of the tokens' values (up) or h (down), by the rows of a copy: 8, 16, 32 and 64.
@@ -592,10 +659,11 @@ __device__ __forceinline__ void xp_tile_end(const XpParams& p, const XpTables& r
 }
 
 // What the warps that see to the results do.
-template <bool DOWN>
+template <bool FP8, bool DOWN>
 struct XpResults {
   const XpParams& p;
   const XpTables& r;
+  const XpLine<FP8, DOWN>& line;
   const XpShares& shares;
   int b0, b1, seg0, nk, chunks, me;
   bool in_place;
@@ -672,7 +740,8 @@ struct XpResults {
         // the end of a tile, or of this SM's part of it
         end_warps_meet<TC>();  // what they have put together is complete
         if (b == b1) break;    // the end of the share is everybody's
-        xp_tile_end<DOWN, THREADS>(p, r, s, shares.owner(tile0), shares.owner(tile1 - 1), me, DOWN ? acc : sum, in_place, tid, s_last, end_warps_meet<TC>);
+        xp_tile_end<DOWN, THREADS>(p, r, s, shares.owner(line.tile_first(tile, walk.a)), shares.owner(line.tile_last(tile, walk.a)), me, DOWN ? acc : sum, in_place, tid, s_last,
+                                     end_warps_meet<TC>);
         end_warps_meet<TC>();  // and is written over next
         if (b == tile1) ++tile;
       }
@@ -747,8 +816,9 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   const int blocks = tiles * chunks * nk;
   const int grid = min((int)gridDim.x, max(1, blocks / kXpMinBlocks));
   const int me = blockIdx.x;
-  const XpShares shares(blocks, grid);
-  const int b0 = me < grid ? shares.begin(me) : blocks, b1 = me < grid ? shares.begin(me + 1) : blocks;
+  const XpLine<FP8, DOWN> line{r, tiles, nk, FP8 && p.tables && cap > 8};
+  const XpShares shares(line.length(), grid);
+  const int b0 = me < grid ? line.block(shares.begin(me)) : blocks, b1 = me < grid ? line.block(shares.begin(me + 1)) : blocks;
   const int seg0 = b0 / nk, kb0 = b0 - seg0 * nk;  // the segment that the share begins in, and where
   float* const sums = reinterpret_cast<float*>(xp_smem + ring.stages * (kXpBlock + ring.x_bytes));
   const int n_sums = xp_sums(FP8, columns);
@@ -842,7 +912,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
       const uint32_t bars = sum_bars + sum_at * 8 * (kXpGroups + 1);
       if (nb <= 1) xp_segment<FP8, DOWN, 1>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
       else if (!FP8 || nb <= 2) xp_segment<FP8, DOWN, 2>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
-      else if constexpr (FP8) {  // 32 tokens at most; three eights are worth a form of their own (64 tokens, 8 experts of 4096 x 8192: 209 us, 231 without)
+      else if constexpr (FP8) {  // 32 tokens at most; three eights are worth a form of their own (64 tokens, top-2 of 8 experts of 4096 x 8192: 209 us, 231 without)
         if (nb == 3) xp_segment<FP8, DOWN, 3>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
         else xp_segment<FP8, DOWN, 4>(ring, mine, end, up_border, sum, bars, sum_ph, warp, lane, abort, d.wait_timeout_ns);
       }
@@ -882,16 +952,16 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
     }
   } else if (!tc || warp < kXpEndThreads<true> / 32) {
     if (DOWN) wait_for_launch_before();
-    const XpResults<DOWN> results{p, r, shares, b0, b1, seg0, nk, chunks, me, in_place, columns, sums, acc, &s_last, abort};
+    const XpResults<FP8, DOWN> results{p, r, line, shares, b0, b1, seg0, nk, chunks, me, in_place, columns, sums, acc, &s_last, abort};
     if (!tc) results.template make<false>(walk, sum_bars, 0, threadIdx.x - kXpWarps * 32);
     else if constexpr (!FP8) results.template make<true>(walk, tc_bars, s_acc, threadIdx.x);
   }
   xp_fence_before();
   __syncthreads();
   if (b0 < b1) {
-    const int seg = (b1 - 1) / nk, tile_segs = DOWN ? chunks : 1, tile = seg / tile_segs, tile0 = tile * tile_segs * nk;
+    const int seg = (b1 - 1) / nk, tile = DOWN ? seg / chunks : seg;
     const XpSegment s = walk.at(seg);
-    xp_tile_end<DOWN, kXpThreads>(p, r, s, shares.owner(tile0), shares.owner(tile0 + tile_segs * nk - 1), me,
+    xp_tile_end<DOWN, kXpThreads>(p, r, s, shares.owner(line.tile_first(tile, walk.a)), shares.owner(line.tile_last(tile, walk.a)), me,
                                   DOWN ? acc : sums + (seg - seg0) % n_sums * columns * kXpLd, in_place, threadIdx.x, &s_last, cta_meets);
   }
   if (!FP8 && tc && warp == kProducts) {
@@ -913,6 +983,10 @@ __global__ void __launch_bounds__(kXpThreads) moe_experts_sort_kernel(const __gr
   XpTables r(xp_smem, d.n_experts, entries);
   const int cap = xp_route(d, p.token_of, most, r, reinterpret_cast<int*>(xp_smem + bytes), s_route);
   if (blockIdx.x == 0) {
+    if (d.fp8 && cap > 8) {
+      if (threadIdx.x < 32) xp_costs(r, threadIdx.x);
+      __syncthreads();
+    }
     for (int i = threadIdx.x; i < bytes / 16; i += kXpThreads) reinterpret_cast<uint4*>(p.tables + 4)[i] = reinterpret_cast<const uint4*>(xp_smem)[i];
     if (threadIdx.x == 0) p.tables[0] = (uint32_t)r.named, p.tables[1] = (uint32_t)cap;
   }

@@ -9,6 +9,9 @@
                                                                            gemm_mx_pull, gemm_fp8_pull: the same for the fp8 kernels)
     python -m execution_ucx_b200.models.profile_case --kernel xfer_peer   (two GPUs, one process: the transfer kernel on GPU 0 writes into GPU 1's memory)
     python -m execution_ucx_b200.models.profile_case --kernel xfer_gather (a transposed matrix gathered into a dense buffer)
+    python -m execution_ucx_b200.models.profile_case --kernel experts     (an expert layer, 64 tokens; experts_fp8: e4m3 weights)
+    python -m execution_ucx_b200.models.profile_case --kernel lora        (adapters of 4096 tokens; lora_few: of 64 tokens)
+    python -m execution_ucx_b200.models.profile_case --kernel route       (choice of experts within groups, 4096 tokens)
 
 Each case keeps well under a few GB on the device, uses inputs larger than L2
 where DRAM figures matter, and launches the kernel of interest a handful of times.
@@ -22,7 +25,7 @@ import torch
 
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("--kernel", choices=["gemm", "gemm_1cta", "gemm_few", "gemm_fp8", "gemm_mx", "xfer", "pull_batch", "moe", "moe_fp8", "gemm_pull", "gemm_mx_pull", "gemm_fp8_pull", "xfer_peer", "xfer_gather"], required=True)
+    ap.add_argument("--kernel", choices=["gemm", "gemm_1cta", "gemm_few", "gemm_fp8", "gemm_mx", "xfer", "pull_batch", "moe", "moe_fp8", "gemm_pull", "gemm_mx_pull", "gemm_fp8_pull", "xfer_peer", "xfer_gather", "experts", "experts_fp8", "lora", "lora_few", "route"], required=True)
     ap.add_argument("--iters", type=int, default=3)
     args = ap.parse_args()
     dev = torch.device("cuda", 0)
@@ -125,6 +128,37 @@ def main() -> None:
             g(xq.data_ptr(), xc.data_ptr(), m, y.data_ptr(), x_is_local=True)
         torch.cuda.synchronize()
         g.check_status()
+    elif args.kernel in ("experts", "experts_fp8"):
+        from ..ops import moe
+        t, h, i, e, k = 64, 4096, 8192, 8, 2  # 1.6 GB of bfloat16 weights, half of that in e4m3; 16 tokens to an expert
+        if args.kernel == "experts_fp8":
+            quantized = lambda *shape: torch.randint(0, 120, shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)  # noqa: E731
+            layer = moe.MoeExperts(quantized(e, 2 * i, h), quantized(e, h, i), torch.full((e, 2 * i // 128, h // 128), 1e-4, device=dev),
+                                   torch.full((e, h // 128, i // 128), 1e-4, device=dev))
+        else:
+            layer = moe.MoeExperts(torch.randn(e, 2 * i, h, dtype=torch.bfloat16, device=dev) * 0.02, torch.randn(e, h, i, dtype=torch.bfloat16, device=dev) * 0.02)
+        x = torch.randn(t, h, device=dev).to(torch.bfloat16)
+        idx, w = moe.route(torch.randn(t, e, device=dev), k)
+        for _ in range(args.iters):
+            layer(x, idx, w)
+        torch.cuda.synchronize()
+        layer.check_status()
+    elif args.kernel in ("lora", "lora_few"):
+        from ..ops import lora
+        t, run = (64, 1) if args.kernel == "lora_few" else (4096, 500)
+        k, n, rank, count = 8192, 8192, 16, 64
+        adapters = lora.LoraAdapters(torch.randn(count, rank, k, device=dev).to(torch.bfloat16), torch.randn(count, n, rank, device=dev).to(torch.bfloat16))
+        ids = torch.randint(0, count, (-(-t // run),), device=dev, dtype=torch.int32).repeat_interleave(run)[:t].contiguous()
+        x, y = torch.randn(t, k, device=dev).to(torch.bfloat16), torch.randn(t, n, device=dev).to(torch.bfloat16)
+        for _ in range(args.iters):
+            adapters(x, ids, y)
+        torch.cuda.synchronize()
+    elif args.kernel == "route":
+        from ..ops import moe
+        logits, bias = torch.randn(4096, 256, device=dev), torch.randn(256, device=dev) * 0.05
+        for _ in range(args.iters):
+            moe.route(logits, 8, scoring="sigmoid", bias=bias, groups=8, topk_groups=4)
+        torch.cuda.synchronize()
     elif args.kernel == "xfer":
         from ..ops import tensor_xfer as tx
         n = 256 << 20  # 256 MiB source + 256 MiB destination

@@ -116,6 +116,24 @@ def test_every_number_of_tokens_that_an_expert_can_have(cuda_device, fp8, t):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("counts", [(128, 1, 1, 1), (20, 9, 3, 33, 1, 0, 17, 8), (12,) + (1,) * 39, (1,) * 39 + (64,), (40, 128, 100, 70)])
+def test_experts_with_very_different_numbers_of_tokens(cuda_device, fp8, counts):
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(len(counts), 400, 336, fp8, cuda_device))
+    idx = torch.full((128, 4), -1, dtype=torch.int32)
+    at = 0
+    for e, n in enumerate(counts):  # entries one after the other, the tokens in turn
+        for j in range(n):
+            idx[at % 128, at // 128] = e
+            at += 1
+    idx = idx[torch.randperm(128, generator=torch.Generator().manual_seed(at))].to(cuda_device)
+    x, w = torch.randn(128, 400, device=cuda_device).to(torch.bfloat16), torch.rand(128, 4, device=cuda_device)
+    out = check(layer, x, idx, w)
+    assert torch.equal(out, layer(x, idx, w))
+    layer.check_status()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_entries_without_an_expert(cuda_device, fp8):
     from execution_ucx_b200.ops import moe
     layer = moe.MoeExperts(*weights(6, 256, 144, fp8, cuda_device))
