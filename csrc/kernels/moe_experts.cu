@@ -24,9 +24,9 @@
 //   more than kXpFewColumns tokens of an expert it is tcgen05, straight from the stages into TMEM.
 //
 // At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks for a block. Measured, in a graph, of
-// the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 418 us (1.00), e4m3 247 us (0.84); one
-// token, 8 experts of that size: 115 us (0.93) and 77 us (0.69); one token, 8 experts of 2048 x 768, bf16: 24 us (0.48: two launches'
-// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 161 us (0.76), e4m3 200 us (0.31: widening
+// the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 423 us (0.99), e4m3 252 us (0.83); one
+// token, 8 experts of that size: 116 us (0.93) and 78 us (0.69); one token, 8 experts of 2048 x 768, bf16: 24 us (0.48: two launches'
+// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 162 us (0.76), e4m3 195 us (0.32: widening
 // and mma.sync are the bound, 32 tokens to an expert).
 //
 // Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, which

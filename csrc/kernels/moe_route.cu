@@ -9,7 +9,9 @@
 // and nothing is rounded before the choice. With them, scores and sums are computed in 64 bits: two experts whose scores
 // differ by less than an fp32 rounding are told apart, and the choice does not depend on the order of a sum.
 // A logit or bias of -inf or NaN takes its expert out; where fewer than k are left, the rest of the row is (-1, 0).
-// Bound by latency: a token is a chain of k warp maxima; the reads (1 KiB per token at E = 256) are never the limit.
+// Bound by latency: a token is a chain of k warp maxima; the reads (1 KiB per token at E = 256) are never the limit. With many tokens and groups it
+// is issue slots, mostly the 64-bit exponentials (46 %). Measured, 256 experts, top-8: one token 3.9 us in a graph; 4096 tokens within 4 of 8
+// groups 16.3 us.
 #include <type_traits>
 
 #include "eux_device.cuh"
