@@ -19,7 +19,7 @@
 //   for all four warps, of y a lane fetches what it will need itself.
 //
 // Measured, in a graph: one token, 4096 x 4096, rank 16: 3.8 us; 64 tokens, 8192 x 8192, rank 16, an adapter each: 13.5 us; 777 tokens, 7168 x
-// 2056, rank 40: 19.0 us (3.6 at the measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 86.5
+// 2056, rank 40: 18.2 us (3.6 at the measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 85.6
 // us (62 at the copy rate).
 #include <algorithm>
 #include <mutex>
@@ -32,7 +32,7 @@ constexpr int kLoraPlain = 512;       // tokens up to which each may stand for i
 constexpr int64_t kLoraPlainBytes = int64_t(64) << 20;  // ... if the adapters that they read then come to no more than this
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
-constexpr int kLoraColumns = 64;      // of N in a stage of expand
+constexpr int kLoraColumns = 128;     // of N in a stage of expand (8192 tokens, 4096 x 4096, rank 64: 66.9 us, 70.0 with 64 columns and three or four stages)
 constexpr int kLoraMaxSlices = 32;    // parts of K of a token
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
@@ -411,13 +411,13 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   if (R8 >= 16) allow_next_launch();
 }
 
-// K16: ranks in 16s, rounded up to a power of two. Columns go 64 at a time, in two runs of 32. A lane's eight columns of a run lie side
+// K16: ranks in 16s, rounded up to a power of two. Columns go 128 at a time, in runs of 32. A lane's eight columns of a run lie side
 // by side, so that y and out are moved 16 bytes at a time: column 2c + i of the product's j-th eight is column 8c + 2j + i of the run,
 // and the rows of B lie in shared memory in the product's order.
 template <int K16>
 struct LoraExpand {
   static constexpr int PITCH = K16 * 32 + 16;  // bytes between rows of B: eight rows on different banks
-  static constexpr int B = kLoraColumns * PITCH, Y = 4 * kLoraThreads * 16, STAGE = B + Y, STAGES = K16 >= 4 ? 3 : 4, BYTES = STAGES * STAGE;
+  static constexpr int B = kLoraColumns * PITCH, Y = kLoraTile * kLoraColumns * 2, STAGE = B + Y, STAGES = 2, BYTES = STAGES * STAGE;
 };
 template <int K16>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_constant__ LoraParams p) {
@@ -452,14 +452,14 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
 #pragma unroll
         for (int i = threadIdx.x; i < kLoraColumns * PIECES; i += kLoraThreads) {
           const int place = i / PIECES, piece = i % PIECES, in = place & 7, eight = place >> 3 & 3;
-          const int col = n + (place & 32) + (in >> 1) * 8 + eight * 2 + (in & 1);
+          const int col = n + (place & ~31) + (in >> 1) * 8 + eight * 2 + (in & 1);
           const bool some = col < n1 && piece * 8 < d.rank;
           lora_cp_16(at + place * S::PITCH + piece * 16, some ? b + (int64_t)col * d.rank + piece * 8 : b, some);
         }
       }
       // y: what this lane needs itself
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < kLoraColumns / 16; ++q) {
         const int h = q & 1, col = n + (q >> 1) * 32 + c * 8;
         if (row[h] && col < n1) lora_cp_16(at + S::B + (q * kLoraThreads + threadIdx.x) * 16, y_row[h] + col, true);
       }
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
     const uint32_t at = smem + s % S::STAGES * S::STAGE;
     if (row0 < t.n) {
 #pragma unroll
-      for (int run = 0; run < 2; ++run) {
+      for (int run = 0; run < kLoraColumns / 32; ++run) {
         float acc[4][4] = {};
         if (has) {
 #pragma unroll
@@ -564,7 +564,9 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     s.per_cta = width * passes;
   } else {
     // Parts of K and of N that the SMs have places for at once: a second wave that is half empty costs as much as a full one.
-    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile, r = d->rank;
+    // How many tiles there will be is not known here: taken to be the tokens' and half a tile for each adapter, of those that can have some (256
+    // tokens, 64 adapters, 8192 x 8192, rank 16: 24.6 us, 28.1 without; 1500 tokens of 16 adapters 21.5 and 24.2; but 1000 of 16 22.0 and 20.4).
+    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile + std::min(d->n_adapters, d->n_tokens / 16) / 2, r = d->rank;
     auto places = [](int smem) { return kSms * (227 * 1024 / (smem + 1024)); };
     const int shrink = places(r <= 8 ? LoraShrink<1, false>::BYTES : r <= 16 ? LoraShrink<2, false>::BYTES : r <= 32 ? LoraShrink<4, false>::BYTES
                               : r <= 64 ? LoraShrink<8, false>::BYTES : LoraShrink<16, false>::BYTES);
