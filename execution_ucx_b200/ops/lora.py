@@ -62,18 +62,25 @@ class LoraAdapters:
         token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``; the rows
         of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
         global _launches
-        if not (isinstance(x, torch.Tensor) and isinstance(ids, torch.Tensor) and isinstance(y, torch.Tensor)
+        K, N = self.K, self.N
+        # what a call usually brings, with as few questions as tell it from everything else
+        if (isinstance(x, torch.Tensor) and isinstance(ids, torch.Tensor) and isinstance(y, torch.Tensor)
                 and x.dtype is torch.bfloat16 and y.dtype is torch.bfloat16 and ids.dtype is torch.int32
-                and x.dim() == y.dim() == 2 and ids.dim() == 1 and x.shape[0] == y.shape[0] == ids.shape[0]
-                and x.shape[1] == self.K and y.shape[1] == self.N and x.is_contiguous() and y.is_contiguous() and ids.is_contiguous()
+                and ids.dim() == 1 and x.shape == (t := ids.numel(), K) and y.shape == (t, N)
+                and x.is_contiguous() and y.is_contiguous() and ids.is_contiguous()
                 and (x.data_ptr() | y.data_ptr()) % 16 == 0 and x.get_device() == y.get_device() == ids.get_device() == self._index):
-            self._require(x, ids, y)
-        t = ids.shape[0]
-        if out is None:
-            out = torch.empty_strided((t, self.N), (self.N, 1), dtype=torch.bfloat16, device=self.device)
+            xs, ys = K, N
         else:
-            ws.require_rows(out, "out", torch.bfloat16, cols=self.N, rows=t)
+            self._require(x, ids, y)
+            t, xs, ys = ids.shape[0], ws.row_stride(x), ws.row_stride(y)
+        if out is None:
+            out, os_ = torch.empty_strided((t, N), (N, 1), dtype=torch.bfloat16, device=self.device), N
+        elif out is y:
+            os_ = ys
+        else:
+            ws.require_rows(out, "out", torch.bfloat16, cols=N, rows=t)
             ws.require_device(self.device, out=out)
+            os_ = ws.row_stride(out)
         if t == 0:
             return out
         lib = _native.load()
@@ -81,7 +88,7 @@ class LoraAdapters:
         if need is None:
             need = self._need[t] = int(lib.eux_lora_workspace_bytes(self._desc(t)))
         workspace, _ = self._scratch.get(need)
-        desc = self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, ws.row_stride(x), ws.row_stride(y), ws.row_stride(out))
+        desc = self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, xs, ys, os_)
         ws.launch(lib.eux_lora_launch, desc, self._index, "eux_lora_launch")
         _launches += 2 if t <= 512 and t * self.rank * (self.K + self.N) * 2 <= 64 << 20 else 3  # as the launch chooses
         return out

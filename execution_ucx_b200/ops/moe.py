@@ -281,21 +281,25 @@ class MoeExperts:
         global _launches
         index, hidden = self._index, self.hidden
         # what a call usually brings, with as few questions as tell it from everything else
-        if not (isinstance(x, torch.Tensor) and isinstance(topk_idx, torch.Tensor) and isinstance(topk_w, torch.Tensor)
+        if (isinstance(x, torch.Tensor) and isinstance(topk_idx, torch.Tensor) and isinstance(topk_w, torch.Tensor)
                 and x.dtype is torch.bfloat16 and topk_idx.dtype is torch.int32 and topk_w.dtype is torch.float32
-                and x.dim() == topk_idx.dim() == 2 and topk_idx.shape == topk_w.shape and x.shape[0] == topk_idx.shape[0]
-                and x.shape[1] == hidden and 1 <= topk_idx.shape[1] <= 32
+                and topk_idx.dim() == 2 and (shape := topk_idx.shape) == topk_w.shape and x.shape == (shape[0], hidden) and 1 <= shape[1] <= 32
                 and x.is_contiguous() and topk_idx.is_contiguous() and topk_w.is_contiguous() and x.data_ptr() % 16 == 0
                 and x.get_device() == topk_idx.get_device() == topk_w.get_device() == index):
+            xs = hidden
+        else:
             self._require(x, topk_idx, topk_w)
-        t, topk = topk_idx.shape
+            shape, xs = topk_idx.shape, ws.row_stride(x)
+        t, topk = shape
         if out is None:
-            out = torch.empty_strided((t, hidden), (hidden, 1), dtype=torch.bfloat16, device=self.device)
+            out, os_ = torch.empty_strided((t, hidden), (hidden, 1), dtype=torch.bfloat16, device=self.device), hidden
+        elif out is x:
+            os_ = xs
         else:
             ws.require_rows(out, "out", torch.bfloat16, cols=hidden, rows=t)
             ws.require_device(self.device, out=out)
+            os_ = ws.row_stride(out)
         lib = _native.load()
-        xs, os_ = ws.row_stride(x), ws.row_stride(out)
         for first in range(0, t, self.MAX_TOKENS):
             n = min(self.MAX_TOKENS, t - first)
             need = self._need.get((n, topk))
