@@ -190,7 +190,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
       else s = d.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - peak) / sum;
     }
     if (d.renormalize) {
-      const Real all = warp_sum(s);
+      Real all = warp_sum(s);
+      if (!WIDE && d.sigmoid && all < 1e-30f) {
+        // All too small for 32 bits: there e^v is the sigmoid to the last bit, and e^(v - the largest v) has the same proportions. What 1 / (1 +
+        // e^-v) has no number for in 64 bits either, where e^-v has none, weighs nothing.
+        const float v = mine >= 0 ? route_logit(d, t, mine) : -INFINITY, first = __shfl_sync(0xffffffffu, v, 0);
+        s = v > -709.78f ? (Real)expf(v - first) : (Real)0;
+        all = warp_sum(s);
+      }
       s = all > 0 ? s / all : (Real)0;  // none taken, or every score too small for a number: no weight
     }
     if (lane < d.topk) {

@@ -161,8 +161,8 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", bias: Op
     ``logits`` is ``[tokens, experts]``, float32 or bfloat16; its rows may lie apart. Scores are the softmax over all
     experts or the sigmoid of each. ``bias`` (float32, ``[experts]``) is added for the choice and left out of the weights.
     With ``groups`` the experts are that many equal runs, and only those of the ``topk_groups`` runs with the largest sum
-    of two scores are chosen from. ``renormalize`` divides a token's weights by their sum (a sum of zero gives weights of
-    zero), ``scale`` multiplies them. An expert whose logit or bias is -inf or NaN is never chosen; where fewer than
+    of two scores are chosen from. ``renormalize`` divides a token's weights by their sum (one that is zero in 64 bits gives weights
+    of zero), ``scale`` multiplies them. An expert whose logit or bias is -inf or NaN is never chosen; where fewer than
     ``topk`` are left, the last places are expert -1 with weight 0. A logit of +inf weighs as the largest number does. For
     inference: the weights have no gradient."""
     global _launches

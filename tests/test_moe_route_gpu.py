@@ -100,12 +100,17 @@ def test_infinite_logits_share_the_weight(cuda_device):
     assert idx.tolist() == [[1, 3, 2]] and w.tolist() == [[0.5, 0.5, 0.0]]
 
 
-def test_scores_too_small_for_a_number_have_no_weight(cuda_device):
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("low", [-90.0, -200.0, -700.0, -800.0, -3e38])
+def test_scores_too_small_for_a_number_of_64_bits_have_no_weight(cuda_device, wide, low):
     from execution_ucx_b200.ops import moe
-    logits = torch.full((2, 4), -200.0, device=cuda_device)
+    logits = torch.full((2, 4), low, device=cuda_device)
     logits[1, 2] = 0
-    idx, w = moe.route(logits, 2, scoring="sigmoid")
-    assert idx.tolist() == [[0, 1], [2, 0]] and w.tolist() == [[0, 0], [1, 0]]
+    idx, w = moe.route(logits, 2, scoring="sigmoid", bias=torch.zeros(4, device=cuda_device) if wide else None)
+    each = 0.5 if low > -745 else 0.0
+    assert idx.tolist() == [[0, 1], [2, 0]] and w.cpu().tolist() == [[each, each], [1.0, pytest.approx(2 * math.exp(low), abs=1e-37)]]
+    idx, w = moe.route(torch.full((1, 3), -math.inf, device=cuda_device), 2, scoring="sigmoid", bias=torch.zeros(3, device=cuda_device) if wide else None)
+    assert idx.tolist() == [[-1, -1]] and w.tolist() == [[0, 0]]
 
 
 def test_rows_that_lie_apart_and_no_rows(cuda_device):
