@@ -74,6 +74,31 @@ def test_choice_with_bias_and_groups(cuda_device, scoring, t, e, topk, groups, t
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("groups,topk_groups", [(1, 1), (4, 2), (8, 3)])
+@pytest.mark.parametrize("apart", [1e-9, 1e-7, 2e-7, 1e-6, 1e-5, 1e-4])
+def test_scores_that_32_bits_cannot_tell_apart(cuda_device, scoring, renormalize, groups, topk_groups, apart):
+    g = torch.Generator().manual_seed(int(1e9 * apart) + groups)
+    e = 64
+    # every expert's score is near another's, and with a bias every group's: the same logits with a bias that is `apart` times a small number
+    logits = torch.randn(40, 8, generator=g).repeat(1, e // 8)
+    bias = apart * torch.randint(-3, 4, (e,), generator=g).float()
+    for order in (torch.arange(e), torch.randperm(e, generator=g)):
+        check(logits[:, order].contiguous().to(cuda_device), 6, scoring=scoring, bias=bias.to(cuda_device), groups=groups, topk_groups=topk_groups,
+              renormalize=renormalize)
+
+
+def test_biases_that_cancel_in_a_group(cuda_device):
+    # each group of two has the sum of its two scores, of which 32 bits lose all next to 2^20; what is left decides
+    g = torch.Generator().manual_seed(3)
+    logits = torch.randn(50, 16, generator=g).to(cuda_device)
+    bias = torch.tensor([2.0 ** 20, -(2.0 ** 20)] * 8, device=cuda_device)
+    check(logits, 2, scoring="sigmoid", bias=bias, groups=8, topk_groups=2)
+    bias = torch.tensor([math.inf, 1.0] * 8, device=cuda_device)
+    check(logits, 3, scoring="sigmoid", bias=bias, groups=8, topk_groups=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("wide", [False, True])
 def test_masks_and_values_that_are_no_numbers(cuda_device, scoring, wide):
     """Rows with fewer experts than places, with none, with NaN among them, with the type's lowest value, with zeros of both
