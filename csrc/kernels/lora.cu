@@ -564,9 +564,10 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     s.per_cta = width * passes;
   } else {
     // Parts of K and of N that the SMs have places for at once: a second wave that is half empty costs as much as a full one.
-    // How many tiles there will be is not known here: taken to be the tokens' and half a tile for each adapter, of those that can have some (256
-    // tokens, 64 adapters, 8192 x 8192, rank 16: 24.6 us, 28.1 without; 1500 tokens of 16 adapters 21.5 and 24.2; but 1000 of 16 22.0 and 20.4).
-    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile + std::min(d->n_adapters, d->n_tokens / 16) / 2, r = d->rank;
+    // How many tiles there will be is not known here: the tokens', and half a tile for each adapter, taken to be a dozen at most (1500 tokens of
+    // 16 adapters, 2048 x 6144, rank 32: 21.2 us, 24.0 without; with every adapter that is there counted 4096 tokens of 9 of 64, 8192 x 8192, rank
+    // 16, took 58 us, 49 so).
+    const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile + std::min({d->n_adapters, d->n_tokens / 16, 12}) / 2, r = d->rank;
     auto places = [](int smem) { return kSms * (227 * 1024 / (smem + 1024)); };
     const int shrink = places(r <= 8 ? LoraShrink<1, false>::BYTES : r <= 16 ? LoraShrink<2, false>::BYTES : r <= 32 ? LoraShrink<4, false>::BYTES
                               : r <= 64 ? LoraShrink<8, false>::BYTES : LoraShrink<16, false>::BYTES);
