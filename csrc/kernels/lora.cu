@@ -7,7 +7,8 @@
 // Two kernels, `shrink` (x to v) and `expand` (v to out), and for many tokens one in front:
 //
 // * Few tokens each stand for themselves: nothing is sorted, and requests that share an adapter read it again from the L2.
-//   lora_shrink_one: a warp has some rows of A and a part of K, both straight into registers; parts of K are added up by expand.
+//   lora_shrink_one: a warp has some rows of A and a part of K, both straight into registers; its CTA adds up four parts, and expand up to
+//   eight of these (with all parts added up by expand 16 tokens, 4096 x 4096, rank 64, took 9.8 us, 6.2 so).
 //   lora_expand_one: a row of B is read by as many lanes as it has 16-byte pieces; a lane group makes eight columns side by side.
 //   All in float32, no shared memory in the way: the chain id, A, v, B is four round trips to memory, and that is the time.
 // * With more, lora_order orders the tokens by adapter, in one CTA, and cuts them into tiles of up to kLoraTile that share one.
@@ -18,7 +19,7 @@
 //   lost is 2^-16 of it, nothing beside the result's rounding), made in registers. y and B go through a ring of stages with cp.async: B
 //   for all four warps, of y a lane fetches what it will need itself.
 //
-// Measured, in a graph: one token, 4096 x 4096, rank 16: 3.8 us; 64 tokens, 8192 x 8192, rank 16, an adapter each: 13.5 us; 777 tokens, 7168 x
+// Measured, in a graph: one token, 4096 x 4096, rank 16: 3.8 us; 64 tokens, 8192 x 8192, rank 16, an adapter each: 11.5 us; 777 tokens, 7168 x
 // 2056, rank 40: 18.2 us (3.6 at the measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 85.6
 // us (62 at the copy rate).
 #include <algorithm>
@@ -33,7 +34,7 @@ constexpr int64_t kLoraPlainBytes = int64_t(64) << 20;  // ... if the adapters t
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
 constexpr int kLoraColumns = 128;     // of N in a stage of expand (8192 tokens, 4096 x 4096, rank 64: 66.9 us, 70.0 with 64 columns and three or four stages)
-constexpr int kLoraMaxSlices = 32;    // parts of K of a token
+constexpr int kLoraMaxSlices = 8;     // parts of K of a token, each of a CTA
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
 struct LoraParams {
@@ -43,7 +44,7 @@ struct LoraParams {
   int* order;        // tokens, those of an adapter side by side
   int* n_tiles;
   int slices;        // parts of K
-  int per_slice;     // of K, a multiple of 256
+  int per_slice;     // of K, a multiple of 256; without tiles of each warp
   int per_cta;       // of N, a multiple of 64; with tiles of 128
 };
 
@@ -85,17 +86,19 @@ __device__ __forceinline__ void lora_floats(const uint4& v, float (&f)[8]) {
   }
 }
 
-// Grid: tokens, and the warps that a token takes, each with eight rows of A and a part of K.
+// Grid: tokens, and the CTAs that a token takes, each with eight rows of A and a part of K, a quarter of it for each warp.
 __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __grid_constant__ LoraParams p) {
   const eux_lora_desc& d = p.d;
-  const int lane = threadIdx.x & 31, unit = blockIdx.y * (kLoraThreads / 32) + (threadIdx.x >> 5);
+  constexpr int WARPS = kLoraThreads / 32;
+  __shared__ float sums[WARPS][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t token = blockIdx.x;
-  const int slice = unit % p.slices, r0 = unit / p.slices * 8;
+  const int slice = blockIdx.y % p.slices, r0 = blockIdx.y / p.slices * 8;
   wait_for_launch_before();
   allow_next_launch();  // expand's CTAs find room beside these, and have much to fetch that does not come from here
   const int adapter = lora_adapter(d, token);
-  const int k0 = slice * p.per_slice, k1 = min(d.k, k0 + p.per_slice);
-  if (r0 < d.rank && adapter < d.n_adapters) {
+  const int k0 = (slice * WARPS + warp) * p.per_slice, k1 = min(d.k, k0 + p.per_slice);
+  if (adapter < d.n_adapters) {
     const __nv_bfloat16* const x = (const __nv_bfloat16*)d.x + token * d.x_stride;
     const __nv_bfloat16* const a = (const __nv_bfloat16*)d.a + ((int64_t)adapter * d.rank + r0) * d.k;
     float acc[8] = {};
@@ -127,7 +130,9 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __g
     float v = acc[0];
     v += __shfl_xor_sync(0xffffffffu, v, 8);
     v += __shfl_xor_sync(0xffffffffu, v, 16);
-    if (lane < 8) p.v[((int64_t)slice * d.n_tokens + token) * d.rank + r0 + lane] = v;
+    if (lane < 8) sums[warp][lane] = v;
+    __syncthreads();
+    if (threadIdx.x < 8) p.v[((int64_t)slice * d.n_tokens + token) * d.rank + r0 + lane] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
   }
 }
 
@@ -541,7 +546,7 @@ static int lora_check(const eux_lora_desc* d) {
 
 struct LoraShape {
   bool one, wide;
-  int tiles, slices, per_slice, units, parts, per_cta;
+  int tiles, slices, per_slice, parts, per_cta;
   size_t v_bytes, tile_bytes, order_bytes, count_bytes;
 };
 // Columns that a CTA of lora_expand_one makes at a time.
@@ -549,17 +554,17 @@ static int lora_width(int rank) { return rank <= 8 ? 1024 : rank <= 16 ? 512 : r
 static LoraShape lora_shape(const eux_lora_desc* d) {
   LoraShape s;
   constexpr int kSms = 148;
-  // Each token for itself, or tiles of those that share an adapter (8192 x 8192, rank 16, an adapter each: 65 tokens, 34 MB, 13.5 and 22.4
+  // Each token for itself, or tiles of those that share an adapter (8192 x 8192, rank 16, an adapter each: 65 tokens, 34 MB, 11.5 and 22.4
   // us; 256 tokens, 134 MB, 26.9 and 29.0, and where they share adapters tiles read fewer).
   s.one = d->n_tokens <= kLoraPlain && (int64_t)d->n_tokens * d->rank * ((int64_t)d->k + d->n) * 2 <= kLoraPlainBytes;
   s.tiles = s.one ? d->n_tokens : (int)std::min<int64_t>(d->n_tokens, d->n_tokens / kLoraTile + (int64_t)d->n_adapters + 1);
   if (s.one) {
     // As many warps as the SMs have places for about, each with 256 of K or a multiple; expand once over its columns, likewise.
     const int64_t units = (int64_t)d->n_tokens * (d->rank / 8);
-    const int want = (int)std::max<int64_t>(1, std::min<int64_t>(kLoraMaxSlices, 32 * kSms / units));
+    constexpr int warps = kLoraThreads / 32;
+    const int want = (int)std::max<int64_t>(1, std::min<int64_t>(warps * kLoraMaxSlices, 32 * kSms / units));
     s.per_slice = ((d->k + want - 1) / want + 255) / 256 * 256;
-    s.slices = (d->k + s.per_slice - 1) / s.per_slice;
-    s.units = s.slices * (d->rank / 8);
+    s.slices = ((d->k + s.per_slice - 1) / s.per_slice + warps - 1) / warps;
     const int width = lora_width(d->rank), passes = (int)std::max<int64_t>(1, (int64_t)d->n_tokens * ((d->n + width - 1) / width) / (16 * kSms));
     s.per_cta = width * passes;
   } else {
@@ -626,7 +631,7 @@ static int lora_expand(const LoraParams& p, const LoraShape& s, int dev, cudaStr
 
 static int lora_run_one(const LoraParams& p, const LoraShape& s, cudaStream_t st) {
   const int r = p.d.rank;
-  if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, (s.units + kLoraThreads / 32 - 1) / (kLoraThreads / 32)), 1, 0, st, p)) return rc;
+  if (int rc = lora_launch(lora_shrink_one_kernel, dim3(s.tiles, s.slices * (r / 8)), 1, 0, st, p)) return rc;
   return lora_launch(r <= 8 ? lora_expand_one_kernel<1> : r <= 16 ? lora_expand_one_kernel<2> : r <= 32 ? lora_expand_one_kernel<4>
                      : r <= 64 ? lora_expand_one_kernel<8> : lora_expand_one_kernel<16>, dim3(s.tiles, s.parts), 1, 0, st, p);
 }
