@@ -30,7 +30,8 @@
 namespace eux {
 
 constexpr int kLoraPlain = 512;       // tokens up to which each may stand for itself ...
-constexpr int64_t kLoraPlainBytes = int64_t(64) << 20;  // ... if the adapters that they read then come to no more than this
+constexpr int64_t kLoraPlainBytes = int64_t(128) << 20;  // ... if the adapters that they read then come to no more than this,
+constexpr int64_t kLoraSharedBytes = int64_t(48) << 20;  // or this where more than four tokens must share one on average
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
 constexpr int kLoraColumns = 128;     // of N in a stage of expand (8192 tokens, 4096 x 4096, rank 64: 66.9 us, 70.0 with 64 columns and three or four stages)
@@ -554,9 +555,11 @@ static int lora_width(int rank) { return rank <= 8 ? 1024 : rank <= 16 ? 512 : r
 static LoraShape lora_shape(const eux_lora_desc* d) {
   LoraShape s;
   constexpr int kSms = 148;
-  // Each token for itself, or tiles of those that share an adapter (8192 x 8192, rank 16, an adapter each: 65 tokens, 34 MB, 11.5 and 22.4
-  // us; 256 tokens, 134 MB, 26.9 and 29.0, and where they share adapters tiles read fewer).
-  s.one = d->n_tokens <= kLoraPlain && (int64_t)d->n_tokens * d->rank * ((int64_t)d->k + d->n) * 2 <= kLoraPlainBytes;
+  // Each token for itself, or tiles of those that share an adapter. 64 adapters: 60 tokens, 8192 x 8192, rank 64, 126 MB, 27.2 and 39.4 us; 200
+  // tokens, rank 16, 105 MB, 23.4 and 27.3; 256, 134 MB, 28.3 and 27.9. 16 adapters, rank 16: 128 tokens, 4096 x 4096, 34 MB, 8.9 and 9.9; 240
+  // tokens, 63 MB, 12.9 and 10.2; 500 tokens, 131 MB, 22.8 and 11.5.
+  s.one = d->n_tokens <= kLoraPlain &&
+          (int64_t)d->n_tokens * d->rank * ((int64_t)d->k + d->n) * 2 <= (d->n_adapters >= d->n_tokens / 4 ? kLoraPlainBytes : kLoraSharedBytes);
   s.tiles = s.one ? d->n_tokens : (int)std::min<int64_t>(d->n_tokens, d->n_tokens / kLoraTile + (int64_t)d->n_adapters + 1);
   if (s.one) {
     // As many warps as the SMs have places for about, each with 256 of K or a multiple; expand once over its columns, likewise.

@@ -90,7 +90,8 @@ class LoraAdapters:
         workspace, _ = self._scratch.get(need)
         desc = self._desc(t, x.data_ptr(), ids.data_ptr(), y.data_ptr(), out.data_ptr(), workspace, xs, ys, os_)
         ws.launch(lib.eux_lora_launch, desc, self._index, "eux_lora_launch")
-        _launches += 2 if t <= 512 and t * self.rank * (self.K + self.N) * 2 <= 64 << 20 else 3  # as the launch chooses
+        few = t <= 512 and t * self.rank * (K + N) * 2 <= (128 if self.n_adapters >= t // 4 else 48) << 20  # as the launch chooses
+        _launches += 2 if few else 3
         return out
 
     def _desc(self, tokens, x=0, ids=0, y=0, out=0, workspace=0, x_stride=0, y_stride=0, out_stride=0):
