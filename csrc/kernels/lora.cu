@@ -8,7 +8,7 @@
 //
 // * Few tokens each stand for themselves: nothing is sorted, and requests that share an adapter read it again from the L2.
 //   lora_shrink_one: a warp has some rows of A and a part of K, both straight into registers; its CTA adds up four parts, and expand up to
-//   eight of these (with all parts added up by expand 16 tokens, 4096 x 4096, rank 64, took 9.8 us, 6.2 so).
+//   eight of these (with all parts added up by expand 16 tokens, 4096 x 4096, rank 64, took 9.8 us, 6.0 to 6.9 so).
 //   lora_expand_one: a row of B is read by as many lanes as it has 16-byte pieces; a lane group makes eight columns side by side.
 //   All in float32, no shared memory in the way: the chain id, A, v, B is four round trips to memory, and that is the time.
 // * With more, lora_order orders the tokens by adapter, in one CTA, and cuts them into tiles of up to kLoraTile that share one.
