@@ -29,8 +29,8 @@
 // beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 162 us (0.76), e4m3 195 us (0.32: widening
 // and mma.sync are the bound, 32 tokens to an expert).
 //
-// Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, which
-// stays below that of the result's own rounding on average.
+// Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, on
+// average as much as the result's own rounding. With few tokens the product has columns to spare, and h is two such numbers (xp_pairs).
 #include <cuda.h>
 
 #include <algorithm>
@@ -63,7 +63,7 @@ constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer c
 struct XpParams {
   eux_experts_desc d;
   __nv_bfloat16* x;      // [entries, x_pitch]: the tokens' values in the order of the entries; null: used where they lie
-  __nv_bfloat16* h;      // [entries, h_pitch], in the same order; zeros behind inner
+  __nv_bfloat16* h;      // [entries, h_pitch], in the same order, or two rows for each (xp_pairs); zeros behind inner
   int x_pitch, h_pitch;
   uint32_t* tables;      // what moe_experts_sort_kernel found (XpTables), with `named` and `cap` in front; null: found by every CTA
   float* part;           // [grid][2][part_rows][128]
@@ -193,6 +193,7 @@ struct XpTables {
   uint16_t* token;   // [entries]: of order
   float* weight;     // [entries]: of order
   int named;
+  int most;          // entries of an expert; not with tables from another kernel
   __device__ XpTables(unsigned char* at, int n_experts, int entries) {
     start = reinterpret_cast<int*>(at);
     first = reinterpret_cast<uint16_t*>(start + n_experts + 1);
@@ -230,6 +231,10 @@ __device__ __forceinline__ void xp_costs(XpTables& r, int lane) {  // by a warp
 struct XpSegment {
   int expert, tile, pos, n;
 };
+
+// Where no expert has more than four entries, and the tokens are used in place, h is kept as two bfloat16 numbers that add up to it, in
+// two rows: the product has eight columns either way.
+__device__ __forceinline__ bool xp_pairs(const XpParams& p, const XpTables& r) { return !p.tables && r.most <= 4; }
 
 __device__ __forceinline__ void xp_locate(const XpTables& r, int a, int chunk, XpSegment* s) {
   const int count = r.start[a + 1] - r.start[a], chunks = r.first[a + 1] - r.first[a];
@@ -303,10 +308,10 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
       }
       if (head) r.expert[before] = (uint16_t)e, r.start[before] = at, r.first[before] = (uint16_t)first;
       const int here = __popc(__ballot_sync(0xffffffffu, lane < n && e < E));
-      if (lane == 0) r.start[named] = here, r.first[named] = (uint16_t)chunks, out[0] = named, out[1] = cap;
+      if (lane == 0) r.start[named] = here, r.first[named] = (uint16_t)chunks, out[0] = named, out[1] = cap, out[2] = top;
     }
     __syncthreads();
-    r.named = out[0];
+    r.named = out[0], r.most = out[2];
     return out[1];
   }
   const int used = min(W, (n + 31) / 32);  // warps that have entries
@@ -380,7 +385,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
     __syncwarp();
   }
   __syncthreads();
-  r.named = named;
+  r.named = named, r.most = out[0];
   return cap;
 }
 
@@ -650,10 +655,22 @@ __device__ __forceinline__ void xp_tile_end(const XpParams& p, const XpTables& r
     } else {
       const int at = s.tile * 64 + q;
       auto gated = [](float g, float w) { return g / (1.f + expf(-g)) * w; };
-      __nv_bfloat16* const h = p.h + (int64_t)(s.pos + j) * p.h_pitch + at;
-      *reinterpret_cast<uint2*>(h) = at < d.inner ? make_uint2(pack_bf16(gated(v.x, u.x), gated(v.y, u.y)), pack_bf16(gated(v.z, u.z), gated(v.w, u.w)))
-                                                  : make_uint2(0, 0);
-      if (s.tile * 64 + 64 >= d.inner && s.tile * 64 + 64 < p.h_pitch) *reinterpret_cast<uint2*>(h + 64) = make_uint2(0, 0);  // the last tile's
+      // what bfloat16 loses; of an infinity nothing
+      auto rest = [](float f) {
+        const float b = __bfloat162float(__float2bfloat16_rn(f));
+        return isinf(b) ? 0.f : f - b;
+      };
+      const bool pairs = xp_pairs(p, r), last = s.tile * 64 + 64 >= d.inner && s.tile * 64 + 64 < p.h_pitch;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at < d.inner) f = make_float4(gated(v.x, u.x), gated(v.y, u.y), gated(v.z, u.z), gated(v.w, u.w));
+      __nv_bfloat16* h = p.h + (int64_t)(s.pos + j) * (pairs ? 2 : 1) * p.h_pitch + at;
+      *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16(f.x, f.y), pack_bf16(f.z, f.w));
+      if (last) *reinterpret_cast<uint2*>(h + 64) = make_uint2(0, 0);
+      if (pairs) {
+        h += p.h_pitch;
+        *reinterpret_cast<uint2*>(h) = make_uint2(pack_bf16(rest(f.x), rest(f.y)), pack_bf16(rest(f.z), rest(f.w)));
+        if (last) *reinterpret_cast<uint2*>(h + 64) = make_uint2(0, 0);
+      }
     }
   }
 }
@@ -719,6 +736,7 @@ struct XpResults {
         __syncwarp();
         if (lane == 0) mbar_arrive(free_bar);
       } else if (DOWN) {
+        const bool pairs = xp_pairs(p, r);
         for (int j0 = 0; j0 < s.n; j0 += 4) {
           float2 v[4];
           float w[4];
@@ -726,7 +744,11 @@ struct XpResults {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = min(j0 + i, s.n - 1);
-            v[i] = reinterpret_cast<const float2*>(sum + j * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
+            v[i] = reinterpret_cast<const float2*>(sum + (pairs ? 2 * j : j) * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
+            if (pairs) {
+              const float2 u = reinterpret_cast<const float2*>(sum + (2 * j + 1) * kXpLd)[tid];
+              v[i].x += u.x, v[i].y += u.y;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -864,7 +886,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
     for (int b = b0, seg = seg0, kb = kb0; b < b1 && !gone; ++seg, kb = 0) {
       const int end = min(nk, kb + (b1 - b));
       const XpSegment s = walk.at(seg);
-      const int nb = in_place ? 1 : (s.n + 7) >> 3, size = nb <= 1 ? 0 : nb <= 2 ? 1 : nb <= 4 ? 2 : 3, row = in_place ? 0 : s.pos;
+      const int nb = in_place ? 1 : (s.n + 7) >> 3, size = nb <= 1 ? 0 : nb <= 2 ? 1 : nb <= 4 ? 2 : 3, row = in_place ? 0 : DOWN && xp_pairs(p, r) ? 2 * s.pos : s.pos;
       // the scales of 32 blocks at a time, one per lane. Down: of the rows. Up: of the gate rows, of the first up rows, of the up rows
       // that lie in the next block.
       const float* const scale = FP8 ? (DOWN ? d.down_scale : d.gate_up_scale) + (int64_t)s.expert * sr * sk : nullptr;
@@ -1061,7 +1083,7 @@ static int xp_part_rows(const eux_experts_desc* d) { return std::max(64, d->n_to
 struct XpSpace {
   int x_pitch, h_pitch;
   bool sorted;
-  size_t h, x, tables, parts;
+  size_t h_rows, h, x, tables, parts;
 };
 static XpSpace xp_space(const eux_experts_desc* d) {
   XpSpace s;
@@ -1069,7 +1091,8 @@ static XpSpace xp_space(const eux_experts_desc* d) {
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   s.x_pitch = (d->hidden + 127) & ~127, s.h_pitch = (d->inner + 127) & ~127;
   s.sorted = d->n_tokens > 8 || d->hidden != s.x_pitch;  // copies take whole runs of columns
-  s.h = up(entries * s.h_pitch * 2);
+  s.h_rows = (s.sorted ? 1 : 2) * entries;  // xp_pairs
+  s.h = up(s.h_rows * s.h_pitch * 2);
   s.x = s.sorted ? up(entries * s.x_pitch * 2) : 0;
   s.tables = s.sorted ? up(16 + xp_table_bytes(d->n_experts, (int)entries)) : 0;
   s.parts = (size_t)kXpMaxGrid * 2 * xp_part_rows(d) * kXpRows * 4;
@@ -1149,7 +1172,7 @@ extern "C" int eux_experts_launch(const eux_experts_desc* d, void* stream) {
   XpMaps x = {}, h = {};
   if (int rc = space.sorted ? xp_map_rows(&x, p.x, entries, p.x_pitch, p.x_pitch, runs, entries)
                             : xp_map_rows(&x, d->x, d->n_tokens, d->hidden, std::max<int64_t>(d->x_stride, d->hidden), runs, 8)) return rc;
-  if (int rc = xp_map_rows(&h, p.h, entries, p.h_pitch, p.h_pitch, runs, entries)) return rc;
+  if (int rc = xp_map_rows(&h, p.h, space.h_rows, p.h_pitch, p.h_pitch, runs, entries)) return rc;
   if (space.sorted) {
     const size_t smem = xp_table_bytes(d->n_experts, entries) + std::max<size_t>((size_t)kXpThreads / 32 * d->n_experts * 4, 16 * kXpThreads);
     if (cudaError_t e = allow_smem<moe_experts_sort_kernel>(dev, 200 * 1024); e != cudaSuccess) return (int)e;

@@ -276,7 +276,7 @@ class MoeExperts:
         per token. An entry whose expert is not in ``[0, experts)`` adds nothing: with the experts of one of several GPUs, pass
         the indices less the number of its first expert, and add up the GPUs' results. A token without entries gets zeros.
         ``out`` may be ``x`` itself; the rows of both may lie apart. Sums are in float32; what lies between the two products is
-        rounded to bfloat16. The same arguments give the same bits. A wait in the kernels that runs out (two seconds) is told by
+        rounded to bfloat16, or with up to eight tokens, of which no expert has more than four, to two such numbers. The same arguments give the same bits. A wait in the kernels that runs out (two seconds) is told by
         ``check_status``; the result is none then."""
         global _launches
         index, hidden = self._index, self.hidden

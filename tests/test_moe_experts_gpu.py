@@ -26,8 +26,8 @@ def weights(e, h, i, fp8, dev, seed=0):
     return out[0], out[2], out[1], out[3]
 
 
-def plain(x, idx, w, gu, down, gus=None, ds=None):
-    """(the result, the bound of its error), both in 64 bits."""
+def plain(x, idx, w, gu, down, gus=None, ds=None, between=BF):
+    """(the result, the bound of its error), both in 64 bits. `between`: of the rounding between the products."""
     def full(m, s):
         m = m.double()
         return m if s is None else m * s.double().repeat_interleave(128, 0)[:m.shape[0]].repeat_interleave(128, 1)[:, :m.shape[1]]
@@ -46,7 +46,7 @@ def plain(x, idx, w, gu, down, gus=None, ds=None):
         hid = s * u
         # silu has a slope of at most 1.1; exp, a division and two products in float32
         dh = 1.1 * dg * u.abs() + s.abs() * du + dg * du * 1.1 + 16 * F * hid.abs()
-        dh = dh + BF * (hid.abs() + dh) + 2.0 ** -134
+        dh = dh + between * (hid.abs() + dh) + 2.0 ** -134
         out.index_add_(0, tok, wj * (hid @ b.t()))
         tol.index_add_(0, tok, wj.abs() * (dh @ b.abs().t() + (i + 40) * F * ((hid.abs() + dh) @ b.abs().t())))
     tol = tol + BF * (out.abs() + tol) + 2.0 ** -134
@@ -113,6 +113,24 @@ def test_every_number_of_tokens_that_an_expert_can_have(cuda_device, fp8, t):
     x = torch.randn(t, 272, device=cuda_device).to(torch.bfloat16)
     check(layer, x, idx, torch.rand(t, 1, device=cuda_device))
     layer.check_status()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,k,e", [(1, 8, 16), (3, 2, 4), (4, 4, 4), (8, 2, 16), (8, 32, 100)])
+def test_few_tokens_lose_nothing_between_the_products(cuda_device, fp8, t, k, e):
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(e, 384, 1040, fp8, cuda_device))
+    g = torch.Generator().manual_seed(t)
+    idx = (torch.arange(t * k).reshape(t, k) % e)[torch.randperm(t, generator=g)].to(torch.int32).to(cuda_device)  # no expert more than four times
+    assert int(torch.bincount(idx.flatten().long()).max()) <= 4
+    x, w = torch.randn(t, 384, device=cuda_device).to(torch.bfloat16), torch.rand(t, k, device=cuda_device)
+    out = check(layer, x, idx, w)
+    # two bfloat16 numbers: the second is off by 2^-8 of what the first left, 2^-8 of the value
+    want, tol = plain(x, idx, w, layer.w_gate_up, layer.w_down, layer.gate_up_scale, layer.down_scale, between=2.0 ** -16)
+    assert bool(((out.double() - want).abs() <= tol).all())
+    x[0, 5] = float("inf")  # stays with its token
+    rest = layer(x, idx, w)
+    assert torch.equal(rest[1:], out[1:])
 
 
 @pytest.mark.parametrize("fp8", [False, True])
