@@ -221,8 +221,9 @@ __global__ void __launch_bounds__(kOrderThreads) lora_order_kernel(const __grid_
   if (!counts) counts = order_smem;
   const eux_lora_desc& d = p.d;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, A = d.n_adapters + 1;
-  for (int i = threadIdx.x; i < A; i += kOrderThreads) counts[i] = 0;
+  // Behind the wait: counts that do not fit shared memory lie in the workspace, which may still be another call's until then.
   wait_for_launch_before();
+  for (int i = threadIdx.x; i < A; i += kOrderThreads) counts[i] = 0;
   constexpr int KEPT = 8;  // a thread's first adapters, fetched at once
   int kept[KEPT];
 #pragma unroll

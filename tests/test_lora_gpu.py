@@ -194,3 +194,40 @@ def test_beside_a_shared_projection(cuda_device):
     assert bool(((shared.double() - base).abs() <= dshared).all())
     want, tol = plain(x, ids, shared, layer.a, layer.b, layer.scale)
     assert bool(((out.double() - want).abs() <= tol).all())
+
+
+def test_more_adapters_than_counts_fit_shared_memory(cuda_device):
+    """Tokens are then counted by adapter in the workspace, which in a graph may be memory that the call in front still uses."""
+    from execution_ucx_b200.ops import lora, moe
+    from test_moe_experts_gpu import routing, weights
+    t, count, width, rank = 600, 60000, 256, 8
+    layer = lora.LoraAdapters(*adapters(count, width, width, rank, cuda_device))
+    experts = moe.MoeExperts(*weights(4, width, 1024, False, cuda_device))
+    x, y = bf(t, width, dev=cuda_device), bf(t, width, dev=cuda_device)
+    before = lora.launch_count()
+    for last in (count, 40, 1):  # a tile for nearly every token, many tokens of an adapter, one adapter
+        ids = torch.randint(-1, last, (t,), device=cuda_device, dtype=torch.int32)
+        ids[7], ids[8], ids[9] = count - 1, count, -1
+        out = layer(x, ids, y)
+        named = ids.unique()
+        named = named[(named >= 0) & (named < count)]
+        at = torch.where((ids >= 0) & (ids < count), torch.searchsorted(named, ids), -1)
+        want, tol = plain(x, at, y, layer.a[named], layer.b[named], layer.scale[named])
+        assert bool(((out.double() - want).abs() <= tol).all()) and torch.equal(out[at < 0], y[at < 0])
+        assert torch.equal(out, layer(x, ids, y))
+    assert lora.launch_count() - before == 6 * 3, "three launches each: ordered by adapter"
+    idx, w = routing(128, 4, 4, cuda_device, 1)
+    want_experts = experts(x[:128], idx, w)
+    want = layer(x, ids, y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = []
+        for _ in range(3):
+            o = experts(x[:128], idx, w)
+            outs.append((o, layer(x, ids, y)))
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        experts.check_status()
+        for o, a in outs:
+            assert torch.equal(o, want_experts) and torch.equal(a, want)
