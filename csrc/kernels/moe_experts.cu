@@ -58,6 +58,7 @@ constexpr int kXpSumBars = 96;                      // bytes: for each of two su
 constexpr int kXpLd = kXpRows + 4;                  // floats between tokens in shared memory: no bank conflicts, 16-byte rows
 constexpr int kXpMaxGrid = 160;
 constexpr size_t kXpDynamic = 226 * 1024;           // shared memory of a launch; the kernel declares a little more itself
+constexpr int64_t kXpMaxLine = 1 << 30;             // places on it are 32 bits, and some lie a little behind its end
 constexpr int kXpMinBlocks = 4;                     // of an SM's share: fewer cost more to add up than they save; none may cost more than all of these (xp_cost)
 
 struct XpParams {
@@ -389,8 +390,7 @@ __device__ __forceinline__ int xp_route(const eux_experts_desc& d, int token_of,
   return cap;
 }
 
-// Equal shares of a line, the first `more` of them one longer. (A line is shorter than 2^31: 180 GB of weights are 12 million blocks
-// that cost 9 at most, and no expert has more than 128 chunks.)
+// Equal shares of a line, the first `more` of them one longer. (A line is no longer than kXpMaxLine, which the host sees to.)
 struct XpShares {
   int each, more;
   __device__ XpShares(int length, int grid) : each(length / grid), more(length % grid) {}
@@ -1070,12 +1070,23 @@ static int xp_map(CUtensorMap* m, const void* base, bool fp8, uint64_t slices, u
   return rc == CUDA_SUCCESS ? 0 : EUX_ERR_BAD_ARG;
 }
 
+// The longest line that a pass can have, of blocks or of what they cost: each named expert has a chunk of up to `most` entries that is not
+// full, the others are.
+static int64_t xp_longest_line(const eux_experts_desc* d) {
+  const int64_t entries = (int64_t)d->n_tokens * d->topk, chunks = std::min<int64_t>(d->n_experts, entries) + entries / (d->fp8 ? 32 : kXpAccColumns);
+  auto runs = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+  const int64_t per_block = d->fp8 ? 128 : 64;
+  const int64_t blocks = std::max(runs(d->inner, 64) * runs(d->hidden, per_block), runs(d->hidden, kXpRows) * runs(d->inner, per_block));
+  return blocks * chunks * (d->fp8 ? 9 : 1);  // xp_cost
+}
+
 static int experts_check(const eux_experts_desc* d) {
   if (!d || d->n_tokens < 0 || d->n_tokens > EUX_EXPERTS_MAX_TOKENS || d->topk < 1 || d->topk > 32) return EUX_ERR_BAD_ARG;
   if (d->n_experts < 1 || d->n_experts > EUX_EXPERTS_MAX_EXPERTS || d->hidden < 1 || d->inner < 1) return EUX_ERR_BAD_ARG;
   if (d->hidden > (1 << 20) || d->inner > (1 << 20)) return EUX_ERR_BAD_ARG;
   const int unit = d->fp8 ? 16 : 8;  // rows of weights begin on 16 bytes
   if (d->hidden % unit || d->inner % unit || d->x_stride % 8 || d->out_stride % 8 || d->x_stride < 0 || d->out_stride < 0) return EUX_ERR_BAD_ARG;
+  if (xp_longest_line(d) > kXpMaxLine) return EUX_ERR_TOO_LARGE;
   return 0;
 }
 static int xp_part_rows(const eux_experts_desc* d) { return std::max(64, d->n_tokens); }

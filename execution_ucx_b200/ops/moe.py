@@ -304,7 +304,9 @@ class MoeExperts:
             n = min(self.MAX_TOKENS, t - first)
             need = self._need.get((n, topk))
             if need is None:
-                need = self._need[n, topk] = int(lib.eux_experts_workspace_bytes(self._desc(n, topk)))
+                need = int(lib.eux_experts_workspace_bytes(self._desc(n, topk)))
+                ws.require(need > 0, f"{n} x {topk} entries of {self.n_experts} experts of {hidden} x {self.inner} are too many for one call")
+                self._need[n, topk] = need
             workspace, counters = self._scratch.get(need)
             desc = self._desc(n, topk, x.data_ptr() + 2 * first * xs, topk_idx.data_ptr() + 4 * first * topk, topk_w.data_ptr() + 4 * first * topk,
                               out.data_ptr() + 2 * first * os_, workspace, counters, xs, os_)

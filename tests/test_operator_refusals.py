@@ -72,6 +72,22 @@ def test_launches_refuse_without_a_gpu(native_build):
     assert lib.eux_lora_launch(C.byref(n.LoraDesc(**{**good, "n_tokens": 0})), None) == 0
 
 
+def test_experts_refuse_passes_that_32_bits_cannot_number(native_build):
+    """The blocks of a pass, times what each may cost, are numbered in 32 bits."""
+    import ctypes as C
+    from execution_ucx_b200.ops import _native as n
+    lib = n.load()
+    size = lambda **kw: lib.eux_experts_workspace_bytes(C.byref(n.ExpertsDesc(**kw)))  # noqa: E731
+    large = dict(hidden=1 << 18, inner=1 << 18, n_experts=1)  # 4096 x 2048 blocks of e4m3 gate and up rows, 137 GB
+    assert size(**large, n_tokens=1, topk=1, fp8=1) > 0 and size(**large, n_tokens=128, topk=1, fp8=1) > 0
+    assert size(**large, n_tokens=128, topk=32, fp8=1) == 0  # 128 chunks of 32 entries that cost 9: 9.7e9
+    wide = dict(hidden=1 << 17, inner=1 << 17, n_experts=1)  # 2048 x 2048 blocks in bfloat16, 69 GB
+    assert size(**wide, n_tokens=128, topk=1) > 0 and size(**wide, n_tokens=128, topk=32) > 0  # 64 chunks: 2.7e8
+    assert size(**{**wide, "n_experts": 1024}, n_tokens=128, topk=32) == 0
+    assert size(hidden=7168, inner=2048, n_experts=1024, n_tokens=128, topk=32, fp8=1) > 0  # 45 GB, every expert named
+    assert size(hidden=16384, inner=16384, n_experts=200, n_tokens=128, topk=32, fp8=1) > 0
+
+
 @pytest.mark.gpu
 def test_calls_refuse(cuda_device):
     from execution_ucx_b200.ops import lora, moe
