@@ -50,6 +50,7 @@ constexpr int kXpWarps = kXpGroups * 4;
 template <bool TC>
 constexpr int kXpEndThreads = TC ? 128 : 64;
 constexpr int kXpAccColumns = 64;                   // of TMEM: the tokens of a segment at most
+constexpr int kXpFewTokens = 8;                     // of a call: used where they lie if their rows allow it, and h may be two numbers (xp_pairs)
 constexpr int kXpFewColumns = 16;                   // bfloat16 weights: up to so many tokens of an expert are multiplied with mma.sync
 constexpr int kXpRows = 128;                        // rows of weights in a block
 constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
@@ -66,7 +67,7 @@ struct XpParams {
   __nv_bfloat16* x;      // [entries, x_pitch]: the tokens' values in the order of the entries; null: used where they lie
   __nv_bfloat16* h;      // [entries, h_pitch], in the same order, or two rows for each (xp_pairs); zeros behind inner
   int x_pitch, h_pitch;
-  uint32_t* tables;      // what moe_experts_sort_kernel found (XpTables), with `named` and `cap` in front; null: found by every CTA
+  uint32_t* tables;      // what moe_experts_sort_kernel found (XpTables), with `named`, `cap` and `most` in front; null: found by every CTA
   float* part;           // [grid][2][part_rows][128]
   int part_rows;
   int token_of;          // ceil(2^20 / topk): entry * token_of >> 20 is entry / topk, for less than 2^20 / topk entries
@@ -194,7 +195,7 @@ struct XpTables {
   uint16_t* token;   // [entries]: of order
   float* weight;     // [entries]: of order
   int named;
-  int most;          // entries of an expert; not with tables from another kernel
+  int most;          // entries of an expert
   __device__ XpTables(unsigned char* at, int n_experts, int entries) {
     start = reinterpret_cast<int*>(at);
     first = reinterpret_cast<uint16_t*>(start + n_experts + 1);
@@ -233,9 +234,9 @@ struct XpSegment {
   int expert, tile, pos, n;
 };
 
-// Where no expert has more than four entries, and the tokens are used in place, h is kept as two bfloat16 numbers that add up to it, in
-// two rows: the product has eight columns either way.
-__device__ __forceinline__ bool xp_pairs(const XpParams& p, const XpTables& r) { return !p.tables && r.most <= 4; }
+// With few tokens, of which no expert has more than four, h is kept as two bfloat16 numbers that add up to it, in two rows: the product has
+// eight columns either way.
+__device__ __forceinline__ bool xp_pairs(const XpParams& p, const XpTables& r) { return p.d.n_tokens <= kXpFewTokens && r.most <= 4; }
 
 __device__ __forceinline__ void xp_locate(const XpTables& r, int a, int chunk, XpSegment* s) {
   const int count = r.start[a + 1] - r.start[a], chunks = r.first[a + 1] - r.first[a];
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   if (p.tables) {
     const uint4* const from = reinterpret_cast<const uint4*>(p.tables + 4);
     for (int i = threadIdx.x; i < xp_table_bytes(d.n_experts, entries) / 16; i += kXpThreads) reinterpret_cast<uint4*>(xp_smem + l.tables)[i] = __ldcg(from + i);
-    r.named = (int)__ldcg(p.tables), cap = (int)__ldcg(p.tables + 1);
+    r.named = (int)__ldcg(p.tables), cap = (int)__ldcg(p.tables + 1), r.most = (int)__ldcg(p.tables + 2);
     __syncthreads();
   } else {
     cap = xp_route(d, p.token_of, FP8 ? 32 : kXpAccColumns, r, reinterpret_cast<int*>(xp_smem), s_route);
@@ -1010,7 +1011,7 @@ __global__ void __launch_bounds__(kXpThreads) moe_experts_sort_kernel(const __gr
       __syncthreads();
     }
     for (int i = threadIdx.x; i < bytes / 16; i += kXpThreads) reinterpret_cast<uint4*>(p.tables + 4)[i] = reinterpret_cast<const uint4*>(xp_smem)[i];
-    if (threadIdx.x == 0) p.tables[0] = (uint32_t)r.named, p.tables[1] = (uint32_t)cap;
+    if (threadIdx.x == 0) p.tables[0] = (uint32_t)r.named, p.tables[1] = (uint32_t)cap, p.tables[2] = (uint32_t)r.most;
   }
   const int here = r.start[r.named], pieces = p.x_pitch / 8;
   for (int i = blockIdx.x * kXpThreads + threadIdx.x; i < here * pieces; i += gridDim.x * kXpThreads) {
@@ -1101,8 +1102,8 @@ static XpSpace xp_space(const eux_experts_desc* d) {
   const size_t entries = (size_t)d->n_tokens * d->topk;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   s.x_pitch = (d->hidden + 127) & ~127, s.h_pitch = (d->inner + 127) & ~127;
-  s.sorted = d->n_tokens > 8 || d->hidden != s.x_pitch;  // copies take whole runs of columns
-  s.h_rows = (s.sorted ? 1 : 2) * entries;  // xp_pairs
+  s.sorted = d->n_tokens > kXpFewTokens || d->hidden != s.x_pitch;  // copies take whole runs of columns
+  s.h_rows = (d->n_tokens > kXpFewTokens ? 1 : 2) * entries;  // xp_pairs
   s.h = up(s.h_rows * s.h_pitch * 2);
   s.x = s.sorted ? up(entries * s.x_pitch * 2) : 0;
   s.tables = s.sorted ? up(16 + xp_table_bytes(d->n_experts, (int)entries)) : 0;

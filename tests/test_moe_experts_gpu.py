@@ -134,6 +134,23 @@ def test_few_tokens_lose_nothing_between_the_products(cuda_device, fp8, t, k, e)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,k,e,h,i", [(1, 8, 16, 1936, 1040), (1, 1, 1, 16, 1000 // 16 * 16), (4, 4, 4, 400, 656), (8, 2, 16, 144, 2064), (8, 32, 100, 80, 304), (7, 4, 30, 208, 64)])
+def test_few_tokens_lose_nothing_between_the_products_whatever_the_width(cuda_device, fp8, t, k, e, h, i):
+    """As above, with rows whose width is no multiple of 128."""
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(e, h, i, fp8, cuda_device))
+    idx = (torch.arange(t * k).reshape(t, k) % e).to(torch.int32)
+    idx[t // 2:, 0] = torch.where(torch.arange(t - t // 2) % 3 == 2, -1, idx[t // 2:, 0])  # and entries without an expert
+    idx = idx.to(cuda_device)
+    assert int(torch.bincount(idx[idx >= 0].long()).max()) <= 4
+    x, w = torch.randn(t, h, device=cuda_device).to(torch.bfloat16), torch.rand(t, k, device=cuda_device)
+    out = check(layer, x, idx, w)
+    assert torch.equal(out, layer(x, idx, w))
+    want, tol = plain(x, idx, w, layer.w_gate_up, layer.w_down, layer.gate_up_scale, layer.down_scale, between=2.0 ** -16)
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("counts", [(128, 1, 1, 1), (20, 9, 3, 33, 1, 0, 17, 8), (12,) + (1,) * 39, (1,) * 39 + (64,), (40, 128, 100, 70)])
 def test_experts_with_very_different_numbers_of_tokens(cuda_device, fp8, counts):
     from execution_ucx_b200.ops import moe
