@@ -137,6 +137,23 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_one_kernel(const __g
   }
 }
 
+// A CTA's results, a column at a time.
+__device__ __noinline__ void lora_one_plainly(const LoraParams& p, int64_t token, int adapter, float scale, const float (*parts)[EUX_LORA_MAX_RANK]) {
+  const eux_lora_desc& d = p.d;
+  const int n1 = min(d.n, (blockIdx.y + 1) * p.per_cta);
+  for (int n = blockIdx.y * p.per_cta + threadIdx.x; n < n1; n += kLoraThreads) {
+    const __nv_bfloat16* const b = (const __nv_bfloat16*)d.b + ((int64_t)adapter * d.n + n) * d.rank;
+    float sum = 0.f;
+    for (int r = 0; r < d.rank; ++r) {
+      float v = 0.f;
+      for (int s = 0; s < p.slices; ++s) v += parts[s][r];
+      sum = fmaf(v, __bfloat162float(b[r]), sum);
+    }
+    const __nv_bfloat16* const y = (const __nv_bfloat16*)d.y + token * d.y_stride + n;
+    ((__nv_bfloat16*)d.out)[token * d.out_stride + n] = __float2bfloat16_rn(fmaf(scale, sum, __bfloat162float(*y)));
+  }
+}
+
 // Grid: tokens, parts of N. LANES: that share a row of B, a power of two of at least rank / 8.
 template <int LANES>
 __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __grid_constant__ LoraParams p) {
@@ -171,6 +188,11 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_one_kernel(const __g
       parts[s][r] = __ldcg(p.v + ((int64_t)s * d.n_tokens + token) * d.rank + r);
     }
     __syncthreads();
+    if (!isfinite(scale)) {  // times each product's terms it would make NaN of signs that differ: behind their sum
+      lora_one_plainly(p, token, adapter, scale, parts);
+      allow_next_launch();
+      return;
+    }
     if (some)
       for (int s = 0; s < p.slices; ++s)
 #pragma unroll
@@ -418,6 +440,29 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const __grid_
   if (R8 >= 16) allow_next_launch();
 }
 
+__device__ __forceinline__ float2 lora_times_zero(float x, float y, float2 to) {  // to + 0 * (x, y)
+  asm("{\n\t.reg .b64 a, b, z;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%0, %1};\n\tmov.b64 z, 0;\n\t"
+      "fma.rn.f32x2 b, a, z, b;\n\tmov.b64 {%0, %1}, b;\n\t}"
+      : "+f"(to.x), "+f"(to.y)
+      : "f"(x), "f"(y));
+  return to;
+}
+// Of eight results those that are no numbers, made again of v in float32: as two bfloat16 numbers v is an infinity where it is above their
+// largest, and the second of them, zero or of the other sign, makes NaN of an infinity of B. `y` lies in shared memory.
+__device__ __forceinline__ void lora_again(__nv_bfloat16* out, uint32_t y, const float* v, const __nv_bfloat16* b, int rank, float scale) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    if (isfinite(__bfloat162float(out[i]))) continue;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < rank; ++r) sum = fmaf(__ldcg(v + r), __bfloat162float(b[(int64_t)i * rank + r]), sum);
+    unsigned short of_y;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(of_y) : "r"(y + 2 * i) : "memory");
+    out[i] = __float2bfloat16_rn(fmaf(scale, sum, __bfloat162float(__ushort_as_bfloat16(of_y))));
+  }
+}
+
 // K16: ranks in 16s, rounded up to a power of two. Columns go 128 at a time, in runs of 32. A lane's eight columns of a run lie side
 // by side, so that y and out are moved 16 bytes at a time: column 2c + i of the product's j-th eight is column 8c + 2j + i of the run,
 // and the rows of B lie in shared memory in the product's order.
@@ -484,16 +529,27 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
       const int at = k * 16 + 2 * c + 8 * (q >> 1);
       float2 v = make_float2(0.f, 0.f);
       if (has && row[q & 1] && at < d.rank) v = __ldcg(reinterpret_cast<const float2*>(p.v + (int64_t)(t.first + row0 + g + 8 * (q & 1)) * d.rank + at));
-      v.x *= scale, v.y *= scale;
       const __nv_bfloat162 u = __floats2bfloat162_rn(v.x, v.y);
       const float2 f = __bfloat1622float2(u);
-      // nothing is lost of an infinity
+      // nothing is lost of an infinity; what else is no number here is made again (lora_again)
       const __nv_bfloat162 l = __floats2bfloat162_rn(isinf(f.x) ? 0.f : v.x - f.x, isinf(f.y) ? 0.f : v.y - f.y);
       hi[k][q] = *reinterpret_cast<const uint32_t*>(&u), lo[k][q] = *reinterpret_cast<const uint32_t*>(&l);
     }
+  float2 none = make_float2(0.f, 0.f);  // zero, or NaN where one of the last step's sums is no number
+  auto again = [&](int step) {
+    none = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int q = 0; q < kLoraColumns / 16; ++q) {
+      const int h = q & 1, col = n0 + step * kLoraColumns + (q >> 1) * 32 + c * 8;
+      if ((h ? row[1] : row[0]) && col < n1)
+        lora_again((h ? out_row[1] : out_row[0]) + col, smem + step % S::STAGES * S::STAGE + S::B + (q * kLoraThreads + threadIdx.x) * 16,
+                   p.v + (int64_t)(t.first + row0 + g + 8 * h) * d.rank, b + (int64_t)col * d.rank, d.rank, scale);
+    }
+  };
   for (int s = 0; s < steps; ++s) {
     lora_cp_wait<S::STAGES - 2>();
     __syncthreads();
+    if (none.x != 0.f || none.y != 0.f) again(s - 1);  // y is still there, until the fetch
     fetch(s + S::STAGES - 1);
     const uint32_t at = smem + s % S::STAGES * S::STAGE;
     if (row0 < t.n) {
@@ -525,7 +581,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const float2 f = __bfloat1622float2(y2[j]);
-                y2[j] = __floats2bfloat162_rn(f.x + acc[j][2 * h], f.y + acc[j][2 * h + 1]);
+                y2[j] = __floats2bfloat162_rn(fmaf(scale, acc[j][2 * h], f.x), fmaf(scale, acc[j][2 * h + 1], f.y));
+                none = lora_times_zero(acc[j][2 * h], acc[j][2 * h + 1], none);
               }
             }
             st_u4(out_row[h] + col, y);
@@ -533,6 +590,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_expand_kernel(const __grid_
       }
     }
   }
+  if (none.x != 0.f || none.y != 0.f) again(steps - 1);
   lora_cp_wait<0>();
   allow_next_launch();
 }

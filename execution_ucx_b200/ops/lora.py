@@ -24,8 +24,8 @@ class LoraAdapters:
     """The adapters of one projection: ``a`` ``[adapters, rank, K]`` and ``b`` ``[adapters, N, rank]``, bfloat16, and ``scale``
     ``[adapters]``, float32 (1 if not given). They are used where they lie: the object keeps the tensors and copies nothing, so
     an adapter that is written into its place holds for the next call. ``rank`` is a multiple of 8 up to 128, K and N are
-    multiples of 8; ``b`` holds no infinities (with many tokens they give NaN). For inference: the result has no gradient. An
-    object is made outside of graph captures; its calls may be captured, and made by several threads."""
+    multiples of 8. For inference: the result has no gradient. An object is made outside of graph captures; its calls may be
+    captured, and made by several threads."""
 
     MAX_RANK = 128
 

@@ -171,3 +171,52 @@ def test_on_a_stream_of_ones_own(cuda_device):
     assert bool(((out.double() - want).abs() <= tol).all())
     want, tol = plain(x, ids, out, layer.a, layer.b, layer.scale)
     assert bool(((again.double() - want).abs() <= tol).all())
+
+
+def same_kind(got, want, tol, either):
+    """Infinities where the statement has infinities of that sign, NaN where it has NaN, numbers within the bound."""
+    got, fine = got.double(), want.isfinite()
+    assert torch.equal(got.isnan(), want.isnan())
+    # an infinite scale times a sum that is within its own error of zero: of either sign
+    assert torch.equal(got[want.isinf()].abs(), want[want.isinf()].abs()) and torch.equal(got[want.isinf() & ~either], want[want.isinf() & ~either])
+    assert bool(((got - want).abs()[fine] <= tol[fine]).all())
+
+
+@pytest.mark.parametrize("t", [20, T])
+@pytest.mark.parametrize("rank", [8, 16, 40, 128])
+def test_infinities_in_an_adapter(cuda_device, rank, t):
+    """An adapter's infinities make infinities, and NaN only where the formula does, whatever the number of tokens."""
+    from execution_ucx_b200.ops import lora
+    k, n = 256, 264
+    a, b, scale = adapters(3, k, n, rank, cuda_device)
+    inf = float("inf")
+    b[0, 7, 0], b[0, 9, rank - 1], b[0, 200, 3], b[0, 200, 5], b[0, 263, 1] = inf, -inf, inf, -inf, float("nan")
+    a[1, 2, 5], b[1, 11, 4], scale[2] = inf, inf, -inf
+    layer = lora.LoraAdapters(a, b, scale)
+    ids = (torch.arange(t, device=cuda_device) % 4 - 1).to(torch.int32)
+    x, y = bf(t, k, dev=cuda_device), bf(t, n, dev=cuda_device)
+    x[1] = 0      # of the first adapter: its products are zeros, which times infinity is NaN
+    y[5, 7] = -inf  # and here an infinity meets one
+    out = layer(x, ids, y)
+    want = lora.reference(x, ids, y, a, b, scale)
+    clean = lambda v: torch.where(v.isfinite(), v, 0.0)  # noqa: E731
+    _, tol = plain(x, ids, clean(y), clean(a), clean(b), clean(scale))
+    assert bool(want.isinf().any()) and bool(want.isnan().any())
+    sums, of_sums = plain(x, ids, torch.zeros_like(y), clean(a), clean(b), torch.ones_like(scale))
+    either = (ids == 2).unsqueeze(1) & (sums.abs() <= of_sums)
+    same_kind(out, want, tol, either)
+
+
+@pytest.mark.parametrize("t", [20, T])
+def test_products_that_only_float32_can_hold(cuda_device, t):
+    """A x is a number of float32 that rounds to an infinity of bfloat16; what it is multiplied with brings it back."""
+    from execution_ucx_b200.ops import lora
+    a, b = torch.zeros(1, 16, 64, dtype=torch.bfloat16, device=cuda_device), torch.zeros(1, 64, 16, dtype=torch.bfloat16, device=cuda_device)
+    a[0, :, 0], a[0, :, 1], b[0, :, 3] = 1, 2.0 ** -7, 2.0 ** -20
+    x, y = torch.zeros(t, 64, dtype=torch.bfloat16, device=cuda_device), bf(t, 64, dev=cuda_device)
+    x[2, 0] = x[2, 1] = torch.finfo(torch.bfloat16).max * 0.99609375
+    x[2, 1] *= 0.9921875
+    layer = lora.LoraAdapters(a, b)
+    v = float(x[2, 0]) + float(x[2, 1]) * 2.0 ** -7
+    assert torch.tensor(v).isfinite() and torch.tensor(v).to(torch.bfloat16).isinf()
+    check(layer, x, torch.zeros(t, dtype=torch.int32, device=cuda_device), y)
