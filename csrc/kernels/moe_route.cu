@@ -91,7 +91,7 @@ __device__ __forceinline__ int take_best(uint64_t (&key)[NV], uint64_t& mine, in
   return e;
 }
 
-// WIDE: scores and keys in 64 bits (bias or groups).
+// WIDE: scores and keys in 64 bits (bias or groups). Without, only a softmax's sum is of 32.
 template <int NV, bool WIDE>
 __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_desc d) {
   using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
@@ -183,26 +183,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(eux_route_d
       const int e = take_best<NV>(key, best, at, lane);
       if (lane == j) mine = e;
     }
-    Real s = 0;
+    // The weights of the few that are chosen, one per lane, in 64 bits: sigmoids and quotients of them that 32 bits have no number for count.
+    double s = 0;
     if (mine >= 0) {
-      const float v = fminf(route_logit(d, t, mine), 3.402823466e38f);
-      if constexpr (WIDE) s = d.sigmoid ? __drcp_rn(1.0 + exp(-(double)v)) : exp((double)v - (double)peak) / sum;
-      else s = d.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - peak) / sum;
+      const double v = fminf(route_logit(d, t, mine), 3.402823466e38f);
+      s = d.sigmoid ? __drcp_rn(1.0 + exp(-v)) : exp(v - (double)peak) / (double)sum;
     }
     if (d.renormalize) {
-      Real all = warp_sum(s);
-      if (!WIDE && d.sigmoid && all < 1e-30f) {
-        // All too small for 32 bits: there e^v is the sigmoid to the last bit, and e^(v - the largest v) has the same proportions. What 1 / (1 +
-        // e^-v) has no number for in 64 bits either, where e^-v has none, weighs nothing.
-        const float v = mine >= 0 ? route_logit(d, t, mine) : -INFINITY, first = __shfl_sync(0xffffffffu, v, 0);
-        s = v > -709.78f ? (Real)expf(v - first) : (Real)0;
-        all = warp_sum(s);
-      }
-      s = all > 0 ? s / all : (Real)0;  // none taken, or every score too small for a number: no weight
+      const double all = warp_sum(s);
+      s = all > 0 ? s / all : 0.0;  // none taken, or every score too small for a number: no weight
     }
     if (lane < d.topk) {
       d.topk_idx[t * d.topk + lane] = mine;
-      d.topk_w[t * d.topk + lane] = (float)(s * (Real)d.scale);
+      d.topk_w[t * d.topk + lane] = (float)(s * (double)d.scale);
     }
   }
   allow_next_launch();

@@ -160,3 +160,22 @@ def test_captured_and_replayed(cuda_device):
         graph.replay()
         want_idx, want_w = moe.route(logits, 4)
         assert torch.equal(idx, want_idx) and torch.equal(w, want_w)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+def test_weights_far_below_the_largest(cuda_device, scoring, renormalize, wide):
+    """Chosen experts whose scores are so far apart that 32 bits have no number for the quotient's parts, but one for the quotient."""
+    from execution_ucx_b200.ops import moe
+    rows = [[-60, -95, -97, -100], [-88, -91, -120, -150], [0, -20, -80, -102], [-300, -310, -330, -380], [-700, -705, -708, -700], [30, -30, -60, -70], [-89, -89, -89, -89]]
+    logits = torch.tensor(rows, dtype=torch.float32, device=cuda_device)
+    kw = dict(scoring=scoring, renormalize=renormalize, bias=torch.zeros(4, device=cuda_device) if wide else None)
+    idx, w = moe.route(logits, 4, **kw)
+    want_idx, want = plain(logits, 4, **kw)
+    # in 64 bits but for a softmax's sum (as above: 37 steps, and the exponentials of it are off by 2 * 2^-24), then rounded once, where there
+    # may be no more than a subnormal number
+    tol = (37 + 2 + 2) * 2.0 ** -24
+    assert bool(((w.cpu().double() - want).abs() <= tol * want + 2.0 ** -149).all())
+    if wide and scoring == "sigmoid":  # equal scores in 64 bits go by their index
+        assert torch.equal(idx.cpu(), want_idx)
