@@ -291,6 +291,12 @@ EUX_API int eux_lora_launch(const eux_lora_desc* d, void* stream);
 EUX_API size_t eux_lora_workspace_bytes(const eux_lora_desc* d);
 EUX_API int eux_lora_preload(void);
 
+/* ---- what captured calls use, for as long as their graphs are there (graph_hold.cu) ----
+ * eux_graph_hold: of the graph that `stream` is being captured into. Once that graph and everything made of it are destroyed, and no replay is
+ * under way, `token` is among those that eux_graphs_gone gives, each once, up to `most` at a time; it returns how many. */
+EUX_API int eux_graph_hold(void* stream, uint64_t token);
+EUX_API int eux_graphs_gone(uint64_t* tokens, int most);
+
 #ifdef __cplusplus
 }
 #endif

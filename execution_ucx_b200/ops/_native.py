@@ -162,6 +162,8 @@ def load():
     lib.eux_moe_combine_launch.argtypes = [P, I, P]
     for op in ("route", "experts", "lora"):
         getattr(lib, f"eux_{op}_launch").argtypes = [P, P]
+    lib.eux_graph_hold.argtypes = [P, U64]
+    lib.eux_graphs_gone.argtypes = [C.POINTER(U64), I]
     lib.eux_experts_maps.argtypes = [P, P]
     lib.eux_experts_find_nan.argtypes = [P, C.c_size_t, P, P]
     for size in ("eux_experts_workspace_bytes", "eux_experts_counter_words", "eux_lora_workspace_bytes"):

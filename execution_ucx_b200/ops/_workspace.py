@@ -2,7 +2,10 @@
 zeroed words for kernels that count their CTAs."""
 from __future__ import annotations
 
+import ctypes as C
+import itertools
 import threading
+import weakref
 
 import torch
 
@@ -75,20 +78,38 @@ def launch(function, desc, index: int, what: str) -> None:
         _native.check(rc, what)
 
 
+# What captured calls use of an object's own memory, by the token that their graph gives back when it is gone.
+_held = {}
+_tokens = itertools.count(1)
+
+
+def _collect() -> None:
+    """Gives what graphs that are gone had used back to where it came from, if that is still there."""
+    tokens = (C.c_uint64 * 64)()
+    while n := _native.load().eux_graphs_gone(tokens, 64):
+        for token in tokens[:n]:
+            _, words, owner = _held.pop(token)
+            owner = owner()
+            if owner is not None and words is not None:
+                owner._spare.append(words)
+
+
 class CallScratch:
     """Memory for calls of a kernel: a workspace, and zeroed words that the kernel leaves zeroed. Calls that may run at the
     same time get memory of their own: those of one stream share some, and every captured call has its own, since graphs may
-    be replayed beside each other and beside plain calls."""
+    be replayed beside each other and beside plain calls. ``keep`` is memory of the object's own that its calls use too. A
+    graph keeps it, and the words, for as long as it is there itself, whatever becomes of the object; then others may have them."""
 
     SLOTS = 16
 
-    def __init__(self, words: int, device):
-        self.words, self.device = words, device
+    def __init__(self, words: int, device, keep=()):
+        self.words, self.device, self._keep = words, device, tuple(keep)
         self._of_stream = {}
-        self._captured, self._kept = [], []
+        self._kept = []
         self._lock = threading.Lock()  # two threads that find nothing for their stream must not both make it
         with on_device(device.index):
-            self._spare = list(torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device).unbind(0)) if words else []
+            self._all = torch.zeros(self.SLOTS, words, dtype=torch.int32, device=device) if words else None
+            self._spare = list(self._all.unbind(0)) if words else []
             torch.cuda.current_stream().synchronize()  # captured calls run on any stream
 
     def get(self, need: int):
@@ -103,12 +124,21 @@ class CallScratch:
     def _get(self, need: int):
         stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         if torch._C._cuda_isCurrentStreamCapturing():
-            # In a capture a tensor's memory is the graph's; the words are zeroed by the graph itself once those that were
-            # zeroed beforehand are given out.
+            # In a capture a tensor's memory is the graph's; the words are zeroed by the graph itself where all that were zeroed
+            # beforehand are given out.
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-            words = self._spare.pop() if self._spare else torch.zeros(self.words, dtype=torch.int32, device=self.device)
-            self._captured.append(words)
-            return workspace.data_ptr(), words.data_ptr()
+            _collect()
+            mine = self._spare.pop() if self._spare else None
+            words = mine if mine is not None or not self.words else torch.zeros(self.words, dtype=torch.int32, device=self.device)
+            if mine is not None or self._keep:
+                token = next(_tokens)
+                _held[token] = (self._keep, mine, weakref.ref(self))
+                if rc := _native.load().eux_graph_hold(stream, token):
+                    del _held[token]
+                    if mine is not None:
+                        self._spare.append(mine)
+                    _native.check(rc, "eux_graph_hold")
+            return workspace.data_ptr(), words.data_ptr() if words is not None else 0
         mine = self._of_stream.get(stream)
         if mine is None or mine[2] < need:
             # A smaller workspace may be another thread's, which has yet to launch with it: it is kept. Powers of two: all that are kept come
@@ -123,5 +153,5 @@ class CallScratch:
 
     def reset(self) -> None:
         """Zeroes all words, after a kernel that gave up: with nothing in flight."""
-        for t in [m[1] for m in self._of_stream.values()] + self._captured:
+        for t in [m[1] for m in self._of_stream.values()] + ([self._all] if self.words else []):
             t.zero_()

@@ -25,7 +25,7 @@ class LoraAdapters:
     ``[adapters]``, float32 (1 if not given). They are used where they lie: the object keeps the tensors and copies nothing, so
     an adapter that is written into its place holds for the next call. ``rank`` is a multiple of 8 up to 128, K and N are
     multiples of 8. For inference: the result has no gradient. An object is made outside of graph captures; its calls may be
-    captured, and made by several threads."""
+    captured, and made by several threads. A graph may outlive the object, but not the tensors given here."""
 
     MAX_RANK = 128
 
@@ -45,12 +45,13 @@ class LoraAdapters:
         ws.require_device(self.device, b=b, scale=scale)
         ws.require_cuda(self.device)
         ws.require((a.data_ptr() | b.data_ptr()) % 16 == 0, "a and b must begin on 16 bytes")
-        scale = scale if scale is not None else torch.ones(self.n_adapters, dtype=torch.float32, device=self.device)
+        own = () if scale is not None else (torch.ones(self.n_adapters, dtype=torch.float32, device=self.device),)
+        scale = own[0] if own else scale
         self._weights = (a, b, scale)
         self._weight_ptrs = (a.data_ptr(), b.data_ptr(), scale.data_ptr())
         self._index = self.device.index
         self._need = {}
-        self._scratch = ws.CallScratch(0, self.device)
+        self._scratch = ws.CallScratch(0, self.device, keep=own)
         _native.load()
 
     a = property(lambda self: self._weights[0])

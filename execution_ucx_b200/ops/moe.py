@@ -214,7 +214,8 @@ class MoeExperts:
 
     Made for few tokens, where the layer is as fast as the weights of the named experts can be read: rows beyond
     ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again. For inference: the result has no
-    gradient. An object is made outside of graph captures; its calls may be captured, and made by several threads."""
+    gradient. An object is made outside of graph captures; its calls may be captured, and made by several threads. A graph may
+    outlive the object, but not the weights."""
 
     MAX_TOKENS = 128
     MAX_EXPERTS = 1024
@@ -258,7 +259,7 @@ class MoeExperts:
         self._maps = (C.addressof(self._room) + 63) & ~63
         with ws.on_device(self._index):
             _native.check(lib.eux_experts_maps(self._desc(1, 1), self._maps), "eux_experts_maps")
-        self._scratch = ws.CallScratch(int(lib.eux_experts_counter_words(self._desc(1, 1))), self.device)
+        self._scratch = ws.CallScratch(int(lib.eux_experts_counter_words(self._desc(1, 1))), self.device, keep=(self.status,))
 
     w_gate_up = property(lambda self: self._weights[0])
     w_down = property(lambda self: self._weights[1])
