@@ -36,6 +36,29 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def require_apart(out: torch.Tensor, other: torch.Tensor, name: str) -> None:
+    """That ``out`` is ``other``, row for row, or shares no memory with it. Both are matrices that ``require_rows`` has seen."""
+    a, b = (t.data_ptr() for t in (out, other))
+    (n, wa, sa), (m, wb, sb) = ((t.shape[0], t.shape[1] * t.element_size(), row_stride(t) * t.element_size()) for t in (out, other))
+    if not out.numel() or not other.numel() or a + (n - 1) * sa + wa <= b or b + (m - 1) * sb + wb <= a:
+        return
+    if (a, n, wa) == (b, m, wb) and (sa == sb or n == 1):
+        return
+    if sa == sb:  # columns beside each other, or a row's end within its distance to the next
+        apart = (b - a) % sa
+        shared = apart < wa or apart + wb > sa
+    else:
+        i = j = shared = 0
+        while i < n and j < m and not shared:
+            if a + i * sa + wa <= b + j * sb:
+                i += 1
+            elif b + j * sb + wb <= a + i * sa:
+                j += 1
+            else:
+                shared = 1
+    require(not shared, f"out may be {name} itself, and else must not share memory with it")
+
+
 def require_dense(t: torch.Tensor, name: str, dtype, shape) -> None:
     require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), f"{name} must have the shape {tuple(shape)}")
     require(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")

@@ -60,8 +60,8 @@ class LoraAdapters:
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` is ``[tokens, K]`` and ``y`` ``[tokens, N]``, bfloat16; ``ids`` ``[tokens]``, int32, names each token's adapter. A
-        token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``; the rows
-        of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
+        token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``, but not
+        share a part of its memory; the rows of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
         global _launches
         K, N = self.K, self.N
         # what a call usually brings, with as few questions as tell it from everything else
@@ -81,6 +81,7 @@ class LoraAdapters:
         else:
             ws.require_rows(out, "out", torch.bfloat16, cols=N, rows=t)
             ws.require_device(self.device, out=out)
+            ws.require_apart(out, y, "y")
             os_ = ws.row_stride(out)
         if t == 0:
             return out

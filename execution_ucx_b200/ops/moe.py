@@ -276,7 +276,7 @@ class MoeExperts:
         """``x`` is ``[tokens, hidden]`` bfloat16, ``topk_idx`` (int32) and ``topk_w`` (float32) are ``[tokens, topk]``, up to 32
         per token. An entry whose expert is not in ``[0, experts)`` adds nothing: with the experts of one of several GPUs, pass
         the indices less the number of its first expert, and add up the GPUs' results. A token without entries gets zeros.
-        ``out`` may be ``x`` itself; the rows of both may lie apart. Sums are in float32; what lies between the two products is
+        ``out`` may be ``x`` itself, but beyond ``MAX_TOKENS`` rows not share a part of its memory; the rows of both may lie apart. Sums are in float32; what lies between the two products is
         rounded to bfloat16, or with up to eight tokens, of which no expert has more than four, to two such numbers. The same arguments give the same bits. A wait in the kernels that runs out (two seconds) is told by
         ``check_status``; the result is none then."""
         global _launches
@@ -299,6 +299,8 @@ class MoeExperts:
         else:
             ws.require_rows(out, "out", torch.bfloat16, cols=hidden, rows=t)
             ws.require_device(self.device, out=out)
+            if t > self.MAX_TOKENS:
+                ws.require_apart(out, x, "x")  # a pass reads what the passes before it have not written
             os_ = ws.row_stride(out)
         lib = _native.load()
         for first in range(0, t, self.MAX_TOKENS):

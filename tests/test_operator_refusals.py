@@ -88,6 +88,58 @@ def test_experts_refuse_passes_that_32_bits_cannot_number(native_build):
     assert size(hidden=16384, inner=16384, n_experts=200, n_tokens=128, topk=32, fp8=1) > 0
 
 
+def test_memory_that_a_result_may_share():
+    """Itself row for row, or none: also where rows lie between another's rows."""
+    from execution_ucx_b200.ops import _workspace as ws
+    room = torch.zeros(4096, dtype=torch.bfloat16)
+    rows = lambda first, count, cols, apart: room.as_strided((count, cols), (apart, 1), first)  # noqa: E731
+    y = rows(512, 10, 24, 64)
+    for out in (y, rows(512, 10, 24, 64), rows(536, 10, 40, 64), rows(544, 10, 8, 64), rows(488, 10, 24, 64), rows(0, 10, 24, 48), rows(1112, 10, 24, 64),
+                rows(536, 3, 40, 128), rows(536, 5, 24, 40 + 88), rows(8, 5, 32, 32), torch.zeros(10, 24, dtype=torch.bfloat16)):
+        ws.require_apart(out, y, "y")
+    for out in (rows(520, 10, 24, 64), rows(576, 10, 24, 64), rows(448, 10, 24, 64), rows(536, 10, 48, 64), rows(512, 10, 24, 32), rows(512, 10, 24, 128),
+                rows(512, 10, 16, 64), rows(1104, 10, 24, 64), rows(0, 10, 24, 64), rows(496, 1, 24, 24), rows(536, 2, 24, 48)):
+        with pytest.raises(ValueError, match="share"):
+            ws.require_apart(out, y, "y")
+    one = rows(512, 1, 24, 24)
+    ws.require_apart(rows(512, 1, 24, 8), one, "y")  # one row: the distance of rows says nothing
+    ws.require_apart(rows(536, 1, 24, 8), one, "y")
+    with pytest.raises(ValueError, match="share"):
+        ws.require_apart(rows(528, 1, 24, 8), one, "y")
+
+
+@pytest.mark.gpu
+def test_results_that_share_a_part_of_what_is_read(cuda_device):
+    from execution_ucx_b200.ops import lora, moe
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, device=cuda_device).to(torch.bfloat16)  # noqa: E731
+    ad = lora.LoraAdapters(r(3, 16, 32), r(3, 24, 16))
+    layer = moe.MoeExperts(r(4, 128, 64) * 0.1, r(4, 64, 64) * 0.1)
+    for t in (5, 600):
+        room, x, ids = r(t + 1, 48), r(t, 32), torch.randint(-1, 3, (t,), generator=g, device=cuda_device, dtype=torch.int32)
+        y = room[1:, :24]
+        want = ad(x, ids, y)
+        for bad in (room[:-1, :24], room[1:, 8:32], room.view(-1)[48:].as_strided((t, 24), (24, 1))):
+            with pytest.raises(ValueError, match="share"):
+                ad(x, ids, y, out=bad)
+        assert torch.equal(ad(x, ids, y, out=room[1:, 24:]), want)
+        assert torch.equal(ad(x, ids, y, out=room[1:, :24]), want)
+    for t in (100, 300):
+        room, w = r(t + 1, 128), torch.rand(t, 2, generator=g, device=cuda_device)
+        idx = torch.randint(0, 4, (t, 2), generator=g, device=cuda_device, dtype=torch.int32)
+        x = room[:-1, :64]
+        want = layer(x, idx, w)
+        assert torch.equal(layer(x, idx, w, out=room[:-1, 64:]), want)
+        if t > layer.MAX_TOKENS:  # a later pass would read what an earlier one wrote
+            with pytest.raises(ValueError, match="share"):
+                layer(x, idx, w, out=room[1:, :64])
+        else:
+            assert torch.equal(layer(x.clone(), idx, w), layer(x, idx, w, out=room[1:, :64]))
+        room[:-1, :64] = x0 = r(t, 64)
+        assert torch.equal(layer(x0, idx, w), layer(room[:-1, :64], idx, w, out=room[:-1, :64]))
+    layer.check_status()
+
+
 @pytest.mark.gpu
 def test_calls_refuse(cuda_device):
     from execution_ucx_b200.ops import lora, moe
