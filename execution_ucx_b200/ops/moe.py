@@ -330,6 +330,7 @@ class MoeExperts:
     def check_status(self) -> None:
         s = int(self.status.item())
         if s:
+            torch.cuda.synchronize(self.device)  # calls on other streams still count in the words
             self._scratch.reset()
             self.status.zero_()
             raise RuntimeError(f"moe experts status code={s & 0xff} where={s >> 8}")

@@ -196,3 +196,32 @@ def test_a_graph_outlives_the_object(cuda_device):
         time.sleep(0.001)
         ws._collect()
     assert not held & set(ws._held)
+
+
+@pytest.mark.gpu
+def test_a_call_that_gave_up_is_told_and_leaves_nothing(cuda_device, monkeypatch):
+    """A status word and counts as a kernel leaves them whose wait has run out, here written by hand: told once, when nothing is in flight
+    any more, and the calls that follow, captured ones too, are right."""
+    moe, parts, args = experts(cuda_device)
+    layer = moe.MoeExperts(*parts)
+    want = layer(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(*args)
+    graph.replay()
+    torch.cuda.synchronize()
+    layer.check_status()
+    layer.status.fill_(1 | 2 << 8)
+    layer._scratch._all.fill_(3)
+    for _, words, *_ in layer._scratch._of_stream.values():
+        words.fill_(5)
+    done, whole, zero = [], torch.cuda.synchronize, layer._scratch.reset
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: (done.append("waited"), whole(*a)))
+    monkeypatch.setattr(layer._scratch, "reset", lambda: (done.append("zeroed"), zero()))
+    with pytest.raises(RuntimeError, match="code=1 where=2"):
+        layer.check_status()
+    assert done == ["waited", "zeroed"]
+    layer.check_status()
+    graph.replay()
+    assert torch.equal(layer(*args), want) and torch.equal(out, want)
+    layer.check_status()
