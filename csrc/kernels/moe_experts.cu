@@ -812,7 +812,8 @@ __global__ void __launch_bounds__(kXpThreads, 1) moe_experts_kernel(const __grid
   if (p.tables) {
     const uint4* const from = reinterpret_cast<const uint4*>(p.tables + 4);
     for (int i = threadIdx.x; i < xp_table_bytes(d.n_experts, entries) / 16; i += kXpThreads) reinterpret_cast<uint4*>(xp_smem + l.tables)[i] = __ldcg(from + i);
-    r.named = (int)__ldcg(p.tables), cap = (int)__ldcg(p.tables + 1), r.most = (int)__ldcg(p.tables + 2);
+    const uint4 head = ld_cg_u4(p.tables);
+    r.named = (int)head.x, cap = (int)head.y, r.most = (int)head.z;
     __syncthreads();
   } else {
     cap = xp_route(d, p.token_of, FP8 ? 32 : kXpAccColumns, r, reinterpret_cast<int*>(xp_smem), s_route);
