@@ -748,7 +748,8 @@ struct XpResults {
             v[i] = reinterpret_cast<const float2*>(sum + (pairs ? 2 * j : j) * kXpLd)[tid], w[i] = r.weight[s.pos + j], t[i] = r.token[s.pos + j];
             if (pairs) {
               const float2 u = reinterpret_cast<const float2*>(sum + (2 * j + 1) * kXpLd)[tid];
-              v[i].x += u.x, v[i].y += u.y;
+              // an infinite weight is met by the first of the two: zero, or the other sign, in the second would make it NaN
+              v[i].x += isfinite(u.x) ? u.x : 0.f, v[i].y += isfinite(u.y) ? u.y : 0.f;
             }
           }
 #pragma unroll

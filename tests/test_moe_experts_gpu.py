@@ -447,3 +447,46 @@ def test_route_dispatch_experts_combine(cuda_device, fp8_rows):
         # the whole layer on one GPU says the same
         whole = moe.MoeExperts(gu, down)(xs[r], idx, w)
         assert bool(((got.double() - whole.double()).abs() <= 2 * tol).all())
+
+
+@pytest.mark.parametrize("t,k,h,what", [(1, 2, 256, "bf16"), (8, 1, 144, "bf16"), (9, 1, 256, "bf16"), (40, 3, 256, "bf16"), (128, 2, 144, "bf16"),
+                                        (1, 2, 256, "scale"), (8, 1, 144, "scale"), (40, 3, 256, "scale")])
+def test_infinities_in_the_weights(cuda_device, t, k, h, what):
+    """A weight (or a block's scale) that is infinite makes infinities, and NaN only where the formula does, whatever the number of tokens."""
+    from execution_ucx_b200.ops import moe
+    i, e, inf = 256, 4, float("inf")
+    gu, down, gus, ds = weights(e, h, i, what == "scale", cuda_device)
+    x = torch.randn(t, h, device=cuda_device).abs().to(torch.bfloat16)
+    idx, w = routing(t, k, e, cuda_device, 5)
+    idx[:, 0] = torch.arange(1, t + 1, device=cuda_device) % e  # the second expert first: one token meets an infinity
+    if what == "bf16":
+        gu[:, 7], gu[:, i + 7] = 0.125, 0.125  # h[7] is well above zero for every token, and so is h[200]
+        gu[:, 200], gu[:, i + 200] = 0.25, 0.125
+        gu[2, 9] = gu[2, i + 9] = 0            # and h[9] of the third expert is zero
+        down[0, 3, 7], down[1, 5, 7], down[1, 5, 200], down[1, 6, 7] = inf, inf, -inf, -inf
+        down[2, 8, 9], down[2, 11, 7], down[3, 12, 7] = inf, -inf, float("nan")
+    else:
+        gu.view(torch.uint8)[:] = gu.view(torch.uint8) & 0x7f  # all is positive: h, and with an infinite scale what it makes
+        down.view(torch.uint8)[:] = (down.view(torch.uint8) & 0x7f).clamp(min=1)
+        ds[1, 0, 0], ds[2, (h - 1) // 128, 1] = inf, -inf
+    layer = moe.MoeExperts(gu, down, gus, ds)
+    out = layer(x, idx, w).double()
+    torch.cuda.synchronize()
+    layer.check_status()
+    want = moe.reference_experts(x, idx, w, gu, down, gus, ds)
+    clean = lambda v: v if v is None else torch.where(v.float().isfinite(), v, 0.0) if what == "bf16" else v  # noqa: E731
+    _, tol = plain(x, idx, w, clean(gu), clean(down), gus, ds if ds is None else torch.where(ds.isfinite(), ds, 0.0))
+    fine = want.isfinite()
+    assert bool(want.isinf().any()) and torch.equal(out.isnan(), want.isnan()) and torch.equal(out[want.isinf()], want[want.isinf()])
+    assert bool(((out - want).abs()[fine] <= tol[fine]).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_as_many_experts_and_entries_as_there_may_be(cuda_device, fp8):
+    from execution_ucx_b200.ops import moe
+    layer = moe.MoeExperts(*weights(1024, 64, 32, fp8, cuda_device))
+    x = torch.randn(128, 64, device=cuda_device).to(torch.bfloat16)
+    check(layer, x, *routing(128, 32, 1024, cuda_device, 3))
+    idx, w = routing(128, 32, 1024, cuda_device, 4)
+    idx[:, :] = 1023
+    check(layer, x, idx, w)
