@@ -13,7 +13,8 @@ namespace eux {
 
 struct GraphNotes {
   std::mutex lock;
-  std::vector<uint64_t> gone;
+  std::vector<uint64_t> gone;  // with room for all that are held: the destructor must not fail
+  size_t held = 0;
 };
 static GraphNotes& graph_notes() {
   static GraphNotes* const notes = new GraphNotes;  // never destroyed: graphs may be, while the process ends
@@ -23,6 +24,7 @@ static void CUDART_CB graph_is_gone(void* token) {
   GraphNotes& notes = graph_notes();
   std::lock_guard<std::mutex> lock(notes.lock);
   notes.gone.push_back((uint64_t)(uintptr_t)token);
+  --notes.held;
 }
 
 }  // namespace eux
@@ -35,10 +37,25 @@ extern "C" int eux_graph_hold(void* stream, uint64_t token) {
   cudaGraph_t graph = nullptr;
   if (cudaError_t e = cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id, &graph); e != cudaSuccess) return (int)e;
   if (status != cudaStreamCaptureStatusActive || !graph) return EUX_ERR_BAD_ARG;
+  GraphNotes& notes = graph_notes();
+  {
+    std::lock_guard<std::mutex> lock(notes.lock);
+    try {
+      const size_t need = notes.gone.size() + notes.held + 1;
+      if (notes.gone.capacity() < need) notes.gone.reserve(2 * need);
+    } catch (...) {
+      return EUX_ERR_TOO_LARGE;
+    }
+    ++notes.held;
+  }
   cudaUserObject_t object;
-  if (cudaError_t e = cudaUserObjectCreate(&object, (void*)(uintptr_t)token, graph_is_gone, 1, cudaUserObjectNoDestructorSync); e != cudaSuccess) return (int)e;
+  if (cudaError_t e = cudaUserObjectCreate(&object, (void*)(uintptr_t)token, graph_is_gone, 1, cudaUserObjectNoDestructorSync); e != cudaSuccess) {
+    std::lock_guard<std::mutex> lock(notes.lock);
+    --notes.held;
+    return (int)e;
+  }
   const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-  if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+  if (e != cudaSuccess) cudaUserObjectRelease(object, 1);  // its destructor leaves the note all the same
   return (int)e;
 }
 

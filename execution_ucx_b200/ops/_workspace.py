@@ -111,8 +111,8 @@ def _collect() -> None:
     tokens = (C.c_uint64 * 64)()
     while n := _native.load().eux_graphs_gone(tokens, 64):
         for token in tokens[:n]:
-            _, words, owner = _held.pop(token)
-            owner = owner()
+            _, words, owner = _held.pop(token, (None, None, None))  # none: the hold failed
+            owner = owner and owner()
             if owner is not None and words is not None:
                 owner._spare.append(words)
 
@@ -157,8 +157,7 @@ class CallScratch:
                 token = next(_tokens)
                 _held[token] = (self._keep, mine, weakref.ref(self))
                 if rc := _native.load().eux_graph_hold(stream, token):
-                    del _held[token]
-                    if mine is not None:
+                    if _held.pop(token, None) and mine is not None:
                         self._spare.append(mine)
                     _native.check(rc, "eux_graph_hold")
             return workspace.data_ptr(), words.data_ptr() if words is not None else 0
