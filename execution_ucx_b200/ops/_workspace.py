@@ -169,6 +169,9 @@ class CallScratch:
             words = mine[1] if mine else torch.zeros(self.words, dtype=torch.int32, device=self.device)
             if mine:
                 self._kept.append(mine[0])
+            else:
+                for t in self._keep:  # made on another stream, perhaps, where it is not free before this one is done with it
+                    t.record_stream(torch.cuda.current_stream())
             workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
             mine = self._of_stream[stream] = (workspace, words, need, (workspace.data_ptr(), words.data_ptr()))
         return mine[3]

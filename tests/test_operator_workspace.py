@@ -225,3 +225,22 @@ def test_a_call_that_gave_up_is_told_and_leaves_nothing(cuda_device, monkeypatch
     graph.replay()
     assert torch.equal(layer(*args), want) and torch.equal(out, want)
     layer.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [12, 600])
+def test_an_object_dropped_while_its_call_on_another_stream_is_under_way(cuda_device, t):
+    from execution_ucx_b200.ops import lora
+    a, b = (torch.randn(*s, device=cuda_device).to(torch.bfloat16) for s in ((3, 16, 256), (3, 256, 16)))
+    x, y = (torch.randn(t, 256, device=cuda_device).to(torch.bfloat16) for _ in range(2))
+    ids = torch.randint(-1, 3, (t,), device=cuda_device, dtype=torch.int32)
+    want = lora.LoraAdapters(a, b, torch.ones(3, device=cuda_device))(x, ids, y)
+    adapters, side = lora.LoraAdapters(a, b), torch.cuda.Stream()  # scales of one, made by the object, on this stream
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # the call's kernels begin some ten milliseconds later
+        out = adapters(x, ids, y)
+    del adapters
+    others = [torch.full((3,), 7.0, device=cuda_device) for _ in range(50)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and all(bool((o == 7).all()) for o in others)
