@@ -22,8 +22,9 @@ def launch_count() -> int:
 
 class LoraAdapters:
     """The adapters of one projection: ``a`` ``[adapters, rank, K]`` and ``b`` ``[adapters, N, rank]``, bfloat16, and ``scale``
-    ``[adapters]``, float32 (1 if not given). They are used where they lie: the object keeps the tensors and copies nothing, so
-    an adapter that is written into its place holds for the next call. ``rank`` is a multiple of 8 up to 128, K and N are
+    ``[adapters]``, float32 (1 if not given). They are used where they lie: the object keeps their memory and copies nothing, so
+    an adapter that is written into its place holds for the next call (a parameter whose ``data`` is set to other memory leaves the
+    object with what it was given). ``rank`` is a multiple of 8 up to 128, K and N are
     multiples of 8. For inference: the result has no gradient. An object is made outside of graph captures; its calls may be
     captured, and made by several threads. A graph may outlive the object, but not the tensors given here."""
 
@@ -47,7 +48,7 @@ class LoraAdapters:
         ws.require((a.data_ptr() | b.data_ptr()) % 16 == 0, "a and b must begin on 16 bytes")
         own = () if scale is not None else (torch.ones(self.n_adapters, dtype=torch.float32, device=self.device),)
         scale = own[0] if own else scale
-        self._weights = (a, b, scale)
+        self._weights = (a.detach(), b.detach(), scale.detach())  # the memory, whatever becomes of the tensors: a parameter's may be exchanged
         self._weight_ptrs = (a.data_ptr(), b.data_ptr(), scale.data_ptr())
         self._index = self.device.index
         self._need = {}

@@ -208,9 +208,10 @@ class MoeExperts:
     ``w_gate_up`` is ``[experts, 2 * inner, hidden]`` (gate rows, then up rows) and ``w_down`` ``[experts, hidden, inner]``,
     both bfloat16, or both float8_e4m3fn with float32 scales of 128 x 128 blocks: ``gate_up_scale`` ``[experts,
     ceil(2 * inner / 128), ceil(hidden / 128)]`` and ``down_scale`` ``[experts, ceil(hidden / 128), ceil(inner / 128)]`` (what
-    ``remote_gemm.quantize_blocks_128x128`` gives for each expert). They are used where they lie: the object keeps the tensors
-    and copies nothing, so what is written into them holds for the next call. ``hidden`` and ``inner`` are multiples of 8
-    (16 for e4m3), e4m3 weights no NaN (checked when they are given).
+    ``remote_gemm.quantize_blocks_128x128`` gives for each expert). They are used where they lie: the object keeps their memory
+    and copies nothing, so what is written into it holds for the next call (a parameter whose ``data`` is set to other memory leaves
+    the object with what it was given). ``hidden`` and ``inner`` are multiples of 8 (16 for e4m3). e4m3 weights are no NaN, which is checked
+    when they are given and not again: one that is written later counts as 480.
 
     Made for few tokens, where the layer is as fast as the weights of the named experts can be read: rows beyond
     ``MAX_TOKENS`` go in passes of that many, each of which reads its experts again. For inference: the result has no
@@ -242,7 +243,8 @@ class MoeExperts:
         ws.require_device(self.device, w_gate_up=w_gate_up, gate_up_scale=gate_up_scale, down_scale=down_scale)
         ws.require_cuda(self.device)
         ws.require((w_gate_up.data_ptr() | w_down.data_ptr()) % 16 == 0, "weights must begin on 16 bytes")
-        self._weights = (w_gate_up, w_down, gate_up_scale, down_scale)
+        # the memory, whatever becomes of the tensors: a parameter's may be exchanged
+        self._weights = tuple(w.detach() if w is not None else None for w in (w_gate_up, w_down, gate_up_scale, down_scale))
         self._weight_ptrs = tuple(w.data_ptr() if w is not None else 0 for w in self._weights)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status_ptr, self._index = self.status.data_ptr(), self.device.index

@@ -244,3 +244,28 @@ def test_an_object_dropped_while_its_call_on_another_stream_is_under_way(cuda_de
     others = [torch.full((3,), 7.0, device=cuda_device) for _ in range(50)]
     torch.cuda.synchronize()
     assert torch.equal(out, want) and all(bool((o == 7).all()) for o in others)
+
+
+@pytest.mark.gpu
+def test_parameters_that_are_given_other_memory(cuda_device):
+    """The object keeps the memory it was given, also where a parameter's ``data`` is set to other memory, as moving a module does."""
+    from execution_ucx_b200.ops import lora
+    moe, parts, args = experts(cuda_device)
+    given = [torch.nn.Parameter(p) for p in parts[:2]]
+    a, b = (torch.nn.Parameter(torch.randn(*s, device=cuda_device).to(torch.bfloat16)) for s in ((3, 16, 256), (3, 256, 16)))
+    scale = torch.nn.Parameter(torch.rand(3, device=cuda_device))
+    ids = torch.randint(-1, 3, (12,), device=cuda_device, dtype=torch.int32)
+    layer, adapters = moe.MoeExperts(*given), lora.LoraAdapters(a, b, scale)
+    want = adapters(args[0], ids, layer(*args))
+    del parts
+    for p in (*given, a, b, scale):
+        p.data = torch.zeros_like(p)
+    others = [torch.full_like(p, 3.0) for p in (*given, a, b, scale) for _ in range(3)]
+    assert torch.equal(adapters(args[0], ids, layer(*args)), want)
+    assert all(bool((o == 3).all()) for o in others)
+    layer.w_down.mul_(2)  # the memory that is used
+    got = layer(*args)
+    from test_moe_experts_gpu import plain
+    want, tol = plain(*args, layer.w_gate_up, layer.w_down)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    assert not layer.w_down.requires_grad and not got.requires_grad
