@@ -17,11 +17,13 @@
 //   atomics.
 //   lora_expand: a warp has 16 tokens and runs over a part of N. v is its first operand, two bfloat16 numbers that add up to it (what is
 //   lost is 2^-16 of it, nothing beside the result's rounding), made in registers. y and B go through a ring of stages with cp.async: B
-//   for all four warps, of y a lane fetches what it will need itself.
+//   for all four warps, of y a lane fetches what it will need itself. Sums that are no numbers are made again in float32, so that an adapter's
+//   infinities give with tiles what they give without.
 //
-// Measured, in a graph: one token, 4096 x 4096, rank 16: 3.8 us; 64 tokens, 8192 x 8192, rank 16, an adapter each: 11.5 us; 777 tokens, 7168 x
-// 2056, rank 40: 18.2 us (3.6 at the measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 85.6
-// us (62 at the copy rate).
+// Measured, in a graph: one token, 4096 x 4096, rank 16: 4.1 us; 64 tokens, 8192 x 8192, rank 16, about 40 adapters: 9.9 us, with an adapter each
+// 11.5 (most of expand's CTAs find no room beside shrink's, and fetch B only then); 777 tokens, 7168 x 2056, rank 40: 17.6 us (3.8 at the
+// measured copy rate; order 2.5, the rest the two kernels' latency); 8192 tokens, 8192 x 8192, rank 16: 86.7 us (62 at the copy rate); 4096 x
+// 4096, rank 64: 67.5 us (32), rank 128: 108.6 (32): A and B come through the L2 for every tile of 64 tokens, and expand multiplies twice.
 #include <algorithm>
 #include <mutex>
 
@@ -34,7 +36,7 @@ constexpr int64_t kLoraPlainBytes = int64_t(128) << 20;  // ... if the adapters 
 constexpr int64_t kLoraSharedBytes = int64_t(48) << 20;  // or this where more than four tokens must share one on average
 constexpr int kLoraTile = 64;         // tokens of a tile, with more
 constexpr int kLoraThreads = 128;
-constexpr int kLoraColumns = 128;     // of N in a stage of expand (8192 tokens, 4096 x 4096, rank 64: 66.9 us, 70.0 with 64 columns and three or four stages)
+constexpr int kLoraColumns = 128;     // of N in a stage of expand (8192 tokens, 4096 x 4096, rank 64: 67.5 us, 3 more with 64 columns and three or four stages)
 constexpr int kLoraMaxSlices = 8;     // parts of K of a token, each of a CTA
 constexpr int kLoraCluster = 8;       // parts of K of a tile at most
 
@@ -633,7 +635,8 @@ static LoraShape lora_shape(const eux_lora_desc* d) {
     // Parts of K and of N that the SMs have places for at once: a second wave that is half empty costs as much as a full one.
     // How many tiles there will be is not known here: the tokens', and half a tile for each adapter, taken to be a dozen at most (1500 tokens of
     // 16 adapters, 2048 x 6144, rank 32: 21.2 us, 24.0 without; with every adapter that is there counted 4096 tokens of 9 of 64, 8192 x 8192, rank
-    // 16, took 58 us, 49 so).
+    // 16, took 58 us, 49 so; it costs where few tokens name many: 256 tokens of 64 adapters, 8192 x 8192, rank 16, in tiles 27.6 us, 24.2 with 16
+    // for the dozen).
     const int likely = (d->n_tokens + kLoraTile - 1) / kLoraTile + std::min({d->n_adapters, d->n_tokens / 16, 12}) / 2, r = d->rank;
     auto places = [](int smem) { return kSms * (227 * 1024 / (smem + 1024)); };
     const int shrink = places(r <= 8 ? LoraShrink<1, false>::BYTES : r <= 16 ? LoraShrink<2, false>::BYTES : r <= 32 ? LoraShrink<4, false>::BYTES

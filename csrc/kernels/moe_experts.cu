@@ -20,17 +20,19 @@
 //   token is a column of every product), more are put into the experts' order by a kernel in front, once for both forms.
 // * The weights are the first operand, 128 rows of them, and the tokens the second: a token costs a column and not a row.
 //   With few tokens, and with e4m3 weights, that is mma.sync m16n8k16, whose 8 columns are the smallest padding for one token and whose
-//   operands go through registers, where e4m3 weights are widened to the tokens' bfloat16, exactly (see widen). With bfloat16 weights and
-//   more than kXpFewColumns tokens of an expert it is tcgen05, straight from the stages into TMEM.
+//   operands go through registers, where e4m3 weights are widened to the tokens' bfloat16, exactly (see widen). With bfloat16 weights, where
+//   an expert of the call has more than kXpFewColumns tokens, it is tcgen05 for all of them, straight from the stages into TMEM.
 //
 // At 16 KiB per 0.37 us and SM (the share of the measured copy bandwidth) an SM has 700 clocks for a block. Measured, in a graph, of
-// the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 423 us (0.99), e4m3 252 us (0.83); one
-// token, 8 experts of that size: 116 us (0.93) and 78 us (0.69); one token, 8 experts of 2048 x 768, bf16: 24 us (0.48: two launches'
-// beginnings and ends are half of it); 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 162 us (0.76), e4m3 195 us (0.32: widening
-// and mma.sync are the bound, 32 tokens to an expert).
+// the measured copy bandwidth (6550 GB/s): 128 tokens, 31 of 32 experts of 7168 x 2048: bf16 426 us (0.98), e4m3 266 us (0.78); one
+// token, 8 experts of that size: 117 us (0.92) and 79 us (0.68); one token, 8 experts of 2048 x 768, bf16: 27 us (0.43: two launches'
+// beginnings and ends are half of it, since the down form's CTAs, which ask for all of an SM's shared memory, find no room beside the up form's);
+// 128 tokens, top-4 of 16 experts of 4096 x 2048: bf16 160 us (0.77), e4m3 193 us (0.32: widening and mma.sync are the bound, 32 tokens to an
+// expert).
 //
 // Sums are float32 throughout. h is rounded to bfloat16, which its product takes: a relative error of up to 2^-8 in each term of a sum, on
-// average as much as the result's own rounding. With few tokens the product has columns to spare, and h is two such numbers (xp_pairs).
+// average as much as the result's own rounding. With few tokens the product has columns to spare, and h is two such numbers (xp_pairs). So a
+// token's last bits depend on what else is in the call.
 #include <cuda.h>
 
 #include <algorithm>
@@ -51,7 +53,7 @@ template <bool TC>
 constexpr int kXpEndThreads = TC ? 128 : 64;
 constexpr int kXpAccColumns = 64;                   // of TMEM: the tokens of a segment at most
 constexpr int kXpFewTokens = 8;                     // of a call: used where they lie if their rows allow it, and h may be two numbers (xp_pairs)
-constexpr int kXpFewColumns = 16;                   // bfloat16 weights: up to so many tokens of an expert are multiplied with mma.sync
+constexpr int kXpFewColumns = 16;                   // bfloat16 weights: calls with up to so many tokens of any expert are multiplied with mma.sync
 constexpr int kXpRows = 128;                        // rows of weights in a block
 constexpr int kXpBlock = kXpRows * 128;             // bytes of a block: 128 of K per row
 constexpr int kXpMaxStages = 13;

@@ -62,7 +62,10 @@ class LoraAdapters:
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, y: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x`` is ``[tokens, K]`` and ``y`` ``[tokens, N]``, bfloat16; ``ids`` ``[tokens]``, int32, names each token's adapter. A
         token whose id is not in ``[0, adapters)`` has none: its row of ``out`` is that of ``y``. ``out`` may be ``y``, but not
-        share a part of its memory; the rows of all three may lie apart. Everything is computed in float32 and rounded once; the same arguments give the same bits."""
+        share a part of its memory; the rows of all three may lie apart. Sums are of float32 and the
+        result is rounded once. With few tokens nothing is rounded between; with many, which go in tiles of an adapter, ``A x`` is taken as two
+        bfloat16 numbers, which lose 2^-16 of it: a token's last bits may depend on how many tokens and adapters there are. The same
+        arguments give the same bits."""
         global _launches
         K, N = self.K, self.N
         # what a call usually brings, with as few questions as tell it from everything else

@@ -278,9 +278,10 @@ class MoeExperts:
         """``x`` is ``[tokens, hidden]`` bfloat16, ``topk_idx`` (int32) and ``topk_w`` (float32) are ``[tokens, topk]``, up to 32
         per token. An entry whose expert is not in ``[0, experts)`` adds nothing: with the experts of one of several GPUs, pass
         the indices less the number of its first expert, and add up the GPUs' results. A token without entries gets zeros.
-        ``out`` may be ``x`` itself, but beyond ``MAX_TOKENS`` rows not share a part of its memory; the rows of both may lie apart. Sums are in float32; what lies between the two products is
-        rounded to bfloat16, or with up to eight tokens, of which no expert has more than four, to two such numbers. The same arguments give the same bits. A wait in the kernels that runs out (two seconds) is told by
-        ``check_status``; the result is none then."""
+        ``out`` may be ``x`` itself, but beyond ``MAX_TOKENS`` rows not share a part of its memory; the rows of both may lie apart.
+        Sums are in float32; what lies between the two products is rounded to bfloat16, or with up to eight tokens, of which no expert
+        has more than four, to two such numbers: a token's last bits may depend on what else is in the call. The same arguments give
+        the same bits. A wait in the kernels that runs out (two seconds) is told by ``check_status``; the result is none then."""
         global _launches
         index, hidden = self._index, self.hidden
         # what a call usually brings, with as few questions as tell it from everything else
